@@ -16,16 +16,44 @@ from .ops import (
     prepare_metadata_and_plan,
     weighted_scatter_add,
 )
+from .quantize import (
+    CompressedRows,
+    Int8NormedRows,
+    Int8Weights,
+    QuantizedRows,
+    add_rms_norm,
+    add_rms_norm_int8,
+    compress_rows,
+    gelu_compress,
+    gelu_compressed_backward,
+    int8_linear,
+    quantize_rows,
+    quantize_weights,
+    restore_rows,
+)
 
 __all__ = [
+    "CompressedRows",
     "GroupedMetadata",
     "GroupedWeightedScatterAdd",
+    "Int8NormedRows",
+    "Int8Weights",
     "MoEFeedForward",
     "MoEImplementation",
     "PermutedTokens",
+    "QuantizedRows",
+    "add_rms_norm",
+    "add_rms_norm_int8",
+    "compress_rows",
     "compute_experts",
     "gate_and_sort",
+    "gelu_compress",
+    "gelu_compressed_backward",
+    "int8_linear",
     "permute_tokens",
+    "quantize_rows",
+    "quantize_weights",
+    "restore_rows",
     "unpermute",
     "build_plan",
     "grouped_weighted_scatter_add",

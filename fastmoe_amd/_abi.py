@@ -19,11 +19,13 @@ ABI_VERSION = 2
 F32, BF16, F16, I64, I32 = 0, 1, 2, 3, 4
 MODE_DET, MODE_ATOMIC, MODE_ATOMIC_PACKED, MODE_DET_STEP = 0, 1, 2, 3
 STREAM_OUT_BYTES = 96 << 20  # FMOE_STREAM_OUT_BYTES
+ACT_NONE, ACT_GELU = 0, 1  # enum fmoe_activation
 OK, EINVAL, EHIP, ERANGE = 0, -1, -2, -3
 
 _c_i64 = ctypes.c_int64
 _c_int = ctypes.c_int
 _c_vp = ctypes.c_void_p
+_c_f32 = ctypes.c_float
 
 # name -> (restype, argtypes); exactly the symbols of include/fastmoe_amd.h
 SIGNATURES: dict[str, tuple] = {
@@ -106,6 +108,36 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_vp, _c_int, _c_vp, _c_int, _c_i64, _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp,
          _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_add_rms_norm": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_i64, _c_i64, _c_int, _c_f32, _c_vp, _c_vp,
+         _c_vp, _c_vp, _c_i64, _c_vp, _c_vp],
+    ),
+    "fmoe_add_rms_norm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64]),
+    "fmoe_add_rms_norm_backward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_int, _c_vp, _c_i64, _c_i64, _c_int,
+         _c_vp, _c_vp, _c_vp, _c_i64, _c_vp],
+    ),
+    "fmoe_quantize_rows": (
+        _c_int,
+        [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_int, _c_vp, _c_i64, _c_vp, _c_vp],
+    ),
+    "fmoe_compress_rows": (
+        _c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_restore_rows": (
+        _c_int, [_c_vp, _c_i64, _c_vp, _c_i64, _c_i64, _c_i64, _c_vp, _c_int, _c_vp],
+    ),
+    "fmoe_gelu_compressed_backward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_int8_linear": (
+        _c_int,
+        [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_vp],
     ),
 }
 

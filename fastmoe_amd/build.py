@@ -25,7 +25,8 @@ LIB_PATH = PKG / LIB_NAME
 HOST_EXT_SOURCE = "host_ext.cpp"
 
 HIP_SOURCES = ["metadata.hip", "plan.hip", "plan_bucket.hip", "plan_radix.hip", "combine_fwd.hip",
-               "combine_bwd.hip", "permute.hip", "noalloc.hip"]
+               "combine_bwd.hip", "permute.hip", "noalloc.hip", "norm_quantize.hip", "hold.hip",
+               "int8_linear.hip"]
 HOST_SOURCES = ["abi.cpp"]
 
 ARCH = "gfx950"

@@ -83,6 +83,12 @@ enum fmoe_mode {
 };
 #define FMOE_STREAM_OUT_BYTES (96ll << 20)
 
+/* What is applied to a value before it is held in 8 bits. */
+enum fmoe_activation {
+  FMOE_ACT_NONE = 0,
+  FMOE_ACT_GELU = 1 /* x * Phi(x), the exact form (not the tanh approximation) */
+};
+
 enum fmoe_status {
   FMOE_OK = 0,
   FMOE_EINVAL = -1,   /* bad argument (null pointer, size, dtype, alignment, layout) */
@@ -417,6 +423,89 @@ FMOE_API int fmoe_permute(const void* d_expert_ids, int id_dtype, const void* d_
                  const void* d_x, int64_t x_row_stride_bytes, int64_t* d_counts,
                  int64_t* d_offsets, int64_t* d_rev, void* d_sorted_gates, int32_t* d_slot_pos,
                  int32_t* d_status, void* d_out, void* d_workspace, void* stream);
+
+/*
+ * Rows in 8 bits (the MoE layer's serving path, and activations held for a training step's backward).
+ *
+ * A value v is held as q = rint(v * (127 / m)) with the scale s = m / 127, m the largest |v| of the
+ * values that share it: a whole row, or a block of 128 columns of one.  Values below 2^-118 only:
+ * s = 0, q = 0.  An infinity or a NaN among them: s = NaN, q = 0.  Rows of q start at multiples of
+ * 16 bytes, q_stride bytes apart, and are padded with zeros to whole pieces of 128 columns.
+ * There is no counterpart in the reference, whose layer has neither a norm's fusion nor 8 bits.
+ */
+
+/*
+ * Residual's addition and root-mean-square norm of `rows` rows:
+ *     h = x + residual (rounded to `dtype`; without a residual, h is x and is not written)
+ *     y = h * w / sqrt(mean(h^2) + eps)
+ * d_residual, d_h (needed with a residual), d_y, d_rstd (fp32[rows], 1 / sqrt(mean + eps), which the
+ * backward reads) and d_q with d_scales (fp32[rows]; y in 8 bits, one scale a row, from the unrounded y)
+ * may be null.  h and y are packed.  weight_dtype: `dtype` or FMOE_F32.  Strides in elements.  d_h may
+ * be d_x's or d_residual's own memory if that is packed.
+ */
+FMOE_API int fmoe_add_rms_norm(const void* d_x, int64_t x_row_stride, const void* d_residual,
+                               int64_t residual_row_stride, const void* d_weight, int weight_dtype,
+                               int64_t rows, int64_t cols, int dtype, float eps, void* d_h,
+                               void* d_y, float* d_rstd, void* d_q, int64_t q_stride,
+                               float* d_scales, void* stream);
+
+/*
+ * Its backward: d_grad_x[rows, cols] (packed), the gradient of x and of the residual alike, and
+ * d_grad_w[cols] in weight_dtype (null where not wanted; else d_workspace holds at least
+ * fmoe_add_rms_norm_backward_workspace_bytes(rows, cols) bytes at a multiple of 16).  d_grad_h, the
+ * gradient that comes through h, may be null.  Sums run in a fixed order.
+ */
+FMOE_API int64_t fmoe_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols);
+FMOE_API int fmoe_add_rms_norm_backward(const void* d_grad_y, int64_t gy_row_stride,
+                                        const void* d_grad_h, int64_t gh_row_stride,
+                                        const void* d_h, int64_t h_row_stride, const void* d_weight,
+                                        int weight_dtype, const float* d_rstd, int64_t rows,
+                                        int64_t cols, int dtype, void* d_grad_x, void* d_grad_w,
+                                        void* d_workspace, int64_t workspace_bytes, void* stream);
+
+/* Rows to 8 bits with one scale each (d_scales: fp32[rows]), after an activation (fmoe_activation). */
+FMOE_API int fmoe_quantize_rows(const void* d_x, int64_t x_row_stride, int64_t rows, int64_t cols,
+                                int dtype, int activation, void* d_q, int64_t q_stride,
+                                float* d_scales, void* stream);
+
+/*
+ * Rows to 8 bits with a scale for every 128 columns (d_scales: fp32[rows, ceil(cols / 128)]), and, where
+ * d_gelu is not null, gelu(x) of the exact x (packed, in `dtype`).
+ */
+FMOE_API int fmoe_compress_rows(const void* d_x, int64_t x_row_stride, int64_t rows, int64_t cols,
+                                int dtype, void* d_q, int64_t q_stride, float* d_scales,
+                                void* d_gelu, void* stream);
+
+/* q * s, packed: with one scale per row or one for every 128 columns (scales_per_row). */
+FMOE_API int fmoe_restore_rows(const void* d_q, int64_t q_stride, const float* d_scales,
+                               int64_t scales_per_row, int64_t rows, int64_t cols, void* d_out,
+                               int dtype, void* stream);
+
+/*
+ * GELU's backward from fmoe_compress_rows' rows: with x' = q * s, d_grad = grad_a * gelu'(x') and, where
+ * d_again is not null, gelu(x') (what the next weights' gradient reads).  Both packed.
+ */
+FMOE_API int fmoe_gelu_compressed_backward(const void* d_q, int64_t q_stride, const float* d_scales,
+                                           const void* d_grad_a, int64_t grad_row_stride,
+                                           int64_t rows, int64_t cols, int dtype, void* d_again,
+                                           void* d_grad, void* stream);
+
+/*
+ * Every expert's product on its own rows in 8-bit integers:
+ *     out[r, n] = (sum_k x[i(r), k] * w[e, n, k]) * sx[i(r)] * sw[e, n] + bias[e, n]
+ * for r in [offsets[e], offsets[e + 1]), offsets[0] read as 0.  i(r) is d_index[r] (int64 or int32), or
+ * r where d_index is null.  d_x: rows as above with one scale each (x_row_stride bytes apart); d_w:
+ * [E, N, Kp] with Kp = K rounded up to 128, zeros from K on, d_w_scales fp32[E, N]; d_bias [E, N] or null.
+ * d_offsets: int64[E + 1] on the device, or null for one expert.  Sums are exact int32 (K <= 131071).
+ * Rows at or beyond offsets[E] are written as zero; a row whose index lies outside [0, x_rows) has
+ * a product of zero.
+ */
+FMOE_API int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows,
+                              const float* d_x_scales, const void* d_index, int index_dtype,
+                              const void* d_w, const float* d_w_scales, const void* d_bias,
+                              int bias_dtype, const int64_t* d_offsets, int64_t num_experts,
+                              int64_t N, int64_t K, int64_t rows, void* d_out,
+                              int64_t out_row_stride, int out_dtype, void* stream);
 
 #ifdef __cplusplus
 }

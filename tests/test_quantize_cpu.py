@@ -1,0 +1,114 @@
+"""Refusals of the 8-bit operators and their C entry points (CPU: nothing is launched)."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import fastmoe_amd as fm
+from fastmoe_amd import _abi
+
+DEV = 0x10000  # stands for a device address: every call here is refused before a launch
+
+
+def test_cpu_tensors_raise():
+    x, w = torch.zeros(2, 8), torch.ones(8)
+    q = fm.QuantizedRows(torch.zeros(2, 128, dtype=torch.int8), torch.ones(2), 8)
+    held = fm.CompressedRows(torch.zeros(2, 128, dtype=torch.int8), torch.ones(2, 1), 8)
+    for call in (lambda: fm.add_rms_norm(x, w), lambda: fm.add_rms_norm_int8(x, w, x),
+                 lambda: fm.quantize_rows(x), lambda: fm.quantize_weights([x]),
+                 lambda: fm.compress_rows(x), lambda: fm.gelu_compress(x),
+                 lambda: q.dequantize(), lambda: fm.restore_rows(held, torch.float32),
+                 lambda: fm.gelu_compressed_backward(held, x),
+                 lambda: fm.int8_linear(q, fm.Int8Weights(q.data, q.scales, 8))):
+        with pytest.raises(RuntimeError, match="only on the GPU"):
+            call()
+
+
+def _norm(x=DEV, xs=8, r=None, w=DEV, wd=_abi.BF16, rows=4, cols=8, dt=_abi.BF16, h=None, y=DEV,
+          q=None, qs=0, sc=None):
+    return _abi.lib().fmoe_add_rms_norm(x, xs, r, xs, w, wd, rows, cols, dt, 1e-6, h, y, None, q, qs,
+                                        sc, None)
+
+
+def test_norm_entry_point_refuses():
+    assert _norm(cols=0) == _abi.EINVAL
+    assert _norm(rows=-1) == _abi.EINVAL
+    assert _norm(dt=_abi.I64) == _abi.EINVAL
+    assert _norm(wd=_abi.F16) == _abi.EINVAL          # neither the rows' type nor fp32
+    assert _norm(w=None) == _abi.EINVAL
+    assert _norm(x=None) == _abi.EINVAL
+    assert _norm(xs=-8) == _abi.EINVAL
+    assert _norm(r=DEV) == _abi.EINVAL                # a residual without the stream's output
+    assert _norm(q=DEV, qs=112, sc=DEV) == _abi.EINVAL   # 8 columns are stored in 128
+    assert _norm(q=DEV + 8, qs=128, sc=DEV) == _abi.EINVAL
+    assert _norm(q=DEV, qs=128) == _abi.EINVAL        # no scales
+    assert _norm(rows=1 << 40) == _abi.ERANGE
+    assert _norm(cols=1 << 31) == _abi.ERANGE
+    assert _norm(rows=0, x=None) == _abi.OK           # nothing to do
+
+
+def test_norm_backward_entry_point_refuses():
+    lib = _abi.lib()
+    need = lib.fmoe_add_rms_norm_backward_workspace_bytes(1000, 8)
+    assert need == 512 * 8 * 4
+    assert lib.fmoe_add_rms_norm_backward_workspace_bytes(3, 8) == 3 * 8 * 4
+    assert lib.fmoe_add_rms_norm_backward_workspace_bytes(-1, 8) < 0
+
+    def call(ws=DEV, nbytes=need, gy=DEV, gw=DEV, wd=_abi.BF16, rows=1000):
+        return lib.fmoe_add_rms_norm_backward(gy, 8, None, 0, DEV, 8, DEV, wd, DEV, rows, 8,
+                                              _abi.BF16, DEV, gw, ws, nbytes, None)
+
+    assert call(nbytes=need - 1) == _abi.EINVAL
+    assert call(ws=None) == _abi.EINVAL
+    assert call(ws=DEV + 4) == _abi.EINVAL
+    assert call(gy=None) == _abi.EINVAL
+    assert call(wd=_abi.F16) == _abi.EINVAL
+    assert call(rows=1 << 40) == _abi.ERANGE
+
+
+def test_row_entry_points_refuse():
+    lib = _abi.lib()
+
+    def rows(act=0, q=DEV, qs=128, sc=DEV, x=DEV, cols=8, n=4, dt=_abi.F16):
+        return lib.fmoe_quantize_rows(x, 8, n, cols, dt, act, q, qs, sc, None)
+
+    assert rows(act=2) == _abi.EINVAL
+    assert rows(q=DEV + 4) == _abi.EINVAL
+    assert rows(qs=136) == _abi.EINVAL
+    assert rows(cols=129) == _abi.EINVAL              # needs a pitch of 256
+    assert rows(sc=None) == _abi.EINVAL
+    assert rows(x=None) == _abi.EINVAL
+    assert rows(dt=_abi.I32) == _abi.EINVAL
+    assert rows(n=1 << 40) == _abi.ERANGE
+    assert lib.fmoe_compress_rows(DEV, 8, 4, 8, _abi.F16, DEV, 64, DEV, None, None) == _abi.EINVAL
+    assert lib.fmoe_compress_rows(None, 8, 4, 8, _abi.F16, DEV, 128, DEV, None, None) == _abi.EINVAL
+    assert lib.fmoe_compress_rows(DEV, 8, 1 << 40, 8, _abi.F16, DEV, 128, DEV, None,
+                                  None) == _abi.ERANGE
+    # three scales per row are neither one nor the two blocks of 200 columns
+    assert lib.fmoe_restore_rows(DEV, 256, DEV, 3, 4, 200, DEV, _abi.F32, None) == _abi.EINVAL
+    assert lib.fmoe_restore_rows(DEV, 256, DEV, 2, 4, 200, None, _abi.F32, None) == _abi.EINVAL
+    assert lib.fmoe_gelu_compressed_backward(DEV, 256, DEV, None, 8, 4, 200, _abi.F32, None, DEV,
+                                             None) == _abi.EINVAL
+
+
+def test_int8_linear_entry_point_refuses():
+    def call(x=DEV, xs=128, xr=4, w=DEV, off=DEV, E=2, N=16, K=100, rows=4, out=DEV, os_=16,
+             od=_abi.BF16, idx=None, it=_abi.I64, bias=None, bt=_abi.F32):
+        return _abi.lib().fmoe_int8_linear(x, xs, xr, DEV, idx, it, w, DEV, bias, bt, off, E, N, K,
+                                           rows, out, os_, od, None)
+
+    assert call(off=None) == _abi.EINVAL              # two experts without offsets
+    assert call(xs=112) == _abi.EINVAL
+    assert call(xs=136) == _abi.EINVAL
+    assert call(x=DEV + 8) == _abi.EINVAL
+    assert call(w=DEV + 8) == _abi.EINVAL
+    assert call(os_=15) == _abi.EINVAL
+    assert call(od=_abi.I64) == _abi.EINVAL
+    assert call(idx=DEV, it=_abi.F32) == _abi.EINVAL
+    assert call(bias=DEV, bt=_abi.I32) == _abi.EINVAL
+    assert call(xr=0) == _abi.EINVAL
+    assert call(E=0) == _abi.EINVAL
+    assert call(K=131072, xs=131072) == _abi.ERANGE   # (-128)^2 * K would pass int32
+    assert call(rows=1 << 31) == _abi.ERANGE
+    assert call(N=1 << 25, os_=1 << 25) == _abi.ERANGE
+    assert call(rows=0, x=None) == _abi.OK
