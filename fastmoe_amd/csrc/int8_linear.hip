@@ -41,48 +41,116 @@ struct Tile {
   int count;
 };
 
-// The `target`-th tile of the packed rows.  Each lane counts one expert's tiles and a prefix sum over
-// the wave finds whose the target is; every wave does it for itself, so there is neither a table in
+__device__ __forceinline__ int64_t bounded(int64_t v, int64_t most) {
+  return min(max(v, (int64_t)0), most);
+}
+
+// The tiles of up to 256 experts from e0 on, four of them in each lane: lo[i] is the first row of the
+// lane's i-th expert, n[i] its tiles, incl the tiles up to and with this lane's.  One round of loads
+// and a prefix sum over the wave; every wave does it for itself, so there is neither a table in
 // memory nor a launch that makes it.  Offsets are held to [0, rows]: no value in them makes a wave
 // read or write outside the arrays.
-template <int BM> __device__ __forceinline__ bool find_tile(const LinearArgs& a, int64_t target, Tile* t) {
-  if (!a.off) {
-    t->expert = 0;
-    t->row = target * BM;
-    if (t->row >= a.rows) return false;
-    t->count = (int)min((int64_t)BM, a.rows - t->row);
-    return true;
-  }
-  const int lane = threadIdx.x & (kWave - 1);
-  int64_t base = 0;
-  for (int64_t e0 = 0; e0 <= a.E; e0 += kWave) {
-    const int64_t e = e0 + lane;
-    int64_t lo = 0, hi = 0;
-    if (e <= a.E) {
-      lo = e == 0 ? 0 : min(max(a.off[e], (int64_t)0), a.rows);
-      hi = e == a.E ? a.rows : min(max(a.off[e + 1], (int64_t)0), a.rows);
+constexpr int kScanExperts = 4 * kWave;
+constexpr int kBand = 4;
+template <int BM> struct TileScan {
+  int64_t lo[5];
+  int n[4], incl;
+  __device__ __forceinline__ void load(const LinearArgs& a, int64_t e0) {
+    const int lane = threadIdx.x & (kWave - 1);
+#pragma unroll
+    for (int i = 0; i < 5; ++i) {
+      const int64_t e = min(e0 + lane * 4 + i, a.E);
+      lo[i] = e == 0 ? 0 : bounded(a.off[e], a.rows);
     }
-    const int n = (int)((max(hi - lo, (int64_t)0) + BM - 1) / BM);
-    int incl = n;
+    incl = 0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {  // beyond E both ends are off[E]: no rows
+      n[i] = (int)((max(lo[i + 1] - lo[i], (int64_t)0) + BM - 1) / BM);
+      incl += n[i];
+    }
 #pragma unroll
     for (int d = 1; d < kWave; d *= 2) {
       const int up = __shfl_up(incl, d);
       if (lane >= d) incl += up;
     }
-    const int all = __builtin_amdgcn_readlane(incl, kWave - 1);
-    if (target < base + all) {
-      const int want = (int)(target - base);
-      const uint64_t hit = __ballot(want >= incl - n && want < incl);
-      const int at = __ffsll((unsigned long long)hit) - 1;
-      t->expert = e0 + at;
-      const int64_t first = __shfl(lo, at) + (int64_t)(want - __shfl(incl - n, at)) * BM;
-      t->row = first;
-      t->count = (int)min((int64_t)BM, (int64_t)__shfl(hi, at) - first);
-      return true;
-    }
-    base += all;
   }
-  return false;
+  __device__ __forceinline__ int total() const { return __builtin_amdgcn_readlane(incl, kWave - 1); }
+  // Tile `want` of these experts, 0 <= want < total(), and its group of columns.  An expert's tiles go
+  // in bands of kBand: the workgroups of a band stand next to each other, columns after columns.
+  // False only for offsets that are no offsets, whose tiles may pass what an int counts.
+  __device__ __forceinline__ bool find(int want, int64_t e0, int groups_n, Tile* t, int* group) const {
+    const int mine = n[0] + n[1] + n[2] + n[3];
+    const int at = __ffsll((unsigned long long)__ballot(want < incl)) - 1;
+    if (at < 0) return false;
+    want -= __builtin_amdgcn_readlane(incl - mine, at);
+    if (want < 0) return false;
+    int64_t expert = e0 + 4 * at, first = 0, end = 0;
+    int of = 0;  // the expert's tiles
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      const int k = __builtin_amdgcn_readlane(n[i], at);
+      if (!of && want < k) {
+        of = k;
+        expert += i;
+        first = __shfl(lo[i], at);
+        end = __shfl(lo[i + 1], at);
+      }
+      if (!of) want -= k;
+    }
+    if (!of) return false;
+    const int band = want / kBand, high = min(kBand, of - band * kBand);
+    const int unit = (want % kBand) * groups_n + *group;
+    want = band * kBand + unit % high;
+    *group = unit / high;
+    t->expert = expert;
+    t->row = first + (int64_t)want * BM;
+    t->count = (int)min((int64_t)BM, end - t->row);
+    return true;
+  }
+};
+
+// Where this workgroup's work lies: a tile of rows and a group of columns.  Workgroups go to the eight
+// XCDs in turn (blockIdx % 8); each XCD gets one contiguous eighth of the tiles that there are, columns
+// innermost, so that the workgroups that run on it together share rows and weights in its L2.
+// False where there is no work: the grid is the most tiles that these sizes can have.
+constexpr unsigned kXcds = 8;
+template <int BM> __device__ __forceinline__ bool place(const LinearArgs& a, Tile* t, int* group) {
+  TileScan<BM> scan;
+  int64_t rest = 0, tiles = (a.rows + BM - 1) / BM;  // rest: first row of no expert
+  int first = 0;                                     // tiles of the first chunk of experts
+  if (a.off) {
+    rest = bounded(a.off[a.E], a.rows);
+    tiles = (a.rows - rest + BM - 1) / BM;
+    for (int64_t e0 = kScanExperts; e0 < a.E; e0 += kScanExperts) {
+      scan.load(a, e0);
+      tiles += scan.total();
+    }
+    scan.load(a, 0);
+    first = scan.total();
+    tiles += first;
+  }
+  const unsigned columns = (unsigned)a.groups_n;
+  const unsigned work = (unsigned)tiles * columns;  // the host has checked that the grid fits 32 bits
+  const unsigned xcd = blockIdx.x % kXcds, turn = blockIdx.x / kXcds;
+  const unsigned each = work / kXcds, over = work % kXcds;
+  if (turn >= each + (xcd < over ? 1 : 0)) return false;
+  const unsigned unit = xcd * each + min(xcd, over) + turn;
+  int64_t want = unit / columns;
+  *group = (int)(unit % columns);
+  if (a.off) {
+    if (want < first) return scan.find((int)want, 0, a.groups_n, t, group);
+    want -= first;
+    for (int64_t e0 = kScanExperts; e0 < a.E; e0 += kScanExperts) {
+      scan.load(a, e0);
+      if (want < scan.total()) return scan.find((int)want, e0, a.groups_n, t, group);
+      want -= scan.total();
+    }
+  }
+  t->expert = a.off ? a.E : 0;
+  t->row = rest + want * BM;
+  if (t->row >= a.rows) return false;
+  t->count = (int)min((int64_t)BM, a.rows - t->row);
+  return true;
 }
 
 // The row of x that packed row r reads; -1 where its index lies outside x.
@@ -127,70 +195,296 @@ __device__ __forceinline__ void zero_rows(const LinearArgs& a, const Tile& t, in
       st1(static_cast<TO*>(a.out) + (t.row + r) * a.out_stride + n, 0.f);
 }
 
-// Few rows per expert: the weights are the traffic, each byte of them used for at most 16 * MT rows.
-// A workgroup has 16 * MT rows and 16 * NB columns of one expert.  Its waves take 128-byte pieces of
-// K in turn, straight from memory to the matrix units' registers (LDS would only add a copy: no
-// two waves share a byte of the weights), and add their int32 parts in LDS at the end.
-template <typename TO, int MT, int NB, int WAVES>
-__global__ __launch_bounds__(WAVES * kWave) void k_int8_stream(LinearArgs a) {
-  __shared__ i32x4 part[WAVES][MT * NB][kWave];
+// Few rows and few columns: 16 x 16 results in a workgroup, whose eight waves take 128-byte pieces of K
+// in turn, straight from memory to the matrix units' registers, and add their int32 parts in LDS.
+// Where even the smallest tile below leaves most CUs without work, splitting K over the waves is what is
+// left: 11.8 against 14.9 us for one row and [2048, 7168] weights, 32 workgroups of 32 x 64 (but 27.8
+// against 26.7 us with eight experts' weights, 256 workgroups).
+constexpr int kFewWaves = 8;
+template <typename TO> __global__ __launch_bounds__(kFewWaves * kWave) void k_int8_few(LinearArgs a) {
+  __shared__ i32x4 part[kFewWaves][kWave];
   Tile t;
-  if (!find_tile<16 * MT>(a, blockIdx.x / (unsigned)a.groups_n, &t)) return;
-  const int64_t n0 = (int64_t)(blockIdx.x % (unsigned)a.groups_n) * (16 * NB);
+  int group;
+  if (!place<16>(a, &t, &group)) return;
+  const int64_t n0 = (int64_t)group * 16;
   if (t.expert == a.E) {
-    zero_rows<TO>(a, t, n0, 16 * NB);
+    zero_rows<TO>(a, t, n0, 16);
     return;
   }
   const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
   const int l16 = lane & 15, quad = lane >> 4;
-  const uint8_t* xp[MT];
+  const int64_t row = source_row(a, t.row + min(l16, t.count - 1));
+  const uint8_t* xp = a.x + max(row, (int64_t)0) * a.x_stride + quad * 16;
+  const uint8_t* wp = a.w + (t.expert * a.N + min(n0 + l16, a.N - 1)) * a.Kp + quad * 16;
+  i32x4 acc = {0, 0, 0, 0};
+  constexpr int kStep = kFewWaves * 128, kAhead = 4;  // pieces asked for before the first is used
+  auto pieces = [&](auto count, int64_t k) {
+    constexpr int n = 2 * decltype(count)::value;
+    i32x4 w[n], x[n];
 #pragma unroll
-  for (int m = 0; m < MT; ++m) {
-    const int64_t i = source_row(a, t.row + min(m * 16 + l16, t.count - 1));
-    xp[m] = a.x + max(i, (int64_t)0) * a.x_stride + quad * 16;
-  }
-  const uint8_t* wp[NB];
-#pragma unroll
-  for (int b = 0; b < NB; ++b)
-    wp[b] = a.w + (t.expert * a.N + min(n0 + b * 16 + l16, a.N - 1)) * a.Kp + quad * 16;
-  i32x4 acc[MT][NB];
-#pragma unroll
-  for (int m = 0; m < MT; ++m)
-#pragma unroll
-    for (int b = 0; b < NB; ++b) acc[m][b] = i32x4{0, 0, 0, 0};
-  for (int64_t k = wave * 128; k < a.Kp; k += WAVES * 128) {
-    i32x4 xv[2][MT], wv[2][NB];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-#pragma unroll
-      for (int b = 0; b < NB; ++b)
-        wv[h][b] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp[b] + k + 64 * h));
-#pragma unroll
-      for (int m = 0; m < MT; ++m) xv[h][m] = *reinterpret_cast<const i32x4*>(xp[m] + k + 64 * h);
+    for (int i = 0; i < n; ++i) {
+      const int64_t at = k + i / 2 * kStep + i % 2 * 64;
+      w[i] = __builtin_nontemporal_load(reinterpret_cast<const i32x4*>(wp + at));
+      x[i] = *reinterpret_cast<const i32x4*>(xp + at);
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int i = 0; i < n; ++i) acc = __builtin_amdgcn_mfma_i32_16x16x64_i8(w[i], x[i], acc, 0, 0, 0);
+  };
+  int64_t k = wave * 128;
+  for (; k + (kAhead - 1) * kStep < a.Kp; k += kAhead * kStep)
+    pieces(std::integral_constant<int, kAhead>{}, k);
+  for (; k < a.Kp; k += kStep) pieces(std::integral_constant<int, 1>{}, k);
+  part[wave][lane] = acc;
+  __syncthreads();
+  if (wave != 0 || l16 >= t.count) return;
 #pragma unroll
-      for (int m = 0; m < MT; ++m)
+  for (int v = 1; v < kFewWaves; ++v) acc += part[v][lane];
+  // lane l of a 16 x 16 result has row l % 16 and columns 4 * (l / 16) + 0..3
+  store4<TO>(a, t, t.row + l16, n0 + quad * 4, acc, row >= 0 ? a.sx[row] : 0.f);
+}
+
+// BM x BN results of one expert in a workgroup of WR x WC waves, each wave (BM / WR) x (BN / WC) of them in
+// its registers as 32 x 32 tiles.  Pieces of KB bytes of K of both operands go through a ring of
+// STAGES buffers in LDS, which the loads write directly (no registers, no LDS store instructions).
+//
+// A row's 16-byte chunks lie in LDS at position chunk ^ swizzle(row): memory is read in whole pieces of
+// a row, and the rows that the lanes of a fragment's read touch together lie in different banks
+// (64 banks of 4 bytes: 256 / KB rows fill them once).
+typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
+#define FMOE_LDS __attribute__((address_space(3)))
+
+__device__ __forceinline__ void load_piece(const uint8_t* from, uint8_t* to) {
+  __builtin_amdgcn_global_load_lds(reinterpret_cast<const FMOE_GLOBAL uint32_t*>(
+                                       reinterpret_cast<uintptr_t>(from)),
+                                   (FMOE_LDS uint32_t*)to, 16, 0, 0);
+}
+// All but the youngest `LOADS` loads of this wave have arrived, and all its LDS reads.
+template <int LOADS> __device__ __forceinline__ void wait_loads() {
+  static_assert(LOADS < 64, "vmcnt has six bits");
+  __builtin_amdgcn_s_waitcnt((LOADS & 15) | (LOADS >> 4) << 14 | 0x70);
+}
+// A barrier alone: __syncthreads would also wait for every load to LDS in flight.  The compiler moves no
+// access to memory across it, and wait_loads before it orders what the waves share.
+__device__ __forceinline__ void barrier() {
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
+
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES>
+__global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
+  constexpr int kWaves = WR * WC;
+  constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 tiles of a wave
+  constexpr int kRows = 1024 / KB;                     // rows of one load of a wave
+  constexpr int PX = BM / kRows / kWaves, PW = BN / kRows / kWaves, kLoads = PX + PW;
+  constexpr int kStage = (BM + BN) * KB, kSteps = KB / 32;
+  static_assert(STAGES == 3 || STAGES == 4, "buffers");
+  static_assert(PX * kRows * kWaves == BM && PW * kRows * kWaves == BN, "whole loads");
+  // separate objects: the compiler then sees that reads of one stage need not wait for the loads in
+  // flight to the others
+  __shared__ __attribute__((aligned(1024))) uint8_t stage0[kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage1[kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage2[kStage];
+  __shared__ __attribute__((aligned(1024))) uint8_t stage3[STAGES > 3 ? kStage : 1];
+  __shared__ float row_scale[BM], col_scale[BN], col_bias[BN];
+  Tile t;
+  int group;
+  if (!place<BM>(a, &t, &group)) return;
+  const int64_t n0 = (int64_t)group * BN;
+  if (t.expert == a.E) {
+    zero_rows<TO>(a, t, n0, BN);
+    return;
+  }
+  const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
+  const uint8_t *xp[PX], *wp[PW];
 #pragma unroll
-        for (int b = 0; b < NB; ++b)
-          acc[m][b] = __builtin_amdgcn_mfma_i32_16x16x64_i8(wv[h][b], xv[h][m], acc[m][b], 0, 0, 0);
+  for (int i = 0; i < PX; ++i) {
+    const int r = (wave * PX + i) * kRows + lane / (KB / 16);
+    xp[i] = a.x + max(source_row(a, t.row + min(r, t.count - 1)), (int64_t)0) * a.x_stride +
+            (lane % (KB / 16) ^ swizzle<KB>(r)) * 16;
   }
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+  for (int i = 0; i < PW; ++i) {
+    const int r = (wave * PW + i) * kRows + lane / (KB / 16);
+    wp[i] = a.w + (t.expert * a.N + min(n0 + r, a.N - 1)) * a.Kp +
+            (lane % (KB / 16) ^ swizzle<KB>(r)) * 16;
+  }
+  auto load_one = [&](uint8_t* s, int64_t at, int i) {
+    if (i < PX) load_piece(xp[i < PX ? i : 0] + at, s + (wave * PX + i) * 1024);
+    else load_piece(wp[i < PX ? 0 : i - PX] + at, s + BM * KB + (wave * PW + i - PX) * 1024);
+  };
+  auto load = [&](uint8_t* s, int64_t at) {
 #pragma unroll
-    for (int b = 0; b < NB; ++b) part[wave][m * NB + b][lane] = acc[m][b];
+    for (int i = 0; i < kLoads; ++i) load_one(s, at, i);
+  };
+  i32x16 acc[TN][TM];
+#pragma unroll
+  for (int n = 0; n < TN; ++n)
+#pragma unroll
+    for (int m = 0; m < TM; ++m)
+#pragma unroll
+      for (int i = 0; i < 16; ++i) acc[n][m][i] = 0;
+  const int l32 = lane & 31, half = lane >> 5;
+  // the waves of a SIMD (every fourth) have different rows: where a tile's last rows are missing, the
+  // matrix units are shared by the waves that have rows
+  const int m0 = (wave / WC) * (BM / WR), w0 = (wave % WC) * (BN / WC);
+  const bool busy = m0 < t.count;
+  // fragments of 32 bytes of K: lane l has row l % 32 and bytes 16 * (l / 32) + 0..15
+  i32x4 xv[2][TM], wv[2][TN];
+  auto read_one = [&](const uint8_t* s, int k, int to, int i) {
+    const int at = ((2 * k + half) ^ swizzle<KB>(l32)) * 16 + l32 * KB;
+    if (i < TM)
+      xv[to][i < TM ? i : 0] = *reinterpret_cast<const i32x4*>(s + (m0 + i * 32) * KB + at);
+    else
+      wv[to][i < TM ? 0 : i - TM] =
+          *reinterpret_cast<const i32x4*>(s + (BM + w0 + (i - TM) * 32) * KB + at);
+  };
+  const int pieces = (int)(a.Kp / KB);
+  // loads beyond the last piece read it once more, into a buffer that nobody reads: the number of
+  // loads in flight is then the same in every step
+  auto at = [&](int piece) { return (int64_t)min(piece, pieces - 1) * KB; };
+  // Step i multiplies piece i in buffer `cur`.  Before its last fragments are multiplied, each wave has
+  // read all of the piece and waits until its loads of piece i + 1 have arrived; behind the barrier that
+  // holds for every wave, so `next` is read.  Meanwhile the piece before (its buffer `old` was read by
+  // every wave before the last step's barrier) is replaced by piece i + STAGES - 1.  Reads and
+  // loads stand between the products, one or two at a time: issued together they would hold the wave
+  // back while the matrix units run dry.
+  auto step = [&](auto works, uint8_t* old, uint8_t* cur, const uint8_t* next, int i) {
+    const int64_t from = at(i + STAGES - 1);
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+      const bool last = k + 1 == kSteps;
+      if (last) {
+        wait_loads<(STAGES - 3) * kLoads + (kSteps - 1) * kLoads / kSteps>();
+        barrier();
+      }
+      constexpr int kOps = TM + TN;
+      const int more = (k + 1) * kLoads / kSteps - k * kLoads / kSteps;  // loads in this part
+      const int ops = kOps + more;
+      if constexpr (decltype(works)::value) {
+#pragma unroll
+        for (int j = 0; j < TM * TN; ++j) {
+          acc[j / TM][j % TM] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
+              wv[k & 1][j / TM], xv[k & 1][j % TM], acc[j / TM][j % TM], 0, 0, 0);
+#pragma unroll
+          for (int o = j * ops / (TM * TN); o < (j + 1) * ops / (TM * TN); ++o) {
+            if (o < kOps) read_one(last ? next : cur, last ? 0 : k + 1, (k + 1) & 1, o);
+            else load_one(old, from, k * kLoads / kSteps + o - kOps);
+          }
+          __builtin_amdgcn_sched_barrier(0);
+        }
+      } else {  // no rows for this wave: it only loads its share
+#pragma unroll
+        for (int o = kOps; o < ops; ++o) load_one(old, from, k * kLoads / kSteps + o - kOps);
+      }
+    }
+  };
+  auto run = [&](auto works) {
+    int i = 0;
+    if constexpr (STAGES == 3) {
+      for (; i + 3 <= pieces; i += 3) {
+        step(works, stage2, stage0, stage1, i);
+        step(works, stage0, stage1, stage2, i + 1);
+        step(works, stage1, stage2, stage0, i + 2);
+      }
+      if (i < pieces) step(works, stage2, stage0, stage1, i);
+      if (i + 1 < pieces) step(works, stage0, stage1, stage2, i + 1);
+    } else {
+      for (; i + 4 <= pieces; i += 4) {
+        step(works, stage3, stage0, stage1, i);
+        step(works, stage0, stage1, stage2, i + 1);
+        step(works, stage1, stage2, stage3, i + 2);
+        step(works, stage2, stage3, stage0, i + 3);
+      }
+      if (i < pieces) step(works, stage3, stage0, stage1, i);
+      if (i + 1 < pieces) step(works, stage0, stage1, stage2, i + 1);
+      if (i + 2 < pieces) step(works, stage1, stage2, stage3, i + 2);
+    }
+  };
+  load(stage0, at(0));
+  __builtin_amdgcn_sched_barrier(0);
+  // the rows' scales, the columns' scales and biases: asked for here, so that they arrive between the
+  // first pieces, and used at the end
+  static_assert(BM <= kWaves * kWave && BN <= kWaves * kWave, "a row and a column for each thread");
+  const int64_t my_row = source_row(a, t.row + min((int)threadIdx.x, t.count - 1));
+  const int64_t my_col = t.expert * a.N + min(n0 + threadIdx.x, a.N - 1);
+  const float my_row_scale = a.sx[max(my_row, (int64_t)0)];
+  const float my_col_scale = a.sw[my_col];
+  const float my_bias = a.bias ? load_weight(a.bias, a.bias_dtype, my_col) : 0.f;
+  __builtin_amdgcn_sched_barrier(0);
+  load(stage1, at(1));
+  if constexpr (STAGES > 3) load(stage2, at(2));
+  __builtin_amdgcn_sched_barrier(0);
+  if (threadIdx.x < BM) row_scale[threadIdx.x] = my_row >= 0 ? my_row_scale : 0.f;
+  if (threadIdx.x < BN) {
+    col_scale[threadIdx.x] = my_col_scale;
+    col_bias[threadIdx.x] = my_bias;
+  }
+  wait_loads<(STAGES - 2) * kLoads>();
+  barrier();
+#pragma unroll
+  for (int i = 0; i < TM + TN; ++i) read_one(stage0, 0, 0, i);
+  if (busy) run(std::true_type{});
+  else run(std::false_type{});
+  wait_loads<0>();
   __syncthreads();
-  // lane l of a 16 x 16 result has row l % 16 and columns 4 * (l / 16) + 0..3
-  for (int p = wave; p < MT * NB; p += WAVES) {
-    i32x4 sum = part[0][p][lane];
+  // Each wave turns its results, 32 rows at a time, into rows of the output's type in LDS and stores
+  // them 16 bytes a lane: whole lines of the output.
+  constexpr int kSize = ElemInfo<TO>::kBytes;
+  // column tiles at a time: as many as the stages hold for every wave
+  constexpr auto fits = [](int tiles) {
+    return kStage / (32 * (tiles * 32 * kSize + 16)) * STAGES >= kWaves;
+  };
+  constexpr int CT = fits(TN) ? TN : fits(TN / 2) ? TN / 2 : TN / 4;
+  constexpr int kPitch = CT * 32 * kSize + 16;  // 16 bytes more: the 32 rows start in different banks
+  constexpr int kPerStage = kStage / (32 * kPitch);
+  static_assert(kPerStage * STAGES >= kWaves, "the stages hold the results");
+  const int place_in = wave / kPerStage;
+  uint8_t* mine = (place_in == 0 ? stage0 : place_in == 1 ? stage1 : place_in == 2 ? stage2 : stage3) +
+                  wave % kPerStage * (32 * kPitch);
 #pragma unroll
-    for (int v = 1; v < WAVES; ++v) sum += part[v][p][lane];
-    const int m = (p / NB) * 16 + l16;
-    if (m < t.count) {
-      const int64_t i = source_row(a, t.row + m);
-      store4<TO>(a, t, t.row + m, n0 + (p % NB) * 16 + quad * 4, i >= 0 ? sum : i32x4{0, 0, 0, 0},
-                 i >= 0 ? a.sx[i] : 0.f);
+  for (int m = 0; m < TM; ++m) {
+    const int first = m0 + m * 32;
+    if (first >= t.count) break;
+    const float sx = row_scale[first + l32];
+    // lane l of a 32 x 32 result has row l % 32 and columns 8 * q + 4 * (l / 32) + 0..3, q = 0..3
+#pragma unroll
+    for (int base = 0; base < TN; base += CT) {
+#pragma unroll
+      for (int n = 0; n < CT; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int c = n * 32 + q * 8 + half * 4;
+          const int at_col = w0 + base * 32 + c;
+          float f[4];
+#pragma unroll
+          for (int j = 0; j < 4; ++j)
+            f[j] = (float)acc[base + n][m][4 * q + j] * sx * col_scale[at_col + j] +
+                   col_bias[at_col + j];
+          *reinterpret_cast<typename Vec<TO, 4>::raw_t*>(mine + l32 * kPitch + c * kSize) =
+              Vec<TO, 4>::pack(f);
+        }
+      constexpr int kLanes = CT * 32 * kSize / 16;  // lanes of a row
+#pragma unroll
+      for (int p = 0; p < 32 * kLanes / kWave; ++p) {
+        const int r = p * (kWave / kLanes) + lane / kLanes, c = lane % kLanes * (16 / kSize);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * kPitch + c * kSize);
+        const int64_t n = n0 + w0 + base * 32 + c;
+        if (first + r >= t.count || n >= a.N) continue;
+        TO* to = static_cast<TO*>(a.out) + (t.row + first + r) * a.out_stride + n;
+        if (n + 16 / kSize <= a.N) {
+          *reinterpret_cast<u32x4_any*>(to) = v;
+        } else {
+          const int left = (int)(a.N - n);
+#pragma unroll
+          for (int j = 0; j < 16 / kSize; ++j)
+            if (j < left) {
+              if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(to)[j] = v[j];
+              else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(v[j / 2] >> (16 * (j % 2)));
+            }
+        }
+      }
     }
   }
 }
@@ -209,23 +503,70 @@ int64_t most_tiles(int64_t rows, int64_t E, bool grouped, int64_t bm) {
   return grouped ? std::min(rows, even + E) : even;
 }
 
-template <typename TO, int MT, int NB, int WAVES> int launch_stream(const char* who, LinearArgs a, hipStream_t s) {
-  const int64_t tiles = most_tiles(a.rows, a.E, a.off != nullptr, 16 * MT);
-  a.groups_n = (int)((a.N + 16 * NB - 1) / (16 * NB));
-  if (tiles > ((int64_t(1) << 32) - 1) / (a.groups_n * (int64_t)WAVES * kWave)) {
-    fmoe_host::set_error("%s: rows=%lld N=%lld too large", who, (long long)a.rows, (long long)a.N);
-    return FMOE_ERANGE;
+// Fills in the groups of `bn` columns; the workgroups of tiles of `bm` rows, or -1 where they are too many.
+int64_t grid_of(const char* who, LinearArgs* a, int64_t bm, int64_t bn, int64_t threads) {
+  const int64_t tiles = most_tiles(a->rows, a->E, a->off != nullptr, bm);
+  a->groups_n = (int)((a->N + bn - 1) / bn);
+  if (tiles > ((int64_t(1) << 32) - 1) / (a->groups_n * threads)) {
+    fmoe_host::set_error("%s: rows=%lld N=%lld too large", who, (long long)a->rows, (long long)a->N);
+    return -1;
   }
-  hipLaunchKernelGGL((k_int8_stream<TO, MT, NB, WAVES>), dim3((unsigned)(tiles * a.groups_n)),
-                     dim3(WAVES * kWave), 0, s, a);
+  return tiles * a->groups_n;
+}
+
+template <typename TO> int launch_few(const char* who, LinearArgs a, hipStream_t s) {
+  const int64_t groups = grid_of(who, &a, 16, 16, kFewWaves * kWave);
+  if (groups < 0) return FMOE_ERANGE;
+  hipLaunchKernelGGL(k_int8_few<TO>, dim3((unsigned)groups), dim3(kFewWaves * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES>
+int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
+  const int64_t groups = grid_of(who, &a, BM, BN, WR * WC * kWave);
+  if (groups < 0) return FMOE_ERANGE;
+  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES>), dim3((unsigned)groups),
+                     dim3(WR * WC * kWave), 0, s, a);
+  return fmoe_host::check_launch(who);
+}
+
+// The variant for these sizes: the largest tile that the experts' rows fill and that leaves no CU
+// without work.  `per` is the rows of an expert were the routing even, work(bm, bn) the workgroups then.
+// Times in us of 32 experts' [2048, 7168] weights / 128 experts' [1024, 2048] / 8 experts' [4096, 4096]:
+//   rows per expert      1              16             48             128            256
+//   32 x 64         58 / 38 / 24   91 / 58 / 34  123 / 86 / 45  214 / 148 / 72  360 / 246 / 115
+//   128 x 128       80 / 44 / 31   94 / 59 / 36  102 / 65 / 38   152 / 95 / 56  233 / 145 / 77
+//   128 x 256       63 / 45 / 35   83 / 55 / 40   88 / 61 / 42   141 / 85 / 47  191 / 124 / 77
+//   256 x 256       81 / 51 / 42   93 / 60 / 46  100 / 68 / 50   114 / 82 / 57  204 / 120 / 62
+enum Variant { kFew = 16016, k32x64 = 32064, k128x128 = 128128, k128x256 = 128256, k256x256 = 256256 };
+Variant pick(int64_t rows, int64_t E, int64_t N) {
+  const int64_t per = rows / E;
+  auto work = [&](int64_t bm, int64_t bn) {
+    return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
+  };
+  if (per >= 112 && work(256, 256) >= 192) return k256x256;
+  if (per >= 16 && work(128, 256) >= 140) return k128x256;
+  if (per >= 40 && work(128, 128) >= 128) return k128x128;
+  if (per <= 16 && work(32, 64) <= 128) return kFew;
+  return k32x64;
+}
+
 template <typename TO> int launch_linear(const char* who, const LinearArgs& a, hipStream_t s) {
-  return launch_stream<TO, 4, 4, 4>(who, a, s);
+  switch (pick(a.rows, a.E, a.N)) {
+    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4>(who, a, s);
+    case k128x256: return launch_tile<TO, 128, 256, 2, 4, 128, 3>(who, a, s);
+    case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4>(who, a, s);
+    case kFew: return launch_few<TO>(who, a, s);
+    default: return launch_tile<TO, 32, 64, 1, 2, 128, 4>(who, a, s);
+  }
 }
 
 }  // namespace
+
+extern "C" int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N) {
+  if (rows < 1 || num_experts < 1 || N < 1) return -1;
+  return pick(rows, num_experts, N);
+}
 
 extern "C" int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows,
                                 const float* d_x_scales, const void* d_index, int index_dtype,

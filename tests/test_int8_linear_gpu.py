@@ -8,6 +8,7 @@ import pytest
 import torch
 
 import fastmoe_amd as fm
+from fastmoe_amd import _abi
 
 pytestmark = pytest.mark.gpu
 U = 2.0 ** -24
@@ -88,6 +89,51 @@ def test_against_whole_numbers(name, K, N, dtype):
     x, w = make(R, K, E, N, seed=K + N)
     got = fm.int8_linear(x, w, route(counts), out_dtype=dtype)
     check(got, *reference(x, w, counts), dtype)
+
+
+def ragged(E, mean, seed=0):
+    """Rows of E experts: none, one, around the tile sizes, the rest to reach the mean."""
+    special = [0, 1, 31, 32, 33, 63, 65, 127, 128, 129, 255, 256, 257, 0]
+    counts = [min(special[(e + seed) % len(special)], 2 * mean) for e in range(E)]
+    short = E * mean - sum(counts)
+    for e in range(0, E, 3):
+        if short > 0:
+            counts[e] += min(short, 2 * mean)
+            short -= min(short, 2 * mean)
+    return counts
+
+
+# (tile, experts, mean rows, columns): the sizes that the choice by size sends to each tile
+TILES = [(256256, 50, 130, 1000), (128256, 40, 40, 1000), (128128, 16, 60, 1024), (32064, 30, 5, 300),
+         (16016, 3, 4, 130)]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("K", [1, 130, 300, 500, 641, 1100])
+@pytest.mark.parametrize("tile,E,mean,N", TILES)
+def test_every_tile(tile, E, mean, N, K, dtype):
+    """Every tile, with rings of every remainder of pieces, ragged experts and column ends."""
+    counts = ragged(E, mean, seed=K)
+    R = sum(counts)
+    assert _abi.lib().fmoe_int8_linear_tile(R, E, N) == tile
+    x, w = make(R, K, E, N, seed=K)
+    bias = torch.randn(E, N, device="cuda")
+    got = fm.int8_linear(x, w, route(counts), bias=bias, out_dtype=dtype)
+    check(got, *reference(x, w, counts, bias=bias), dtype)
+    g = torch.Generator(device="cuda").manual_seed(K)
+    rows = torch.randint(-2, R + 2, (R + 37,), generator=g, device="cuda")
+    got = fm.int8_linear(x, w, route(counts), rows=rows, out_dtype=dtype)
+    check(got, *reference(x, w, counts, rows), dtype)
+
+
+def test_more_experts_than_one_scan_and_offsets_that_are_none():
+    counts = [(5 * e) % 7 if e % 3 else 0 for e in range(1000)]
+    R = sum(counts)
+    x, w = make(R, 64, 1000, 33)
+    check(fm.int8_linear(x, w, route(counts)), *reference(x, w, counts), torch.bfloat16)
+    zigzag = torch.tensor([0, R] * 500 + [0], device="cuda")
+    fm.int8_linear(x, w, zigzag)  # bounded: each workgroup's tile lies within the rows
+    torch.cuda.synchronize()
 
 
 @pytest.mark.parametrize("index", [torch.int64, torch.int32])
