@@ -46,10 +46,10 @@ template <typename T, bool GELU> __global__ __launch_bounds__(kGroup) void k_com
       V::template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols);
   float f[8];
   V::V::cvt(raw, f);
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
-  const Scale8 s = scale8(row_max(top));
+  for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
+  const Scale8 s = scale8(row_max(abs_bits(top)));
   if (col % kHoldBlock == 0) a.scales[row * a.blocks + col / kHoldBlock] = s.scale;
   *reinterpret_cast<u32x2*>(a.q + row * a.q_stride + col) = pack8(f, s);
   if constexpr (GELU) {

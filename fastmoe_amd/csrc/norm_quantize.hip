@@ -78,7 +78,7 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm(NormArgs a) {
   }
   const float c = 1.0f / sqrtf(group_sum<THREADS>(sum, lds_sum) / (float)a.cols + a.eps);
   if (a.rstd && tid == 0) a.rstd[row] = c;
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     float w[8];
@@ -86,14 +86,14 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       f[v][i] = f[v][i] * c * w[i];
-      top = max(top, abs_bits(f[v][i]));
+      top = larger(top, f[v][i]);
     }
     if (a.y)
       V::store(static_cast<T*>(a.y) + row * a.cols, (v * THREADS + tid) * 8, a.cols,
                V::V::pack(f[v]));
   }
   if (!a.q) return;
-  const Scale8 s = scale8(group_max<THREADS>(top, lds_max));
+  const Scale8 s = scale8(group_max<THREADS>(abs_bits(top), lds_max));
   if (tid == 0) a.scales[row] = s.scale;
   uint8_t* q = a.q + row * a.q_stride;
 #pragma unroll
@@ -142,16 +142,16 @@ __global__ __launch_bounds__(1024) void k_norm_long(NormArgs a) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) f[i] = f[i] * c * w[i];
   };
-  uint32_t top = 0;
+  float top = 0.f;
   for (int64_t col = threadIdx.x * 8; col < a.cols; col += kThreads * 8) {
     float f[8];
     normed(col, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
+    for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
     if (a.y) V::store(static_cast<T*>(a.y) + row * a.cols, col, a.cols, V::V::pack(f));
   }
   if (!a.q) return;
-  const Scale8 s = scale8(group_max<kThreads>(top, lds_max));
+  const Scale8 s = scale8(group_max<kThreads>(abs_bits(top), lds_max));
   if (threadIdx.x == 0) a.scales[row] = s.scale;
   for (int64_t col = threadIdx.x * 8; col < a.q_cols; col += kThreads * 8) {
     float f[8];
@@ -166,18 +166,19 @@ struct NormBwdArgs {
   int64_t gy_stride, gh_stride, h_stride;  // elements
   int64_t rows, cols;
   void* gx;         // packed
-  float* partials;  // [units, cols]: each unit's sum over its rows of grad_y * h * c; or null
-  int64_t units;
+  float* partials;  // [workgroups, cols]: each one's sum over its rows of grad_y * h * c; or null
+  int64_t units;    // rows in flight: workgroups times rows_per_group
 };
 
 // A unit (the threads that hold a row) takes rows unit, unit + units, ... and keeps its part of
-// grad_w in registers: one pass over the three inputs, whatever the number of rows.
+// grad_w in registers: one pass over the three inputs, whatever the number of rows.  Where a unit is a
+// wave, the workgroup's four join their parts in LDS.
 template <typename T, typename TW, int THREADS, int VPT>
 __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm_bwd(NormBwdArgs a) {
   __shared__ float lds[2][16];
   constexpr int kRows = rows_per_group<THREADS>();
+  __shared__ float join[kRows > 1 ? kRows : 1][kRows > 1 ? THREADS * VPT * 8 : 1];
   const int64_t unit = (int64_t)blockIdx.x * kRows + threadIdx.x / THREADS;
-  if (unit >= a.units) return;
   const int tid = threadIdx.x % THREADS;
   using V = Eight<T>;
   using W = Eight<TW>;
@@ -239,7 +240,22 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm_bwd(NormBwdAr
     }
   }
   if (!a.partials) return;
-  float* out = a.partials + unit * a.cols;
+  float* out = a.partials + (int64_t)blockIdx.x * a.cols;
+  if constexpr (kRows > 1) {
+    float* mine = join[threadIdx.x / THREADS];
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mine[(v * 8 + i) * THREADS + tid] = gw[v][i];
+    __syncthreads();
+    if (threadIdx.x >= THREADS) return;
+#pragma unroll
+    for (int v = 0; v < VPT; ++v)
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int r = 1; r < kRows; ++r) gw[v][i] += join[r][(v * 8 + i) * THREADS + tid];
+  }
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     const int64_t col = (v * THREADS + tid) * 8;
@@ -301,23 +317,28 @@ __global__ __launch_bounds__(kGroup) void k_norm_bwd_long_w(NormBwdArgs a) {
   Eight<float>::store(a.partials + unit * a.cols, col, a.cols, Eight<float>::V::pack(gw));
 }
 
-// grad_w[c] = sum over the units of partials[unit, c], each column in one fixed order: a workgroup
-// takes 64 columns, its four waves every fourth unit.
+// grad_w[c] = sum over the parts of partials[part, c], each column in one fixed order: a workgroup takes 64
+// columns, its sixteen waves every sixteenth part.  (Four waves took 7.7 us for 512 parts of 16384.)
+constexpr int kSumWaves = 16;
 template <typename TW>
-__global__ __launch_bounds__(kGroup) void k_norm_bwd_w(const float* __restrict__ partials,
-                                                       int64_t units, int64_t cols,
-                                                       TW* __restrict__ out) {
-  __shared__ float lds[kWavesPerGroup][kWave];
+__global__ __launch_bounds__(kSumWaves * kWave) void k_norm_bwd_w(const float* __restrict__ partials,
+                                                                  int64_t parts, int64_t cols,
+                                                                  TW* __restrict__ out) {
+  __shared__ float lds[kSumWaves][kWave];
   const int lane = threadIdx.x % kWave, wave = threadIdx.x / kWave;
   const int64_t col = (int64_t)blockIdx.x * kWave + lane;
   float sum = 0.f;
   if (col < cols) {
 #pragma unroll 8
-    for (int64_t u = wave; u < units; u += kWavesPerGroup) sum += partials[u * cols + col];
+    for (int64_t p = wave; p < parts; p += kSumWaves) sum += partials[p * cols + col];
   }
   lds[wave][lane] = sum;
   __syncthreads();
-  if (wave == 0 && col < cols) st1(out + col, ((lds[0][lane] + lds[1][lane]) + lds[2][lane]) + lds[3][lane]);
+  if (wave == 0 && col < cols) {
+#pragma unroll
+    for (int v = 1; v < kSumWaves; ++v) sum += lds[v][lane];
+    st1(out + col, sum);
+  }
 }
 
 // ---- rows to 8 bits and back ----------------------------------------------------------------
@@ -342,17 +363,17 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_rows8(RowsArgs a) 
 #pragma unroll
   for (int v = 0; v < VPT; ++v) raw[v] = V::template load<true>(x, (v * THREADS + tid) * 8, a.cols);
   float f[VPT][8];
-  uint32_t top = 0;
+  float top = 0.f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     V::V::cvt(raw[v], f[v]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (GELU) f[v][i] = gelu<T>(f[v][i]);
-      top = max(top, abs_bits(f[v][i]));
+      if constexpr (GELU) f[v][i] = gelu<typename Gelu8<T>::type>(f[v][i]);
+      top = larger(top, f[v][i]);
     }
   }
-  const Scale8 s = scale8(group_max<THREADS>(top, lds));
+  const Scale8 s = scale8(group_max<THREADS>(abs_bits(top), lds));
   if (tid == 0) a.scales[row] = s.scale;
   uint8_t* q = a.q + row * a.q_stride;
 #pragma unroll
@@ -373,17 +394,17 @@ __global__ __launch_bounds__(1024) void k_rows8_long(RowsArgs a) {
     V::V::cvt(V::template load<false>(x, col, a.cols), f);
     if constexpr (GELU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = gelu<T>(f[i]);
+      for (int i = 0; i < 8; ++i) f[i] = gelu<typename Gelu8<T>::type>(f[i]);
     }
   };
-  uint32_t top = 0;
+  float top = 0.f;
   for (int64_t col = threadIdx.x * 8; col < a.cols; col += kThreads * 8) {
     float f[8];
     read(col, f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = max(top, abs_bits(f[i]));
+    for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
   }
-  const Scale8 s = scale8(group_max<kThreads>(top, lds));
+  const Scale8 s = scale8(group_max<kThreads>(abs_bits(top), lds));
   if (threadIdx.x == 0) a.scales[row] = s.scale;
   for (int64_t col = threadIdx.x * 8; col < a.q_cols; col += kThreads * 8) {
     float f[8];
@@ -399,25 +420,27 @@ using namespace fmoe;
 namespace {
 
 constexpr int kMaxRegCols = 16384;          // columns that the largest register variant holds
-constexpr int64_t kBwdUnits = 512;          // rows in flight of the backward, as many parts of grad_w
+constexpr int64_t kBwdGroups = 512;         // workgroups of the backward, as many parts of grad_w
 constexpr int64_t kMaxCols = int64_t(1) << 30;
 
-// Calls f(threads, vectors) with the variant that holds a row of `cols`: the fewest threads that
-// need at most four vectors each.
+// Calls f(threads, vectors) with the variant that holds a row of `cols` in at most four vectors a thread.
+// Up to 2048 columns a row is a wave's: no barrier, and more of its loads in flight (GELU to 8 bits of
+// 49152 x 2048: 64 us against 77 with 256 threads; the norm 46 against 48).  At 4096 columns 256
+// threads are better than 512 (43 against 51 us), beyond that there is little between them.
 template <typename F> void by_cols(int64_t cols, F&& f) {
   using std::integral_constant;
   const int64_t v = (cols + 7) / 8;
   auto go = [&](auto t, auto n) { f(t, n); };
   if (v <= 64) go(integral_constant<int, 64>{}, integral_constant<int, 1>{});
   else if (v <= 128) go(integral_constant<int, 64>{}, integral_constant<int, 2>{});
-  else if (v <= 256) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
+  else if (v <= 256) go(integral_constant<int, 64>{}, integral_constant<int, 4>{});
   else if (v <= 512) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
   else if (v <= 1024) go(integral_constant<int, 256>{}, integral_constant<int, 4>{});
   else go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
 }
-// The backward holds three inputs, the weight and its gradient's part: at most two vectors each (four
-// took 250 registers, and 1024 threads of them spilled).
-template <typename F> void by_cols_backward(int64_t cols, F&& f) {
+// The backward holds three inputs, the weight and its gradient's part: two vectors each (four take 250
+// registers).  fp32 rows above 8192 columns take four all the same: two with 1024 threads spill.
+template <typename T, typename F> void by_cols_backward(int64_t cols, F&& f) {
   using std::integral_constant;
   const int64_t v = (cols + 7) / 8;
   auto go = [&](auto t, auto n) { f(t, n); };
@@ -426,6 +449,7 @@ template <typename F> void by_cols_backward(int64_t cols, F&& f) {
   else if (v <= 256) go(integral_constant<int, 256>{}, integral_constant<int, 1>{});
   else if (v <= 512) go(integral_constant<int, 256>{}, integral_constant<int, 2>{});
   else if (v <= 1024) go(integral_constant<int, 512>{}, integral_constant<int, 2>{});
+  else if constexpr (std::is_same<T, float>::value) go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
   else go(integral_constant<int, 1024>{}, integral_constant<int, 2>{});
 }
 
@@ -448,7 +472,7 @@ int check_sizes(const char* who, int64_t rows, int64_t cols, int dtype) {
                (long long)cols);
   FMOE_REQUIRE(fmoe_host::is_float_dtype(dtype), "%s: bad dtype %d", who, dtype);
   // a launch has fewer than 2^32 threads: by_cols's for each row, and a workgroup to spare
-  const int64_t threads = cols <= 1024 ? 64 : cols <= 8192 ? 256 : 1024;
+  const int64_t threads = cols <= 2048 ? 64 : cols <= 8192 ? 256 : 1024;
   if (cols > kMaxCols || rows > ((int64_t(1) << 32) - 1024) / threads) {
     fmoe_host::set_error("%s: rows=%lld or columns=%lld too large", who, (long long)rows,
                          (long long)cols);
@@ -519,7 +543,7 @@ extern "C" int fmoe_add_rms_norm(const void* d_x, int64_t x_row_stride, const vo
 
 extern "C" int64_t fmoe_add_rms_norm_backward_workspace_bytes(int64_t rows, int64_t cols) {
   if (rows < 0 || cols < 1) return -1;
-  return std::max<int64_t>(std::min(rows, kBwdUnits), 1) * cols * 4;
+  return std::max<int64_t>(std::min(rows, kBwdGroups), 1) * cols * 4;
 }
 
 extern "C" int fmoe_add_rms_norm_backward(const void* d_grad_y, int64_t gy_row_stride,
@@ -542,26 +566,29 @@ extern "C" int fmoe_add_rms_norm_backward(const void* d_grad_y, int64_t gy_row_s
                              reinterpret_cast<uintptr_t>(d_workspace) % 16 == 0),
                "%s: the weight's gradient needs an aligned workspace of %lld bytes", who,
                (long long)need);
-  const int64_t units = std::min(rows, kBwdUnits);
-  const NormBwdArgs a{d_grad_y, d_grad_h, d_h, d_weight, d_rstd, gy_row_stride, gh_row_stride,
-                      h_row_stride, rows, cols, d_grad_x,
-                      d_grad_w ? static_cast<float*>(d_workspace) : nullptr, units};
+  NormBwdArgs a{d_grad_y, d_grad_h, d_h, d_weight, d_rstd, gy_row_stride, gh_row_stride,
+                h_row_stride, rows, cols, d_grad_x,
+                d_grad_w ? static_cast<float*>(d_workspace) : nullptr, 0};
   hipStream_t s = static_cast<hipStream_t>(stream);
+  int64_t parts = 0;
   if (rows > 0) {
     by_weight(dtype, weight_dtype, [&](auto t, auto tw) {
       using T = decltype(t);
       using TW = decltype(tw);
       if (cols > kMaxRegCols) {
+        a.units = parts = std::min(rows, kBwdGroups);
         hipLaunchKernelGGL((k_norm_bwd_long<T, TW>), dim3((unsigned)rows), dim3(1024), 0, s, a);
         if (d_grad_w)
           hipLaunchKernelGGL((k_norm_bwd_long_w<T>),
-                             dim3((unsigned)units, (unsigned)((cols + kGroup * 8 - 1) / (kGroup * 8))),
+                             dim3((unsigned)parts, (unsigned)((cols + kGroup * 8 - 1) / (kGroup * 8))),
                              dim3(kGroup), 0, s, a);
         return;
       }
-      by_cols_backward(cols, [&](auto th, auto v) {
-        constexpr int kT = decltype(th)::value;
-        hipLaunchKernelGGL((k_norm_bwd<T, TW, kT, decltype(v)::value>), row_grid<kT>(units),
+      by_cols_backward<T>(cols, [&](auto th, auto v) {
+        constexpr int kT = decltype(th)::value, kRows = rows_per_group<kT>();
+        parts = std::min((rows + kRows - 1) / kRows, kBwdGroups);
+        a.units = parts * kRows;
+        hipLaunchKernelGGL((k_norm_bwd<T, TW, kT, decltype(v)::value>), dim3((unsigned)parts),
                            dim3(group_threads<kT>()), 0, s, a);
       });
     });
@@ -570,7 +597,8 @@ extern "C" int fmoe_add_rms_norm_backward(const void* d_grad_y, int64_t gy_row_s
     by_float(weight_dtype, [&](auto tw) {
       using TW = decltype(tw);
       hipLaunchKernelGGL((k_norm_bwd_w<TW>), dim3((unsigned)((cols + kWave - 1) / kWave)),
-                         dim3(kGroup), 0, s, a.partials, units, cols, static_cast<TW*>(d_grad_w));
+                         dim3(kSumWaves * kWave), 0, s, a.partials, parts, cols,
+                         static_cast<TW*>(d_grad_w));
     });
   return fmoe_host::check_launch(who);
 }

@@ -126,8 +126,12 @@ template <int THREADS> __device__ __forceinline__ float group_sum(float v, float
 }
 
 // ---- the 8-bit form ---------------------------------------------------------------------------
-// |v| as ordered bits: an infinity orders above every number and a NaN above the infinities, so an
-// unsigned maximum finds either (a floating-point maximum would drop a NaN).
+// The largest |v| so far.  `maximum` keeps a NaN (fmax would drop it) and is one instruction for two
+// values (v_maximum3_f32).  Across lanes the result is compared by its bits: an infinity orders above
+// every number and a NaN above the infinities.
+__device__ __forceinline__ float larger(float top, float v) {
+  return __builtin_elementwise_maximum(top, __builtin_fabsf(v));
+}
 __device__ __forceinline__ uint32_t abs_bits(float v) { return __float_as_uint(v) & 0x7fffffffu; }
 
 struct Scale8 {
@@ -172,17 +176,19 @@ __device__ __forceinline__ void unpack8(u32x2 q, float scale, float* v) {
 
 // ---- GELU ---------------------------------------------------------------------------------------
 // gelu(x) = x * Phi(x) with Phi the normal distribution function.  For 16-bit types Phi(x) is
-// 1 / (1 + 2^-(x * P(x^2))): the log-odds of Phi are odd and smooth, so P is a polynomial of degree
-// 8 in x^2, fitted here by reweighted least squares on [0, 5.5^2] (beyond, x^2 is held there and
-// Phi is below 4e-8 from 0 or 1).  x * Phi is within 4e-7 of the true value, and within 2e-5 of
-// it relatively down to x = -5, a twentieth of fp16's half step.  About 20 instructions an
-// element, where erf takes about 50: at 2 bytes an element erf bounds the kernel instead of HBM.
+// 1 / (1 + 2^-(x * P(x^2))): the log-odds of Phi are odd and smooth, so P is a polynomial in x^2,
+// fitted here by reweighted least squares up to |x| = T; beyond, both stay positive and x * P(x^2)
+// rises, so Phi goes to 0 or 1.  With degree 8 and T = 5.5, x * Phi is within 4e-7 of the true value,
+// and relatively within 2e-5 down to x = -T; with degree 6 and T = 5 within 3e-6, relatively 2.4e-4:
+// a sixteenth of bf16's half step, a seventeenth of half an 8-bit step.  13 and 11 instructions and
+// two quarter-rate ones (2^x, 1 / x) an element, where erf takes about 50: at 2 bytes an element
+// those bound the kernels instead of HBM.
 // fp32 values take erfc, which is exact to its last bits.
 template <typename T> __device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (ElemInfo<T>::kBytes == 4) {
     return 0.5f * erfcf(-0.70710678118654752f * x);
-  } else {
-    const float u = __builtin_fminf(x * x, 30.25f);
+  } else if constexpr (std::is_same<T, f16_t>::value) {
+    const float u = x * x;
     float p = 1.4901355e-12f;
     p = __builtin_fmaf(p, u, -2.3464275e-10f);
     p = __builtin_fmaf(p, u, 1.5883325e-08f);
@@ -193,13 +199,27 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float x) {
     p = __builtin_fmaf(p, u, 1.0480524e-01f);
     p = __builtin_fmaf(p, u, 2.3022187f);
     return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-(p * x)));
+  } else {
+    const float u = x * x;
+    float p = 2.4839388e-09f;
+    p = __builtin_fmaf(p, u, -2.2724015e-07f);
+    p = __builtin_fmaf(p, u, 8.1067028e-06f);
+    p = __builtin_fmaf(p, u, -1.2739214e-04f);
+    p = __builtin_fmaf(p, u, -2.3266282e-04f);
+    p = __builtin_fmaf(p, u, 1.0507021e-01f);
+    p = __builtin_fmaf(p, u, 2.3020976f);
+    return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-(p * x)));
   }
 }
-// An infinite x gives x * Phi(x) = inf * 1 or -inf * 0; the latter is -0 in the limit.
+// x = -inf would give -inf * 0: the least number stands for it, whose GELU is -0, the limit.  (`maximum`
+// keeps a NaN.)
 template <typename T> __device__ __forceinline__ float gelu(float x) {
-  const float c = normal_cdf<T>(x);
-  return c == 0.f ? -0.f : x * c;
+  x = __builtin_elementwise_maximum(x, -3.402823466e38f);
+  return x * normal_cdf<T>(x);
 }
+// The type whose GELU is close enough for a result of 8 bits.
+template <typename T> struct Gelu8 { using type = bf16_t; };
+template <> struct Gelu8<float> { using type = float; };
 // d gelu / dx = Phi(x) + x * phi(x)
 template <typename T> __device__ __forceinline__ float gelu_slope(float x, float cdf) {
   const float e = __builtin_amdgcn_exp2f(-0.72134752f * x * x);

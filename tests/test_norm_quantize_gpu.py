@@ -167,6 +167,12 @@ def test_strided_rows_and_odd_starts():
     assert torch.equal(a, b)
 
 
+# GELU's error beside rounding, as the kernels state it: fp32 erfc; polynomials for 16-bit types (bf16's
+# degree also serves every 16-bit type whose result has 8 bits)
+ERROR = {torch.float32: (16 * U, 1e-7), torch.float16: (2e-5, 4e-7), torch.bfloat16: (2.4e-4, 3e-6)}
+ERROR8 = {torch.float32: 1e-7, torch.float16: 3e-6, torch.bfloat16: 3e-6}
+
+
 def cdf64(x):
     return 0.5 * torch.erfc(-x * 0.5 ** 0.5)
 
@@ -179,14 +185,15 @@ def test_quantize_rows(C, dtype):
     check_rows8(q, x.double(), 0)
     back = q.dequantize(dtype)
     close(back, q.data[:, :C].double() * q.scales.double().unsqueeze(1), half(dtype) + U, 2.0 ** -25)
-    # GELU in fp32 is within 6e-7 of the value, which is at least 0.01 in a row of five normal values
+    # GELU is within e of the value: the scale within e / 127, so 127 steps within e, and the value itself
+    e = ERROR8[dtype] + 16 * U * float(x.double().abs().max())
     v = x.double() * cdf64(x.double())
     g = fm.quantize_rows(x, activation="gelu")
     top = v.abs().amax(-1)
-    close(g.scales, top / 127, 8 * U, 6e-7 / 127)
+    close(g.scales, top / 127, 8 * U, e / 127)
     step = g.scales.double().unsqueeze(-1)
     err = (g.data[:, :C].double() * step - v).abs()
-    assert (err <= 0.5 * step + 1.3e-6 + 64 * U * v.abs()).all()
+    assert (err <= 0.5 * step + 2 * e + 64 * U * v.abs()).all()
 
 
 @pytest.mark.parametrize("dtype", TYPES)
@@ -254,12 +261,17 @@ def test_held_rows_and_gelu(R, C, dtype):
     a, again_held = fm.gelu_compress(x)
     assert torch.equal(again_held.data, held.data) and torch.equal(again_held.scales, held.scales)
     x64 = x.double()
-    close(a, x64 * cdf64(x64), half(dtype) + 16 * U, 6e-7)
+    _, absolute = ERROR[dtype]
+    close(a, x64 * cdf64(x64), half(dtype) + 16 * U, absolute + 2.0 ** -25)
     again, grad = fm.gelu_compressed_backward(held, ga)
     value = value.float().double()  # q * s is rounded once to fp32
-    close(again, value * cdf64(value), half(dtype) + 16 * U, 6e-7)
+    close(again, value * cdf64(value), half(dtype) + 16 * U, absolute + 2.0 ** -25)
     slope = cdf64(value) + value * torch.exp(-value ** 2 / 2) * 0.3989422804014327
-    close(grad, ga.double() * slope, half(dtype), 2e-6 * ga.double().abs() + 2.0 ** -25)
+    # Phi = (x * Phi) / x: where |x| is small its log-odds' error, at most the relative one, counts a
+    # quarter; phi and the sums add a few u
+    rel, _ = ERROR[dtype]
+    close(grad, ga.double() * slope, half(dtype),
+          (min(rel / 4, 10 * absolute) + 64 * U) * ga.double().abs() + 2.0 ** -25)
     none, grad2 = fm.gelu_compressed_backward(held, ga, again=False)
     assert none is None and torch.equal(grad, grad2)
 
@@ -279,10 +291,10 @@ def test_gelu_over_its_whole_range(dtype):
     a, _ = fm.gelu_compress(x)
     x64 = x.double()
     want = x64 * cdf64(x64)
-    close(a, want, half(dtype) + 16 * U, 6e-7)
-    if dtype is not torch.float32:  # the polynomial also holds relatively where fp16 can tell
-        at = (x64 < -0.01) & (x64 > -3.5)
-        close(a[at], want[at], half(dtype) * 2 + 4e-5, 2.0 ** -25)
+    rel, absolute = ERROR[dtype]
+    close(a, want, half(dtype) + 16 * U, absolute + 2.0 ** -25)
+    at = (x64 < -0.01) & (x64 > -3.5)  # and relatively, where 1 + erf would have lost its bits
+    close(a[at], want[at], half(dtype) + rel + 16 * U, 2.0 ** -25)
 
 
 def test_another_stream():
