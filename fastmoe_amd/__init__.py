@@ -5,7 +5,14 @@ The operator API mirrors ``fastmoe.kernels.ops``; the work runs in hand-written 
 """
 from .consts import MoEImplementation
 from .dispatch import PermutedTokens, permute_tokens
-from .moe import MoEFeedForward, compute_experts, gate_and_sort, unpermute
+from .moe import (
+    Int8MoEFeedForward,
+    MoEFeedForward,
+    NormedMoEFeedForward,
+    compute_experts,
+    gate_and_sort,
+    unpermute,
+)
 from .ops import (
     GroupedMetadata,
     GroupedWeightedScatterAdd,
@@ -36,10 +43,12 @@ __all__ = [
     "CompressedRows",
     "GroupedMetadata",
     "GroupedWeightedScatterAdd",
+    "Int8MoEFeedForward",
     "Int8NormedRows",
     "Int8Weights",
     "MoEFeedForward",
     "MoEImplementation",
+    "NormedMoEFeedForward",
     "PermutedTokens",
     "QuantizedRows",
     "add_rms_norm",

@@ -16,6 +16,13 @@ ragged per-expert list instead of a ``torch.cat`` of it:
   MoEFeedForward   the layer wiring these stages (router + experts as in :66-77)
 
 The router GEMM, top-k, softmax and the expert MLPs are torch library calls, as in the reference.
+
+Beyond the reference, on the 8-bit operators of ``quantize``:
+
+  compute_experts(..., checkpoint="int8")  holds the experts' inputs and hidden rows in 8 bits until
+                              the backward (``MoEFeedForward(..., checkpoint="int8")``)
+  NormedMoEFeedForward        the layer behind a root-mean-square norm with the residual's addition
+  Int8MoEFeedForward          either layer for serving, with rows and experts' weights in 8 bits
 """
 from __future__ import annotations
 
@@ -27,10 +34,21 @@ import torch.nn.functional as F
 
 from .consts import MoEImplementation
 from .dispatch import PermutedTokens, permute_tokens
-from .ops import (_apply, _combine_forward, _GroupedCombinePermuted, _runs_plain,
-                  grouped_weighted_scatter_add)
+from .ops import (_apply, _combine_forward, _GroupedCombinePermuted, _refuse_autograd_capture,
+                  _runs_plain, grouped_weighted_scatter_add)
+from .quantize import (CompressedRows, Int8Weights, _check_matrix, _compress, add_rms_norm,
+                       add_rms_norm_int8, gelu_compressed_backward, int8_linear, quantize_rows,
+                       quantize_weights, restore_rows)
 
-__all__ = ["MoEFeedForward", "compute_experts", "gate_and_sort", "unpermute"]
+__all__ = ["Int8MoEFeedForward", "MoEFeedForward", "NormedMoEFeedForward", "compute_experts",
+           "gate_and_sort", "unpermute"]
+
+
+def _route(x_flat: torch.Tensor, router: nn.Module, top_k: int):
+    """(gates in x's type, expert ids), each [T, k] (tiny_model.py:92-100)."""
+    logits = router(x_flat)
+    topk_weights, topk_indices = torch.topk(logits, top_k, dim=-1)
+    return F.softmax(topk_weights, dim=-1, dtype=torch.float32).type_as(x_flat), topk_indices
 
 
 def gate_and_sort(x: torch.Tensor, router: nn.Module, top_k: int, num_experts: int):
@@ -42,9 +60,7 @@ def gate_and_sort(x: torch.Tensor, router: nn.Module, top_k: int, num_experts: i
     """
     B, T, D = x.shape
     x_flat = x.reshape(-1, D)
-    logits = router(x_flat)
-    topk_weights, topk_indices = torch.topk(logits, top_k, dim=-1)
-    topk_weights = F.softmax(topk_weights, dim=-1, dtype=torch.float32).type_as(x)
+    topk_weights, topk_indices = _route(x_flat, router, top_k)
     p = permute_tokens(x_flat, topk_indices, topk_weights, num_experts)
     rank_counts = torch.tensor([p.permuted_data.shape[0]], device=x.device, dtype=torch.long)
     return _Routed((p.permuted_data, rank_counts, p.expert_counts.view(1, num_experts),
@@ -61,9 +77,22 @@ class _Routed(tuple):
 
 
 def compute_experts(experts: Sequence[nn.Module], recv_data: torch.Tensor,
-                    tokens_per_expert: Sequence[int]) -> List[torch.Tensor]:
+                    tokens_per_expert: Sequence[int], *,
+                    checkpoint: Optional[str] = None) -> List[torch.Tensor]:
     """Each expert on its own rows (tiny_model.py:282-291); the per-expert outputs stay separate
-    allocations (no :294 cat).  An expert with no rows yields an empty [0, D] tensor."""
+    allocations (no :294 cat).  An expert with no rows yields an empty [0, D] tensor.
+
+    ``checkpoint="int8"`` (experts ``Sequential(Linear, GELU(), Linear)``) keeps for the backward the
+    rows and the first product in 8 bits, a scale for every 128 columns, instead of the rows, the
+    first product and GELU's output in their own type: about D + F bytes a row instead of 2 D + 4 F at 16
+    bits.  The forward is exact; the gradients are those of the held values (each within 1/254 of
+    its block's largest).  Rows and weights share one dtype (autocast's, where it is on).
+    """
+    if checkpoint is not None:
+        if checkpoint != "int8":
+            raise ValueError(f"fastmoe_amd: unknown checkpoint {checkpoint!r} (expected None or "
+                             "'int8')")
+        return _compute_experts_held(experts, recv_data, [int(n) for n in tokens_per_expert])
     chunks = recv_data.split(list(tokens_per_expert), dim=0)
     out = []
     for chunk, expert in zip(chunks, experts):
@@ -73,6 +102,128 @@ def compute_experts(experts: Sequence[nn.Module], recv_data: torch.Tensor,
             out.append(torch.empty(0, recv_data.shape[1], device=recv_data.device,
                                    dtype=recv_data.dtype))
     return out
+
+
+def _mlp_parameters(experts: Sequence[nn.Module]):
+    """[(w1, b1, w2, b2), ...] of experts Sequential(Linear, GELU(), Linear); biases may be None."""
+    out = []
+    for e, expert in enumerate(experts):
+        parts = list(expert.children()) if isinstance(expert, nn.Sequential) else []
+        if (len(parts) != 3 or not isinstance(parts[0], nn.Linear)
+                or not isinstance(parts[1], nn.GELU) or not isinstance(parts[2], nn.Linear)):
+            raise TypeError(f"fastmoe_amd: expert {e} is not Sequential(Linear, GELU, Linear)")
+        if parts[1].approximate != "none":
+            raise ValueError(f"fastmoe_amd: expert {e} has a GELU approximation "
+                             f"({parts[1].approximate!r}); the 8-bit operators compute the exact form")
+        out.append((parts[0].weight, parts[0].bias, parts[2].weight, parts[2].bias))
+        if any(getattr(p, "_forward_hooks", None) or getattr(p, "_forward_pre_hooks", None)
+               for p in (expert, *parts)):
+            raise ValueError(f"fastmoe_amd: expert {e} has forward hooks, which the 8-bit operators "
+                             "would not call")
+    if not out:
+        raise ValueError("fastmoe_amd: no experts")
+    return out
+
+
+def _compute_experts_held(experts, recv_data, counts) -> List[torch.Tensor]:
+    params = _mlp_parameters(experts)
+    if torch.is_autocast_enabled("cuda"):
+        dtype = torch.get_autocast_dtype("cuda")
+        recv_data = recv_data.to(dtype)
+        params = [tuple(None if t is None else t.to(dtype) for t in p) for p in params]
+    _check_matrix(recv_data, "recv_data")
+    N, D = recv_data.shape
+    hidden = params[0][0].shape[0]
+    if len(counts) != len(params) or sum(counts) != N or min(counts) < 0:
+        raise ValueError(f"fastmoe_amd: tokens_per_expert {counts} does not split {N} rows over "
+                         f"{len(params)} experts")
+    for e, (w1, b1, w2, b2) in enumerate(params):
+        if tuple(w1.shape) != (hidden, D) or w2.shape[1] != hidden or w2.shape[0] != params[0][2].shape[0]:
+            raise ValueError(f"fastmoe_amd: expert {e} has weights {tuple(w1.shape)} and "
+                             f"{tuple(w2.shape)}; expert 0 has ({hidden}, {D}) and "
+                             f"{tuple(params[0][2].shape)}")
+        for t in (w1, b1, w2, b2):
+            if t is not None and (t.dtype != recv_data.dtype or t.device != recv_data.device):
+                raise TypeError(f"fastmoe_amd: expert {e} has {t.dtype} parameters on {t.device}, "
+                                f"the rows are {recv_data.dtype} on {recv_data.device}")
+    flat = [t for p in params for t in p]
+    records = torch.is_grad_enabled() and any(
+        t is not None and t.requires_grad for t in (recv_data, *flat))
+    _refuse_autograd_capture("the experts with held activations", recv_data, records)
+    # autocast has done its casts: the products below run in the rows' type
+    with torch.autocast("cuda", enabled=False):
+        return list(_HeldExperts.apply(counts, recv_data, *flat))
+
+
+def _mm(x, w, bias, out):
+    """out = x @ w + bias"""
+    if bias is None:
+        torch.mm(x, w, out=out)
+    else:
+        torch.addmm(bias, x, w, out=out)
+
+
+class _HeldExperts(torch.autograd.Function):
+    """Every expert's Linear, GELU, Linear over the packed rows; what the backward needs of the
+    activations is held in 8 bits.  One launch each way holds or restores all experts' rows."""
+
+    @staticmethod
+    def forward(ctx, counts, x, *flat):
+        params = [flat[i:i + 4] for i in range(0, len(flat), 4)]
+        h = x.new_empty((x.shape[0], params[0][0].shape[0]))
+        for xe, he, (w1, b1, _, _) in zip(x.split(counts), h.split(counts), params):
+            if xe.shape[0]:
+                _mm(xe, w1.t(), b1, he)
+        a, held_h = _compress(h, True)
+        del h
+        outs = []
+        for ae, (_, _, w2, b2) in zip(a.split(counts), params):
+            y = a.new_empty((ae.shape[0], w2.shape[0]))
+            if ae.shape[0]:
+                _mm(ae, w2.t(), b2, y)
+            outs.append(y)
+        held_x = _compress(x, False)[1] if any(ctx.needs_input_grad[2::4]) else None
+        ctx.counts, ctx.dtype = counts, x.dtype
+        ctx.features = (x.shape[1], a.shape[1])
+        ctx.save_for_backward(held_h.data, held_h.scales, *(held_x[:2] if held_x else (None, None)),
+                              *flat)
+        ctx.set_materialize_grads(False)
+        return tuple(outs)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, *grads):
+        hd, hs, xd, xs, *flat = ctx.saved_tensors
+        _refuse_autograd_capture("the held experts' backward", hd)
+        counts, (D, hidden) = ctx.counts, ctx.features
+        params = [flat[i:i + 4] for i in range(0, len(flat), 4)]
+        needs = ctx.needs_input_grad[2:]
+        N = hd.shape[0]
+        da = torch.empty((N, hidden), dtype=ctx.dtype, device=hd.device)
+        for g, de, (_, _, w2, _) in zip(grads, da.split(counts), params):
+            if g is None:
+                de.zero_()  # this expert's output had no part in the loss
+            elif de.shape[0]:
+                torch.mm(g, w2, out=de)
+        a, dh = gelu_compressed_backward(CompressedRows(hd, hs, hidden), da, again=any(needs[2::4]))
+        del da
+        x = None
+        if any(needs[0::4]):
+            x = restore_rows(CompressedRows(xd, xs, D), ctx.dtype).split(counts)
+        dx = torch.empty((N, D), dtype=ctx.dtype, device=hd.device) if ctx.needs_input_grad[1] else None
+        dxs = dx.split(counts) if dx is not None else None
+        a = a.split(counts) if a is not None else None
+        out = []
+        for e, (g, he, (w1, _, w2, _)) in enumerate(zip(grads, dh.split(counts), params)):
+            n1, nb1, n2, nb2 = needs[4 * e:4 * e + 4]
+            live = counts[e] > 0 and g is not None
+            if dx is not None and counts[e]:
+                torch.mm(he, w1, out=dxs[e])
+            out += [torch.mm(he.t(), x[e]) if n1 and live else None,
+                    he.sum(0) if nb1 and live else None,
+                    torch.mm(g.t(), a[e]) if n2 and live else None,
+                    g.sum(0) if nb2 and live else None]
+        return (None, dx, *out)
 
 
 def unpermute(x_out: Union[torch.Tensor, Sequence[torch.Tensor]], reverse_map_indices: torch.Tensor,
@@ -111,11 +262,18 @@ def unpermute(x_out: Union[torch.Tensor, Sequence[torch.Tensor]], reverse_map_in
 
 class MoEFeedForward(nn.Module):
     """MoE feed-forward layer of tiny_model.py:42-77 on one GPU: router, E experts
-    (Linear -> GELU -> Linear), HIP permutation, per-expert compute, grouped combine."""
+    (Linear -> GELU -> Linear), HIP permutation, per-expert compute, grouped combine.
+
+    ``checkpoint="int8"`` holds the experts' activations in 8 bits until the backward (see
+    ``compute_experts``); :meth:`int8` makes the layer that serves with 8-bit rows and weights."""
 
     def __init__(self, dim: int, ff_dim: int, num_experts: int, top_k: int,
-                 implementation=MoEImplementation.FAST) -> None:
+                 implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None) -> None:
         super().__init__()
+        if checkpoint not in (None, "int8"):
+            raise ValueError(f"fastmoe_amd: unknown checkpoint {checkpoint!r} (expected None or "
+                             "'int8')")
+        self.checkpoint = checkpoint
         self.dim = dim
         self.num_experts = num_experts
         self.top_k = top_k
@@ -130,8 +288,106 @@ class MoEFeedForward(nn.Module):
         permuted, _, counts_by_rank, rev, weights, shape = routed
         # the split sizes go to the host, as in the reference (recv_splits .tolist(), :197-207)
         tokens_per_expert = counts_by_rank.view(-1).tolist()
-        outs = compute_experts(self.experts, permuted, tokens_per_expert)
+        outs = compute_experts(self.experts, permuted, tokens_per_expert,
+                               checkpoint=self.checkpoint)
         if self.implementation == MoEImplementation.FAST:
             return unpermute(outs, rev, weights, shape, self.implementation,
                              permutation=routed.permutation)
         return unpermute(torch.cat(outs, 0), rev, weights, shape, self.implementation)
+
+    def int8(self) -> "Int8MoEFeedForward":
+        """This layer for serving, its experts' weights in 8 bits (a copy: later changes of this layer
+        do not reach it)."""
+        return Int8MoEFeedForward(self)
+
+
+class NormedMoEFeedForward(nn.Module):
+    """A :class:`MoEFeedForward` behind the root-mean-square norm of a pre-norm block: the residual's
+    addition and the norm are one kernel (``add_rms_norm``).  ``forward(x, residual=None)`` returns
+    ``(moe(norm(x + residual)), x + residual)``: the layer's output and the stream it is added to."""
+
+    def __init__(self, moe: MoEFeedForward, eps: float = 1e-6) -> None:
+        super().__init__()
+        self.moe = moe
+        self.eps = eps
+        self.norm_weight = nn.Parameter(torch.ones(moe.dim, dtype=moe.router.weight.dtype,
+                                                   device=moe.router.weight.device))
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        flat = None if residual is None else residual.reshape(-1, x.shape[-1])
+        y, stream = add_rms_norm(x.reshape(-1, x.shape[-1]), self.norm_weight, flat, eps=self.eps)
+        return self.moe(y.view(x.shape)), stream.view(x.shape)
+
+    def int8(self) -> "Int8MoEFeedForward":
+        """As :meth:`MoEFeedForward.int8`, the norm included."""
+        return Int8MoEFeedForward(self.moe, self.norm_weight, self.eps)
+
+
+class Int8MoEFeedForward(nn.Module):
+    """An MoE layer for serving in 8 bits: rows with one scale each, experts' weights with one scale for
+    each output (Linear -> GELU -> Linear, biases in their own type).  Made by
+    :meth:`MoEFeedForward.int8` or :meth:`NormedMoEFeedForward.int8`.
+
+    ``forward(x)`` without a norm returns the layer's output; with one, ``forward(x, residual=None)``
+    returns ``(output, x + residual)``.  The router stays in its own type and reads the unquantised
+    rows.  The experts' first product reads each token's 8-bit row through the reverse map: no
+    [T*k, D] copy of the rows is made.  The host reads nothing back, so a call can be captured in a
+    HIP graph.  No gradients; convert the layer to its type before making this one (casting it
+    later would cast the scales, which the products refuse).
+    """
+
+    def __init__(self, moe: MoEFeedForward, norm_weight: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6) -> None:
+        super().__init__()
+        params = _mlp_parameters(moe.experts)
+        self.dim, self.num_experts, self.top_k, self.eps = moe.dim, moe.num_experts, moe.top_k, eps
+        self.hidden = params[0][0].shape[0]
+        self.router = nn.Linear(moe.dim, moe.num_experts, bias=moe.router.bias is not None,
+                                dtype=moe.router.weight.dtype, device=moe.router.weight.device)
+        self.router.load_state_dict(moe.router.state_dict())
+        self.router.requires_grad_(False)
+
+        def keep(name, t):
+            self.register_buffer(name, None if t is None else t.detach().clone())
+
+        keep("norm_weight", norm_weight)
+        for i, name in ((0, "1"), (2, "2")):
+            w = quantize_weights([p[i] for p in params])
+            self.register_buffer("w" + name, w.data)
+            self.register_buffer("s" + name, w.scales)
+            biases = [p[i + 1] for p in params]
+            if any((b is None) != (biases[0] is None) for b in biases):
+                raise ValueError("fastmoe_amd: some experts have biases and some have none")
+            keep("b" + name, None if biases[0] is None else torch.stack([b.detach() for b in biases]))
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        if x.dim() != 3 or x.shape[2] != self.dim:
+            raise ValueError(f"fastmoe_amd: x must be [batch, tokens, {self.dim}], got "
+                             f"{tuple(x.shape)}")
+        B, T, D = x.shape
+        flat = x.reshape(-1, D)
+        if self.norm_weight is None:
+            if residual is not None:
+                raise ValueError("fastmoe_amd: a residual needs the norm (NormedMoEFeedForward.int8)")
+            rows, y = quantize_rows(flat), flat
+        else:
+            if residual is not None and residual.shape != x.shape:
+                raise ValueError(f"fastmoe_amd: residual must be {tuple(x.shape)}, got "
+                                 f"{tuple(residual.shape)}")
+            rows, y, stream = add_rms_norm_int8(
+                flat, self.norm_weight, None if residual is None else residual.reshape(-1, D),
+                eps=self.eps)
+        if flat.shape[0] == 0:
+            out = x.new_empty(x.shape)
+        else:
+            gates, ids = _route(y, self.router, self.top_k)
+            # the sort alone: what it gathers are the rows' scales, four bytes each
+            p = permute_tokens(rows.scales.view(-1, 1), ids, gates, self.num_experts)
+            h = int8_linear(rows, Int8Weights(self.w1, self.s1, D), p.expert_offsets,
+                            rows=p.reverse_map_indices, bias=self.b1, out_dtype=x.dtype)
+            h = int8_linear(quantize_rows(h, activation="gelu"),
+                            Int8Weights(self.w2, self.s2, self.hidden), p.expert_offsets,
+                            bias=self.b2, out_dtype=x.dtype)
+            out = unpermute(h, p.reverse_map_indices, p.sorted_weights, (B, T), permutation=p)
+        return out if self.norm_weight is None else (out, stream.view(x.shape))

@@ -1,0 +1,340 @@
+"""The 8-bit operators run together: the serving layer, the held experts' training step, and the layer
+behind its norm."""
+from __future__ import annotations
+
+import pytest
+import torch
+import torch.nn as nn
+
+import fastmoe_amd as fm
+
+pytestmark = pytest.mark.gpu
+U = 2.0 ** -24
+
+
+def layer(dim, ff, E, k, dtype=torch.bfloat16, seed=0, bias=False, **kw):
+    torch.manual_seed(seed)
+    moe = fm.MoEFeedForward(dim, ff, E, k, **kw)
+    if bias:
+        for e in moe.experts:
+            e[0].bias = nn.Parameter(torch.randn(ff) * 0.1)
+            e[2].bias = nn.Parameter(torch.randn(dim) * 0.1)
+    return moe.cuda().to(dtype)
+
+
+def rand(*shape, dtype=torch.float32, seed=0):
+    g = torch.Generator(device="cuda").manual_seed(seed)
+    return torch.randn(*shape, generator=g, device="cuda").to(dtype)
+
+
+def by_hand(moe, x, norm_weight=None, residual=None):
+    """The layer's calls one after the other, as a user would write them."""
+    flat = x.reshape(-1, x.shape[-1])
+    if norm_weight is None:
+        rows, y, stream = fm.quantize_rows(flat), flat, None
+    else:
+        rows, y, stream = fm.add_rms_norm_int8(
+            flat, norm_weight, None if residual is None else residual.reshape(flat.shape))
+    logits = moe.router(y)
+    gates, ids = torch.topk(logits, moe.top_k, dim=-1)
+    gates = torch.softmax(gates, dim=-1, dtype=torch.float32).to(x.dtype)
+    p = fm.permute_tokens(flat, ids, gates, moe.num_experts)
+    w1 = fm.quantize_weights([e[0].weight for e in moe.experts])
+    w2 = fm.quantize_weights([e[2].weight for e in moe.experts])
+    b1, b2 = ([e[i].bias for e in moe.experts] for i in (0, 2))
+    b1, b2 = (None if b[0] is None else torch.stack(b) for b in (b1, b2))
+    h = fm.int8_linear(rows, w1, p.expert_offsets, rows=p.reverse_map_indices, bias=b1,
+                       out_dtype=x.dtype)
+    y2 = fm.int8_linear(fm.quantize_rows(h, activation="gelu"), w2, p.expert_offsets, bias=b2,
+                        out_dtype=x.dtype)
+    out = fm.weighted_scatter_add(y2, p.reverse_map_indices, p.sorted_weights, flat.shape)
+    return out.view(x.shape), stream, (rows, w1, w2, p, gates, ids, h)
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("B,T,dim,ff,E,k", [(1, 1, 64, 32, 4, 2), (2, 33, 200, 72, 7, 3),
+                                            (4, 300, 256, 512, 8, 2), (1, 2048, 128, 256, 16, 4)])
+def test_serving_layer_is_its_calls(B, T, dim, ff, E, k, dtype, bias):
+    moe = layer(dim, ff, E, k, dtype, bias=bias)
+    x = rand(B, T, dim, dtype=dtype, seed=1)
+    with torch.no_grad():
+        want, _, _ = by_hand(moe, x)
+        got = moe.int8()(x)
+    assert torch.equal(got, want) and not got.requires_grad
+
+
+def test_serving_layer_against_64_bits():
+    """Within what 8 bits can be off, counted through the layer: every row value by half its scale, every
+    weight by half of its; GELU's slope is at most 1.13; then the roundings to bf16."""
+    dim, ff, E, k = 256, 128, 6, 2
+    moe = layer(dim, ff, E, k, bias=True)
+    x = rand(1, 50, dim, dtype=torch.bfloat16, seed=3)
+    with torch.no_grad():
+        got = moe.int8()(x).double().view(-1, dim)
+        _, _, (rows, w1, w2, p, gates, ids, h) = by_hand(moe, x)
+        q2 = fm.quantize_rows(h, activation="gelu")
+        half = 2.0 ** -8
+        x64, out, bound = x.double().view(-1, dim), torch.zeros_like(got), torch.zeros_like(got)
+        for slot, token in enumerate(p.reverse_map_indices.tolist()):
+            e = int(torch.searchsorted(p.expert_offsets, slot, right=True)) - 1
+            a, b, c, d = (t.double() for t in (moe.experts[e][0].weight, moe.experts[e][0].bias,
+                                               moe.experts[e][2].weight, moe.experts[e][2].bias))
+            gate = float(p.sorted_weights[slot])
+            row = x64[token]
+            dx = torch.full_like(row, float(rows.scales[token]) * 0.501)
+            dw = w1.scales[e].double().unsqueeze(1) * 0.501
+            pre = a @ row + b
+            dpre = a.abs() @ dx + (dw * (row.abs() + dx)).sum(1)
+            dpre = dpre + half * (pre.abs() + dpre)
+            act = pre * 0.5 * torch.erfc(-pre * 0.5 ** 0.5)
+            dact = 1.13 * dpre + 4e-6 + float(q2.scales[slot]) * 0.501
+            dw = w2.scales[e].double().unsqueeze(1) * 0.501
+            y = c @ act + d
+            dy = c.abs() @ dact + (dw * (act.abs() + dact)).sum(1)
+            dy = dy + half * (y.abs() + dy)
+            out[token] += gate * y
+            bound[token] += abs(gate) * dy
+        bound += half * (out.abs() + bound)
+    err = (got - out).abs()
+    assert (err <= bound).all()
+    # and far below it in the mean: roundings do not all point one way
+    assert float(err.norm() / out.norm()) < 0.05
+
+
+@pytest.mark.parametrize("with_residual", [False, True])
+def test_normed_layer_trains_and_serves(with_residual):
+    B, T, dim = 2, 20, 96
+    block = fm.NormedMoEFeedForward(layer(dim, 64, 5, 2, torch.float32)).cuda()
+    with torch.no_grad():
+        block.norm_weight.copy_(1 + 0.1 * rand(dim))
+    x = rand(B, T, dim, seed=1).requires_grad_(True)
+    r = rand(B, T, dim, seed=2).requires_grad_(True) if with_residual else None
+    out, stream = block(x, r)
+    h = x if r is None else x + r
+    assert torch.equal(stream, h)
+    y = h * torch.rsqrt(h.square().mean(-1, keepdim=True) + 1e-6) * block.norm_weight
+    want = block.moe(y)
+    assert (out - want).abs().max() <= 1e-4  # the norm's 64 u and the products' sums of 96 terms
+    leaves = [t for t in (x, r, block.norm_weight, *block.moe.parameters()) if t is not None]
+    g, gs = rand(B, T, dim, seed=5), rand(B, T, dim, seed=6)
+    got = torch.autograd.grad([out, stream], leaves, [g, gs], allow_unused=True)
+    ref = torch.autograd.grad([want, h], leaves, [g, gs], allow_unused=True)
+    for a, b in zip(got, ref):
+        assert (a is None) == (b is None)
+        if a is not None:
+            assert (a - b).norm() <= 1e-4 * b.norm() + 1e-6
+    serve = block.int8()
+    with torch.no_grad():
+        o, s = serve(x, r)
+        hand, hs, _ = by_hand(block.moe, x, block.norm_weight, r)
+    assert torch.equal(o, hand) and torch.equal(s.view(-1, dim), hs)
+
+
+def test_serving_layer_in_a_graph():
+    """Captured once, replayed on other tokens: routing, products and combine follow the new rows."""
+    block = fm.NormedMoEFeedForward(layer(256, 128, 8, 2)).cuda().to(torch.bfloat16).int8()
+    x, r = rand(1, 24, 256, dtype=torch.bfloat16), rand(1, 24, 256, dtype=torch.bfloat16, seed=1)
+    s = torch.cuda.Stream()
+    s.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(s):
+        for _ in range(2):
+            block(x, r)
+    torch.cuda.current_stream().wait_stream(s)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out, stream = block(x, r)
+    for seed in (7, 8, 9):
+        x.copy_(rand(1, 24, 256, dtype=torch.bfloat16, seed=seed))
+        g.replay()
+        torch.cuda.synchronize()
+        want, want_stream = block(x, r)
+        assert torch.equal(out, want) and torch.equal(stream, want_stream)
+
+
+def test_serving_layer_state_and_refusals():
+    moe = layer(128, 64, 4, 2)
+    a, b = moe.int8(), layer(128, 64, 4, 2, seed=9).int8()
+    x = rand(1, 6, 128, dtype=torch.bfloat16)
+    b.load_state_dict(a.state_dict())
+    assert torch.equal(a(x), b(x))
+    assert a(x[:, :0]).shape == (1, 0, 128)
+    with pytest.raises(ValueError, match="batch"):
+        a(x[0])
+    with pytest.raises(ValueError, match="needs the norm"):
+        a(x, x)
+    with pytest.raises(TypeError, match="float32"):
+        a.to(torch.float16)(x.half())
+    tanh = layer(128, 64, 4, 2)
+    tanh.experts[1][1] = nn.GELU(approximate="tanh")
+    with pytest.raises(ValueError, match="approximation"):
+        tanh.int8()
+    other = layer(128, 64, 4, 2)
+    other.experts[0][1] = nn.ReLU()
+    with pytest.raises(TypeError, match="Sequential"):
+        other.int8()
+    mixed = layer(128, 64, 4, 2)
+    mixed.experts[0][0].bias = nn.Parameter(torch.zeros(64, device="cuda", dtype=torch.bfloat16))
+    with pytest.raises(ValueError, match="some have none"):
+        mixed.int8()
+
+
+def held64(x):
+    """The values that compress_rows holds, in 64 bits."""
+    h = fm.compress_rows(x.detach())
+    blocks = h.scales.shape[1]
+    v = h.data.double().view(x.shape[0], blocks, 128) * h.scales.double().unsqueeze(-1)
+    return v.view(x.shape[0], -1)[:, :x.shape[1]].float().double()
+
+
+def cdf64(x):
+    return 0.5 * torch.erfc(-x * 0.5 ** 0.5)
+
+
+def slope64(x):
+    return cdf64(x) + x * torch.exp(-x * x / 2) * 0.3989422804014327
+
+
+@pytest.mark.parametrize("bias", [False, True])
+@pytest.mark.parametrize("counts", [[5, 0, 17, 1], [40], [0, 0, 3], [0, 0]])
+def test_held_experts_against_the_formula(counts, bias):
+    D, H = 150, 200
+    moe = layer(D, H, len(counts), 1, torch.float32, bias=bias)
+    N = sum(counts)
+    x = rand(N, D, seed=1).requires_grad_(True)
+    outs = fm.compute_experts(moe.experts, x, counts, checkpoint="int8")
+    params = list(moe.experts.parameters())
+    grads = [rand(n, D, seed=10 + e) for e, n in enumerate(counts)]
+    got = torch.autograd.grad(outs, [x, *params], grads, allow_unused=True)
+    got = dict(zip([id(x), *map(id, params)], got))
+    xh = held64(x) if N else x.detach().double()
+    # sums of up to n fp32 products: (n + 16) u of the sum of their sizes, through three products and
+    # GELU (1.13) at most; a value next to a rounding border of the held rows may take the next step
+    with torch.no_grad():
+        dx = torch.zeros(N, D, dtype=torch.float64, device="cuda")
+        for e, (xe, he) in enumerate(zip(x.split(counts), xh.split(counts))):
+            lin1, lin2 = moe.experts[e][0], moe.experts[e][2]
+            w1, w2 = lin1.weight.double(), lin2.weight.double()
+            b1 = lin1.bias.double() if bias else 0
+            b2 = lin2.bias.double() if bias else 0
+            at = slice(sum(counts[:e]), sum(counts[:e + 1]))
+            if not counts[e]:
+                assert outs[e].shape == (0, D)
+                assert all(got[id(p)] is None for p in moe.experts[e].parameters())
+                continue
+            pre = xe.double() @ w1.t() + b1
+            y = (pre * cdf64(pre)) @ w2.t() + b2
+            assert (outs[e] - y).abs().max() <= 1e-4 * (1 + y.abs().max())
+            g = grads[e].double()
+            ph = held64(pre.float())
+            da = g @ w2
+            dh = da * slope64(ph)
+            dx[at] = dh @ w1
+            want = {id(lin1.weight): dh.t() @ he, id(lin2.weight): g.t() @ (ph * cdf64(ph))}
+            if bias:
+                want |= {id(lin1.bias): dh.sum(0), id(lin2.bias): g.sum(0)}
+            for key, value in want.items():
+                step = (ph.abs().max() / 127) * 2  # of a value that took the next step
+                assert (got[key] - value).norm() <= 1e-4 * value.norm() + 1e-2 * step
+        if N:
+            assert (got[id(x)] - dx).norm() <= 1e-4 * dx.norm() + 1e-3
+
+
+def test_gradient_of_the_held_gelu_against_differences():
+    """Against central differences of GELU at the exact values: held values are half a step off, and
+    GELU's slope changes by at most 0.8 a unit (|gelu''| <= 2 phi(0)); the difference's own cubic
+    term is below 1e-9 at a step of 1e-4 in 64 bits."""
+    x, g = rand(40, 384, seed=2) * 2, rand(40, 384, seed=3)
+    _, held = fm.gelu_compress(x)
+    _, grad = fm.gelu_compressed_backward(held, g)
+    x64, e = x.double(), 1e-4
+    gelu = lambda v: v * cdf64(v)  # noqa: E731
+    diff = (gelu(x64 + e) - gelu(x64 - e)) / (2 * e) * g.double()
+    step = held.scales.repeat_interleave(128, 1).double()
+    assert ((grad - diff).abs() <= g.double().abs() * (0.8 * 0.501 * step + 1e-6)).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+def test_held_layer_trains_like_the_plain_one(dtype):
+    """Same parameters: the forward agrees to the type's rounding, the gradients to 8 bits' error."""
+    plain = layer(256, 512, 4, 2, dtype)
+    held = layer(256, 512, 4, 2, dtype, checkpoint="int8")
+    held.load_state_dict(plain.state_dict())
+    x = rand(2, 64, 256, dtype=dtype, seed=1)
+    g = rand(2, 64, 256, dtype=dtype, seed=2)
+    a, b = plain(x), held(x)
+    assert (a - b).norm() <= 2e-2 * a.norm()
+    ga = torch.autograd.grad(a, list(plain.parameters()), g)
+    gb = torch.autograd.grad(b, list(held.parameters()), g)
+    for u, v in zip(ga, gb):
+        assert (u - v).norm() <= 3e-2 * u.norm()
+    with torch.no_grad():
+        assert torch.equal(held(x), b)
+
+
+def test_held_experts_hold_less():
+    D, H, N = 1024, 2048, 4096
+    moe = layer(D, H, 4, 1)
+    sizes = {}
+    for checkpoint in (None, "int8"):
+        x = rand(N, D, dtype=torch.bfloat16, seed=1).requires_grad_(True)
+        torch.cuda.synchronize()
+        before = torch.cuda.memory_allocated()
+        outs = fm.compute_experts(moe.experts, x * 1, [N // 4] * 4, checkpoint=checkpoint)
+        sizes[checkpoint] = torch.cuda.memory_allocated() - before - sum(o.numel() * 2 for o in outs)
+        del outs
+    # 2 D + 4 H bytes a row (x, the first product, GELU's output) against D + H and the scales
+    assert sizes["int8"] <= 0.55 * sizes[None] * (D + H) / (D + 2 * H) * 1.1
+
+
+def test_held_experts_parts_of_the_gradient():
+    """Frozen weights, a loss that leaves experts out, autocast, and no gradient at all."""
+    counts = [8, 9, 0]
+    moe = layer(64, 96, 3, 1, torch.float32)
+    x = rand(17, 64, seed=1)
+    for p in moe.experts[0].parameters():
+        p.requires_grad_(False)
+    outs = fm.compute_experts(moe.experts, x, counts, checkpoint="int8")
+    outs[1].sum().backward()
+    assert moe.experts[0][0].weight.grad is None and moe.experts[1][2].weight.grad is not None
+    full = moe.experts[1][2].weight.grad.clone()
+    moe.zero_grad()
+    xg = x.clone().requires_grad_(True)
+    outs = fm.compute_experts(moe.experts, xg, counts, checkpoint="int8")
+    outs[1].sum().backward()
+    assert torch.equal(moe.experts[1][2].weight.grad, full)
+    assert not xg.grad[:8].any() and xg.grad[8:].any()
+    with torch.autocast("cuda", dtype=torch.bfloat16):
+        outs = fm.compute_experts(moe.experts, xg, counts, checkpoint="int8")
+    assert outs[0].dtype == torch.bfloat16
+    outs[1].float().sum().backward()
+    assert moe.experts[1][0].weight.grad.dtype == torch.float32
+    with torch.no_grad():
+        assert not fm.compute_experts(moe.experts, x, counts, checkpoint="int8")[0].requires_grad
+
+
+def test_held_experts_refusals():
+    moe = layer(64, 96, 2, 1, torch.float32)
+    x = rand(8, 64)
+    with pytest.raises(ValueError, match="checkpoint"):
+        fm.compute_experts(moe.experts, x, [4, 4], checkpoint="fp8")
+    with pytest.raises(ValueError, match="checkpoint"):
+        fm.MoEFeedForward(8, 8, 2, 1, checkpoint="fp8")
+    with pytest.raises(ValueError, match="split"):
+        fm.compute_experts(moe.experts, x, [4, 3], checkpoint="int8")
+    with pytest.raises(TypeError, match="parameters"):
+        fm.compute_experts(moe.experts, x.half(), [4, 4], checkpoint="int8")
+    with pytest.raises(RuntimeError, match="only on the GPU"):
+        fm.compute_experts(layer(64, 96, 2, 1).cpu().experts, x.cpu().bfloat16(), [4, 4],
+                           checkpoint="int8")
+    moe.experts[0].register_forward_hook(lambda *a: None)
+    with pytest.raises(ValueError, match="hooks"):
+        fm.compute_experts(moe.experts, x, [4, 4], checkpoint="int8")
+    moe = layer(64, 96, 2, 1, torch.float32)
+    g = torch.cuda.CUDAGraph()
+    fm.compute_experts(moe.experts, x, [4, 4], checkpoint="int8")
+    torch.cuda.synchronize()
+    with torch.cuda.graph(g):
+        y = x * 2
+        with pytest.raises(RuntimeError, match="graph capture"):
+            fm.compute_experts(moe.experts, x, [4, 4], checkpoint="int8")
