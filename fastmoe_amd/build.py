@@ -20,9 +20,10 @@ BUILD_DIR = PKG / "_build"
 LIB_NAME = "libfastmoe_amd.so"
 LIB_PATH = PKG / LIB_NAME
 
-# The operator layer's host helper module (fastmoe_amd._host, a CPython extension built against
-# the installed torch): it reads tensor properties in C++, and is not part of the C ABI.
-HOST_EXT_SOURCE = "host_ext.cpp"
+# The operator layer's host helper modules (CPython extensions built against the installed torch, not
+# part of the C ABI): fastmoe_amd._host reads tensor properties in C++, fastmoe_amd._rows allocates
+# for and calls the entry points of the 8-bit operators and the norm.
+HOST_EXT_SOURCES = {"_host": "host_ext.cpp", "_rows": "rows_ext.cpp"}
 
 HIP_SOURCES = ["metadata.hip", "plan.hip", "plan_bucket.hip", "plan_radix.hip", "combine_fwd.hip",
                "combine_bwd.hip", "permute.hip", "noalloc.hip", "norm_quantize.hip", "hold.hip",
@@ -87,28 +88,31 @@ def _run(cmd: list[str]) -> None:
         print(out, file=sys.stderr)
 
 
-def _host_ext_command(cxx: str):
-    """g++ command of the host helper module: (command, temporary output, final path)."""
+def _host_ext_command(cxx: str, name: str, source: str):
+    """g++ command of a host helper module: (command, temporary output, final path)."""
     import sysconfig
 
     import torch
     from torch.utils import cpp_extension
 
-    path = PKG / ("_host" + sysconfig.get_config_var("EXT_SUFFIX"))
+    path = PKG / (name + sysconfig.get_config_var("EXT_SUFFIX"))
     tmp = path.with_name(path.name + ".tmp")
-    incs = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"]]
+    rocm = Path(os.environ.get("ROCM_PATH", "/opt/rocm"))
+    incs = [*cpp_extension.include_paths(), sysconfig.get_paths()["include"], str(rocm / "include")]
     libdirs = cpp_extension.library_paths()
     abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
-    cmd = [cxx, *CXX_FLAGS, "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", str(CSRC / HOST_EXT_SOURCE),
-           "-o", str(tmp), *[f"-I{i}" for i in incs], *[f"-L{d}" for d in libdirs],
-           *[f"-Wl,-rpath,{d}" for d in libdirs], "-lc10", "-ltorch", "-ltorch_python"]
+    # torch's stream header includes HIP's, which asks the host compiler for its platform
+    cmd = [cxx, *CXX_FLAGS, "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__",
+           str(CSRC / source), "-o", str(tmp), *[f"-I{i}" for i in incs],
+           *[f"-L{d}" for d in libdirs], *[f"-Wl,-rpath,{d}" for d in libdirs], "-lc10", "-lc10_hip",
+           "-ltorch", "-ltorch_cpu", "-ltorch_python"]
     return cmd, tmp, path
 
 
 def build(verbose: bool = True, jobs: int | None = None, defines: list[str] | None = None,
           out: Path | None = None, build_dir: Path | None = None) -> Path:
     """Compile every translation unit and link ``libfastmoe_amd.so``; returns its path.  The
-    in-tree build also compiles the host helper module ``fastmoe_amd._host``.
+    in-tree build also compiles the host helper modules ``fastmoe_amd._host`` and ``_rows``.
 
     ``defines`` (e.g. ``["FMOE_BWD_WAVES=8"]``) set the kernels' compile-time knobs; ``out`` and
     ``build_dir`` redirect the result (tuning builds), by default the in-tree library.
@@ -129,13 +133,12 @@ def build(verbose: bool = True, jobs: int | None = None, defines: list[str] | No
         obj = bdir / (src + ".o")
         cmds.append([cxx, *CXX_FLAGS, "-c", str(CSRC / src), "-o", str(obj)])
         objs.append(str(obj))
-    ext_cmd, ext_tmp, ext_path = (None, None, None) if out else _host_ext_command(cxx)
-    if ext_cmd:
-        cmds.append(ext_cmd)
+    exts = [] if out else [_host_ext_command(cxx, n, f) for n, f in HOST_EXT_SOURCES.items()]
+    cmds += [cmd for cmd, _, _ in exts]
     jobs = jobs or min(len(cmds), max(1, (os.cpu_count() or 4)))
     with ThreadPoolExecutor(max_workers=jobs) as ex:
         list(ex.map(_run, cmds))
-    if ext_cmd:
+    for _, ext_tmp, ext_path in exts:
         os.replace(ext_tmp, ext_path)
     tmp = lib_path.with_suffix(".so.tmp")
     _run([hipcc, f"--offload-arch={ARCH}", "-shared", "-fPIC", *objs, "-o", str(tmp)])

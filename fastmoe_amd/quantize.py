@@ -27,13 +27,17 @@ row in the activations' type).  CPU tensors raise.
 """
 from __future__ import annotations
 
+import ctypes
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
 
-from . import _abi
-from .ops import (_FLOAT_CODES, _INDEX_CODES, _on_device, _refuse_autograd_capture, _runs_plain,
-                  _span, _stream_handle, _validate_default)
+
+
+from torch.autograd import forward_ad
+
+from . import _abi, ops
+from .ops import _FLOAT_CODES, _INDEX_CODES, _refuse_autograd_capture, _validate_default
 
 __all__ = [
     "CompressedRows",
@@ -55,6 +59,35 @@ PITCH = 128  # a row of whole numbers is padded with zeros to a multiple of this
 BLOCK = 128  # columns of a held activation that share a scale
 
 _ACTIVATIONS = {None: _abi.ACT_NONE, "gelu": _abi.ACT_GELU}
+
+_ROWS: list = []
+
+
+def _rows_module():
+    """The host helper module ``fastmoe_amd._rows`` (built with the library), which allocates for and
+    calls the entry points; raises if it or the library is missing."""
+    if not _ROWS:
+        lib = _abi.lib()
+        try:
+            from . import _rows as mod
+        except ImportError as exc:
+            raise _abi.FastMoEError(
+                "fastmoe_amd: the host helper module fastmoe_amd._rows is not built "
+                "(run python -m fastmoe_amd.build)") from exc
+        names = [n for n in _abi.SIGNATURES if hasattr(lib, n)]
+        mod.bind({n: ctypes.cast(getattr(lib, n), ctypes.c_void_p).value for n in names})
+        _ROWS.append(mod)
+    return _ROWS[0]
+
+
+def _call(name: str, *args):
+    """A function of the helper module, in a span of its name where calls are timed.  NotImplemented
+    where it does not take its arguments: the caller then checks them one by one."""
+    fn = getattr(_ROWS[0] if _ROWS else _rows_module(), name)
+    if ops._TIMER is None:
+        return fn(*args)
+    with ops._TIMER.span(name):
+        return fn(*args)
 
 
 def _pad(n: int) -> int:
@@ -82,11 +115,6 @@ def _check_matrix(t, what: str) -> None:
         raise ValueError(f"fastmoe_amd: {what} must have unit column stride")
 
 
-def _row_stride(t: torch.Tensor) -> int:
-    """Elements from row to row (a single row's stride is free to be anything)."""
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
 def _same_device(first: torch.Tensor, **others) -> None:
     for name, t in others.items():
         if t is not None and t.device != first.device:
@@ -111,6 +139,17 @@ def _check_int8(data, scales, features, what: str, dims: int) -> None:
                          "multiple of 16 bytes")
 
 
+def _float_code(dtype, what: str = "dtype") -> int:
+    code = _FLOAT_CODES.get(dtype)
+    if code is None:
+        raise TypeError(f"fastmoe_amd: unsupported {what} {dtype}")
+    return code
+
+
+def _not_taken(what: str) -> None:
+    raise ValueError(f"fastmoe_amd: {what} does not take these tensors")
+
+
 class QuantizedRows(NamedTuple):
     """Rows in 8 bits with one scale each: row r stands for ``data[r, :features] * scales[r]``."""
 
@@ -120,8 +159,11 @@ class QuantizedRows(NamedTuple):
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """The values that the rows stand for, [R, features]."""
-        _check_rows8(self, "rows")
-        return _restore(self.data, self.scales, 1, self.features, dtype)
+        out = _call("restore", self.data, self.scales, False, self.features, _float_code(dtype))
+        if out is NotImplemented:
+            _check_rows8(self, "rows")
+            _not_taken("dequantize")
+        return out
 
 
 class Int8Weights(NamedTuple):
@@ -159,11 +201,6 @@ def _check_rows8(x: QuantizedRows, what: str) -> None:
                          "least its columns")
 
 
-def _new_rows8(rows: int, cols: int, dev) -> QuantizedRows:
-    return QuantizedRows(torch.empty((rows, _pad(cols)), dtype=torch.int8, device=dev),
-                         torch.empty(rows, dtype=torch.float32, device=dev), cols)
-
-
 # ---- the norm ---------------------------------------------------------------------------------
 
 def _check_norm(x, weight, residual, eps) -> None:
@@ -184,68 +221,14 @@ def _check_norm(x, weight, residual, eps) -> None:
         raise ValueError(f"fastmoe_amd: eps must be finite and not negative, got {eps}")
 
 
-def _norm(x, weight, residual, eps, *, y: bool, rstd: bool, rows8: bool):
-    """(stream, y, rstd, 8-bit rows) of checked arguments; None where not asked for."""
-    T, D = x.shape
-    dev = x.device
-    h = x if residual is None else torch.empty((T, D), dtype=x.dtype, device=dev)
-    out = torch.empty((T, D), dtype=x.dtype, device=dev) if y else None
-    factor = torch.empty(T, dtype=torch.float32, device=dev) if rstd else None
-    q = _new_rows8(T, D, dev) if rows8 else None
-    if T:
-        with _on_device(dev), _span("add_rms_norm"):
-            rc = _abi.lib().fmoe_add_rms_norm(
-                x.data_ptr(), _row_stride(x),
-                residual.data_ptr() if residual is not None else None,
-                _row_stride(residual) if residual is not None else 0,
-                weight.data_ptr(), _FLOAT_CODES[weight.dtype], T, D, _FLOAT_CODES[x.dtype],
-                float(eps), h.data_ptr() if residual is not None else None,
-                out.data_ptr() if y else None, factor.data_ptr() if rstd else None,
-                q.data.data_ptr() if rows8 else None, q.data.shape[1] if rows8 else 0,
-                q.scales.data_ptr() if rows8 else None, _stream_handle(dev))
-        _abi.check(rc, "fmoe_add_rms_norm")
-    return h, out, factor, q
-
-
-class _AddRmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, eps):
-        h, y, rstd, _ = _norm(x, weight, residual, eps, y=True, rstd=True, rows8=False)
-        ctx.save_for_backward(h, weight, rstd)
-        ctx.has_residual = residual is not None
-        ctx.set_materialize_grads(False)
-        return (y, h) if residual is not None else y
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, gy, gh=None):
-        h, weight, rstd = ctx.saved_tensors
-        _refuse_autograd_capture("the norm's backward", h)
-        need_x, need_w, need_r = ctx.needs_input_grad[:3]
-        gw = None
-        if gy is None:  # only the stream was used
-            gw = torch.zeros_like(weight) if need_w else None
-            return gh if need_x else None, gw, gh if need_r else None, None
-        T, D = h.shape
-        gy = gy if D == 1 or gy.stride(1) == 1 else gy.contiguous()
-        if gh is not None and D > 1 and gh.stride(1) != 1:
-            gh = gh.contiguous()
-        lib = _abi.lib()
-        gx = torch.empty((T, D), dtype=h.dtype, device=h.device)
-        nbytes, ws = 0, None
-        if need_w:
-            gw = torch.empty_like(weight)
-            nbytes = lib.fmoe_add_rms_norm_backward_workspace_bytes(T, D)
-            ws = torch.empty(nbytes, dtype=torch.uint8, device=h.device)
-        with _on_device(h.device), _span("add_rms_norm_backward"):
-            rc = lib.fmoe_add_rms_norm_backward(
-                gy.data_ptr(), _row_stride(gy), gh.data_ptr() if gh is not None else None,
-                _row_stride(gh) if gh is not None else 0, h.data_ptr(), _row_stride(h),
-                weight.data_ptr(), _FLOAT_CODES[weight.dtype], rstd.data_ptr(), T, D,
-                _FLOAT_CODES[h.dtype], gx.data_ptr(), gw.data_ptr() if need_w else None,
-                ws.data_ptr() if need_w else None, nbytes, _stream_handle(h.device))
-        _abi.check(rc, "fmoe_add_rms_norm_backward")
-        return gx if need_x else None, gw, gx if need_r else None, None
+def _refuse_transforms(what: str) -> None:
+    """These calls are opaque to functorch's transforms, forward-mode gradients and tracing."""
+    if torch.compiler.is_compiling():  # first: the compiler does not trace the others
+        return
+    if (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+            or torch._C._get_tracing_state() is not None):
+        raise RuntimeError(f"fastmoe_amd: {what} does not run under functorch transforms, "
+                           "forward-mode gradients or tracing")
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,
@@ -257,15 +240,16 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     once.  Without a residual, h is ``x`` itself.  Differentiable in all three; the gradient of the
     weight sums the rows in a fixed order.
     """
+    _refuse_transforms("add_rms_norm")
+    out = _call("norm", x, weight, residual, eps, True, False)
+    if out is not NotImplemented:  # nothing to record
+        return out[1], x if residual is None else out[0]
     _check_norm(x, weight, residual, eps)
-    inputs = [t for t in (x, weight, residual) if t is not None]
-    if _runs_plain(inputs):
-        h, y, _, _ = _norm(x, weight, residual, eps, y=True, rstd=False, rows8=False)
-        return y, h
-    records = torch.is_grad_enabled() and any(t.requires_grad for t in inputs)
-    _refuse_autograd_capture("the autograd norm", x, records)
-    out = _AddRmsNorm.apply(x, weight, residual, float(eps))
-    return out if residual is not None else (out, x)
+    _refuse_autograd_capture("the autograd norm", x)
+    out = _call("norm_recorded", x, weight, residual, eps)
+    if out is NotImplemented:
+        _not_taken("add_rms_norm")
+    return out
 
 
 def _no_gradient(what: str, *tensors) -> None:
@@ -281,10 +265,13 @@ def add_rms_norm_int8(x: torch.Tensor, weight: torch.Tensor, residual: Optional[
     Without ``keep_normed`` only the 8-bit rows are written.  For serving: it records no backward,
     and refuses inputs that require one.
     """
-    _check_norm(x, weight, residual, eps)
-    _no_gradient("add_rms_norm_int8", x, weight, residual)
-    h, y, _, q = _norm(x, weight, residual, eps, y=bool(keep_normed), rstd=False, rows8=True)
-    return Int8NormedRows(q, y, h)
+    out = _call("norm", x, weight, residual, eps, bool(keep_normed), True)
+    if out is NotImplemented:
+        _check_norm(x, weight, residual, eps)
+        _no_gradient("add_rms_norm_int8", x, weight, residual)
+        _not_taken("add_rms_norm_int8")
+    h, y, q, scales = out
+    return Int8NormedRows(QuantizedRows(q, scales, x.shape[1]), y, x if residual is None else h)
 
 
 # ---- rows and weights in 8 bits ---------------------------------------------------------------
@@ -293,19 +280,14 @@ def quantize_rows(x: torch.Tensor, *, activation: Optional[str] = None) -> Quant
     """Rows [R, C] (unit column stride) in 8 bits with one scale each, after ``activation``: None or
     "gelu" (the exact form, as ``torch.nn.GELU()``).  Records no backward, and refuses inputs that
     require one."""
-    _check_matrix(x, "x")
     if activation not in _ACTIVATIONS:
         raise ValueError(f"fastmoe_amd: unknown activation {activation!r} (expected None or 'gelu')")
-    _no_gradient("quantize_rows", x)
-    R, C = x.shape
-    q = _new_rows8(R, C, x.device)
-    if R:
-        with _on_device(x.device), _span("quantize_rows"):
-            rc = _abi.lib().fmoe_quantize_rows(
-                x.data_ptr(), _row_stride(x), R, C, _FLOAT_CODES[x.dtype], _ACTIVATIONS[activation],
-                q.data.data_ptr(), q.data.shape[1], q.scales.data_ptr(), _stream_handle(x.device))
-        _abi.check(rc, "fmoe_quantize_rows")
-    return q
+    out = _call("quantize", x, _ACTIVATIONS[activation])
+    if out is NotImplemented:
+        _check_matrix(x, "x")
+        _no_gradient("quantize_rows", x)
+        _not_taken("quantize_rows")
+    return QuantizedRows(*out, x.shape[1])
 
 
 def quantize_weights(weight: Union[torch.Tensor, Sequence[torch.Tensor]]) -> Int8Weights:
@@ -352,20 +334,40 @@ def int8_linear(x: QuantizedRows, weights: Int8Weights,
     x; ``validate=True`` (or ``FASTMOE_VALIDATE=1``) raises IndexError for such entries and for
     offsets that fall or end outside the rows (one synchronisation).  It has no gradient.
     """
+    if _validate_default(validate):
+        _check_linear(x, weights, expert_offsets, rows, bias, out_dtype)
+        _validate_linear(x, expert_offsets, rows)
+    args = (x.data, x.scales, x.features, weights.data, weights.scales)
+    code = _FLOAT_CODES.get(out_dtype)
+    out = NotImplemented
+    if code is not None and weights.features == x.features:
+        out = _call("linear", *args, expert_offsets, rows, bias, code)
+    if out is NotImplemented:
+        _check_linear(x, weights, expert_offsets, rows, bias, out_dtype)
+        # what is left: indices, offsets or a bias with gaps between their elements
+        expert_offsets, rows, bias = (t if t is None else t.contiguous()
+                                      for t in (expert_offsets, rows, bias))
+        out = _call("linear", *args, expert_offsets, rows, bias, code)
+        if out is NotImplemented:
+            _not_taken("int8_linear")
+    return out
+
+
+def _check_linear(x, weights, expert_offsets, rows, bias, out_dtype) -> None:
+    """Says what is wrong with int8_linear's arguments, if anything is."""
     _check_rows8(x, "x")
     data, scales = weights.data, weights.scales
-    if data.dim() == 2:
+    if isinstance(data, torch.Tensor) and data.dim() == 2:
         data, scales = data.unsqueeze(0), scales.unsqueeze(0)
     _check_int8(data, scales, weights.features, "weights", 3)
-    E, N, Kp = data.shape
+    E, N, _ = data.shape
     if weights.features != x.features:
         raise ValueError(f"fastmoe_amd: x has {x.features} features, the weights {weights.features}")
     if E < 1 or N < 1 or tuple(scales.shape) != (E, N):
         raise ValueError(f"fastmoe_amd: weight scales must be [{E}, {N}], got {tuple(scales.shape)}")
     if not data.is_contiguous() or not scales.is_contiguous():
         raise ValueError("fastmoe_amd: weights and their scales must be contiguous")
-    if out_dtype not in _FLOAT_CODES:
-        raise TypeError(f"fastmoe_amd: unsupported out_dtype {out_dtype}")
+    _float_code(out_dtype, "out_dtype")
     if expert_offsets is None:
         if E != 1:
             raise ValueError(f"fastmoe_amd: {E} experts need expert_offsets")
@@ -374,15 +376,13 @@ def int8_linear(x: QuantizedRows, weights: Int8Weights,
         if expert_offsets.dtype != torch.int64 or tuple(expert_offsets.shape) != (E + 1,):
             raise ValueError(f"fastmoe_amd: expert_offsets must be int64 [{E + 1}], got "
                              f"{expert_offsets.dtype} {tuple(expert_offsets.shape)}")
-        expert_offsets = expert_offsets.contiguous()
-    R = x.data.shape[0]
     if rows is not None:
         _need_gpu(rows, "rows")
         if rows.dtype not in _INDEX_CODES or rows.dim() != 1:
             raise TypeError(f"fastmoe_amd: rows must be int64 or int32 with one dimension, got "
                             f"{rows.dtype} {tuple(rows.shape)}")
-        rows = rows.contiguous()
-        R = rows.shape[0]
+        if rows.shape[0] and not x.data.shape[0]:
+            raise ValueError("fastmoe_amd: rows is not empty, and x is")
     if bias is not None:
         _need_gpu(bias, "bias")
         if bias.dtype not in _FLOAT_CODES:
@@ -390,30 +390,11 @@ def int8_linear(x: QuantizedRows, weights: Int8Weights,
         if tuple(bias.shape) != (E, N) and not (E == 1 and tuple(bias.shape) == (N,)):
             raise ValueError(f"fastmoe_amd: bias must be [{E}, {N}], got {tuple(bias.shape)}")
         _no_gradient("int8_linear", bias)
-        bias = bias.contiguous()
     _same_device(x.data, weights=data, expert_offsets=expert_offsets, rows=rows, bias=bias)
-    if R and not x.data.shape[0]:
-        raise ValueError("fastmoe_amd: rows is not empty, and x is")
-    dev = x.data.device
-    if _validate_default(validate):
-        _validate_linear(x, expert_offsets, rows, R)
-    out = torch.empty((R, N), dtype=out_dtype, device=dev)
-    if R:
-        with _on_device(dev), _span("int8_linear"):
-            rc = _abi.lib().fmoe_int8_linear(
-                x.data.data_ptr(), x.data.stride(0) if x.data.shape[0] > 1 else Kp,
-                x.data.shape[0], x.scales.data_ptr(),
-                rows.data_ptr() if rows is not None else None,
-                _INDEX_CODES[rows.dtype] if rows is not None else _abi.I64,
-                data.data_ptr(), scales.data_ptr(), bias.data_ptr() if bias is not None else None,
-                _FLOAT_CODES[bias.dtype] if bias is not None else _abi.F32,
-                expert_offsets.data_ptr() if expert_offsets is not None else None, E, N, x.features,
-                R, out.data_ptr(), N, _FLOAT_CODES[out_dtype], _stream_handle(dev))
-        _abi.check(rc, "fmoe_int8_linear")
-    return out
 
 
-def _validate_linear(x: QuantizedRows, offsets, rows, R: int) -> None:
+def _validate_linear(x: QuantizedRows, offsets, rows) -> None:
+    R = x.data.shape[0] if rows is None else rows.shape[0]
     bad = torch.zeros((), dtype=torch.int64, device=x.data.device)
     if rows is not None and R:
         bad = bad + ((rows < 0) | (rows >= x.data.shape[0])).sum()
@@ -426,21 +407,6 @@ def _validate_linear(x: QuantizedRows, offsets, rows, R: int) -> None:
 
 # ---- activations held in 8 bits ---------------------------------------------------------------
 
-def _restore(data, scales, per_row: int, features: int, dtype) -> torch.Tensor:
-    if dtype not in _FLOAT_CODES:
-        raise TypeError(f"fastmoe_amd: unsupported dtype {dtype}")
-    R = data.shape[0]
-    out = torch.empty((R, features), dtype=dtype, device=data.device)
-    if R:
-        with _on_device(data.device), _span("restore_rows"):
-            rc = _abi.lib().fmoe_restore_rows(
-                data.data_ptr(), data.stride(0) if R > 1 else data.shape[1], scales.data_ptr(),
-                per_row, R, features, out.data_ptr(), _FLOAT_CODES[dtype],
-                _stream_handle(data.device))
-        _abi.check(rc, "fmoe_restore_rows")
-    return out
-
-
 def _check_held(held: CompressedRows) -> None:
     _check_int8(held.data, held.scales, held.features, "held", 2)
     want = (held.data.shape[0], -(-held.features // BLOCK))
@@ -451,44 +417,37 @@ def _check_held(held: CompressedRows) -> None:
         raise ValueError("fastmoe_amd: held data must be contiguous")
 
 
-def _compress(x: torch.Tensor, gelu: bool):
-    R, C = x.shape
-    dev = x.device
-    held = CompressedRows(torch.empty((R, _pad(C)), dtype=torch.int8, device=dev),
-                          torch.empty((R, -(-C // BLOCK)), dtype=torch.float32, device=dev), C)
-    a = torch.empty((R, C), dtype=x.dtype, device=dev) if gelu else None
-    if R:
-        with _on_device(dev), _span("compress_rows"):
-            rc = _abi.lib().fmoe_compress_rows(
-                x.data_ptr(), _row_stride(x), R, C, _FLOAT_CODES[x.dtype], held.data.data_ptr(),
-                held.data.shape[1], held.scales.data_ptr(), a.data_ptr() if gelu else None,
-                _stream_handle(dev))
-        _abi.check(rc, "fmoe_compress_rows")
-    return a, held
+def _compress(x: torch.Tensor, gelu: bool, what: str = "compress_rows"):
+    out = _call("compress", x, gelu)
+    if out is NotImplemented:
+        _check_matrix(x, "x")
+        _no_gradient(what, x)
+        _not_taken(what)
+    a, q, scales = out
+    return a, CompressedRows(q, scales, x.shape[1])
 
 
 def compress_rows(x: torch.Tensor) -> CompressedRows:
     """Rows [R, C] (unit column stride) held in 8 bits, a scale for every 128 columns of a row: each
     value within 1/254 of the largest of its block.  Records no backward, and refuses inputs that
     require one (an autograd Function's forward, which records nothing, is where it is called)."""
-    _check_matrix(x, "x")
-    _no_gradient("compress_rows", x)
     return _compress(x, False)[1]
 
 
 def restore_rows(held: CompressedRows, dtype: torch.dtype) -> torch.Tensor:
     """The values that held rows stand for, [R, C] in ``dtype``."""
-    _check_held(held)
-    return _restore(held.data, held.scales, held.scales.shape[1], held.features, dtype)
+    out = _call("restore", held.data, held.scales, True, held.features, _float_code(dtype))
+    if out is NotImplemented:
+        _check_held(held)
+        _not_taken("restore_rows")
+    return out
 
 
 def gelu_compress(x: torch.Tensor) -> Tuple[torch.Tensor, CompressedRows]:
     """``(gelu(x), x held in 8 bits)`` in one pass: the forward of a GELU whose backward is
     :func:`gelu_compressed_backward`.  GELU is exact (``torch.nn.GELU()``) and taken of the exact x.
     Records no backward, and refuses inputs that require one."""
-    _check_matrix(x, "x")
-    _no_gradient("gelu_compress", x)
-    return _compress(x, True)
+    return _compress(x, True, "gelu_compress")
 
 
 def gelu_compressed_backward(held: CompressedRows, grad: torch.Tensor, *,
@@ -496,20 +455,14 @@ def gelu_compressed_backward(held: CompressedRows, grad: torch.Tensor, *,
     """``(gelu(x'), grad * gelu'(x'))`` of the held rows x', in ``grad``'s type: GELU's output once
     more, which the gradient of the weights after it reads (None without ``again``), and the
     gradient of GELU's input."""
-    _check_held(held)
-    _check_matrix(grad, "grad")
-    R, C = held.data.shape[0], held.features
-    if tuple(grad.shape) != (R, C):
-        raise ValueError(f"fastmoe_amd: grad must be [{R}, {C}], got {tuple(grad.shape)}")
-    _same_device(held.data, grad=grad)
-    _no_gradient("gelu_compressed_backward", grad)
-    out = torch.empty((R, C), dtype=grad.dtype, device=grad.device)
-    a = torch.empty_like(out) if again else None
-    if R:
-        with _on_device(grad.device), _span("gelu_compressed_backward"):
-            rc = _abi.lib().fmoe_gelu_compressed_backward(
-                held.data.data_ptr(), held.data.shape[1], held.scales.data_ptr(), grad.data_ptr(),
-                _row_stride(grad), R, C, _FLOAT_CODES[grad.dtype], a.data_ptr() if again else None,
-                out.data_ptr(), _stream_handle(grad.device))
-        _abi.check(rc, "fmoe_gelu_compressed_backward")
-    return a, out
+    out = _call("gelu_backward", held.data, held.scales, held.features, grad, bool(again))
+    if out is NotImplemented:
+        _check_held(held)
+        _check_matrix(grad, "grad")
+        R, C = held.data.shape[0], held.features
+        if tuple(grad.shape) != (R, C):
+            raise ValueError(f"fastmoe_amd: grad must be [{R}, {C}], got {tuple(grad.shape)}")
+        _same_device(held.data, grad=grad)
+        _no_gradient("gelu_compressed_backward", grad)
+        _not_taken("gelu_compressed_backward")
+    return out
