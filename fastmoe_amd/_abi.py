@@ -134,7 +134,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_vp, _c_i64, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp],
     ),
-    "fmoe_int8_linear_tile": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "fmoe_int8_linear_tile": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "fmoe_int8_linear": (
         _c_int,
         [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_i64,

@@ -538,8 +538,11 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 128       80 / 44 / 31   94 / 59 / 36  102 / 65 / 38   152 / 95 / 56  233 / 145 / 77
 //   128 x 256       63 / 45 / 35   83 / 55 / 40   88 / 61 / 42   141 / 85 / 47  191 / 124 / 77
 //   256 x 256       81 / 51 / 42   93 / 60 / 46  100 / 68 / 50   114 / 82 / 57  204 / 120 / 62
-enum Variant { kFew = 16016, k32x64 = 32064, k128x128 = 128128, k128x256 = 128256, k256x256 = 256256 };
-Variant pick(int64_t rows, int64_t E, int64_t N) {
+// Long rows of few experts' rows each are streamed best 128 columns wide, where that leaves two workgroups
+// for every CU: 80 against 88 us for 4 rows of each of 32 experts ([2048, 7168]), 142 against 147 for 64 rows
+// over 256 experts, but 391 against 384 for 256 rows, and 43 against 38 at K = 2048.
+enum Variant { kFew = 16016, k32x64 = 32064, k32x128 = 32128, k128x128 = 128128, k128x256 = 128256, k256x256 = 256256 };
+Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   const int64_t per = rows / E;
   auto work = [&](int64_t bm, int64_t bn) {
     return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
@@ -548,14 +551,16 @@ Variant pick(int64_t rows, int64_t E, int64_t N) {
   if (per >= 16 && work(128, 256) >= 140) return k128x256;
   if (per >= 40 && work(128, 128) >= 128) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
+  if (K >= 4096 && work(32, 128) >= 512) return k32x128;
   return k32x64;
 }
 
 template <typename TO> int launch_linear(const char* who, const LinearArgs& a, hipStream_t s) {
-  switch (pick(a.rows, a.E, a.N)) {
+  switch (pick(a.rows, a.E, a.N, a.Kp)) {
     case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4>(who, a, s);
     case k128x256: return launch_tile<TO, 128, 256, 2, 4, 128, 3>(who, a, s);
     case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4>(who, a, s);
+    case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3>(who, a, s);
     case kFew: return launch_few<TO>(who, a, s);
     default: return launch_tile<TO, 32, 64, 1, 2, 128, 4>(who, a, s);
   }
@@ -563,9 +568,9 @@ template <typename TO> int launch_linear(const char* who, const LinearArgs& a, h
 
 }  // namespace
 
-extern "C" int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N) {
-  if (rows < 1 || num_experts < 1 || N < 1) return -1;
-  return pick(rows, num_experts, N);
+extern "C" int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N, int64_t K) {
+  if (rows < 1 || num_experts < 1 || N < 1 || K < 1) return -1;
+  return pick(rows, num_experts, N, fmoe_host::round_up(K, kRowsPitch));
 }
 
 extern "C" int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows,

@@ -508,7 +508,7 @@ FMOE_API int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_r
                               int64_t out_row_stride, int out_dtype, void* stream);
 
 /* The tile that fmoe_int8_linear chooses by size, as 1000 * rows + columns (introspection). */
-FMOE_API int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N);
+FMOE_API int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N, int64_t K);
 
 #ifdef __cplusplus
 }

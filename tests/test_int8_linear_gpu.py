@@ -108,14 +108,17 @@ TILES = [(256256, 50, 130, 1000), (128256, 40, 40, 1000), (128128, 16, 60, 1024)
          (16016, 3, 4, 130)]
 
 
+KS = [1, 130, 300, 500, 641, 1100]
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
-@pytest.mark.parametrize("K", [1, 130, 300, 500, 641, 1100])
-@pytest.mark.parametrize("tile,E,mean,N", TILES)
+@pytest.mark.parametrize("tile,E,mean,N,K", [(*t, K) for t in TILES for K in KS] +
+                         [(32128, 130, 5, 500, K) for K in (4000, 4097, 4225)])
 def test_every_tile(tile, E, mean, N, K, dtype):
     """Every tile, with rings of every remainder of pieces, ragged experts and column ends."""
     counts = ragged(E, mean, seed=K)
     R = sum(counts)
-    assert _abi.lib().fmoe_int8_linear_tile(R, E, N) == tile
+    assert _abi.lib().fmoe_int8_linear_tile(R, E, N, K) == tile
     x, w = make(R, K, E, N, seed=K)
     bias = torch.randn(E, N, device="cuda")
     got = fm.int8_linear(x, w, route(counts), bias=bias, out_dtype=dtype)
