@@ -29,6 +29,7 @@ struct NormArgs {
   int64_t rows, cols;
   float eps;
   void *h, *y;    // packed; null where not wanted
+  int stream_y;   // store y past the caches
   float* rstd;    // null where not wanted
   uint8_t* q;     // null where not wanted
   int64_t q_stride, q_cols;  // bytes from row to row; bytes written of each: the columns, zeros after them
@@ -88,9 +89,12 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm(NormArgs a) {
       f[v][i] = f[v][i] * c * w[i];
       top = larger(top, f[v][i]);
     }
-    if (a.y)
-      V::store(static_cast<T*>(a.y) + row * a.cols, (v * THREADS + tid) * 8, a.cols,
-               V::V::pack(f[v]));
+    if (a.y) {
+      T* y = static_cast<T*>(a.y) + row * a.cols;
+      const typename V::raw_t p = V::V::pack(f[v]);
+      if (a.stream_y) V::template store<true>(y, (v * THREADS + tid) * 8, a.cols, p);
+      else V::store(y, (v * THREADS + tid) * 8, a.cols, p);
+    }
   }
   if (!a.q) return;
   const Scale8 s = scale8(group_max<THREADS>(abs_bits(top), lds_max));
@@ -191,35 +195,46 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm_bwd(NormBwdAr
     for (int i = 0; i < 8; ++i) gw[v][i] = 0.f;
   }
   const float inv_cols = 1.0f / (float)a.cols;
-  int turn = 0;
-  for (int64_t row = unit; row < a.rows; row += a.units, turn ^= 1) {
+  struct Row {
+    typename V::raw_t gy[VPT], h[VPT], gh[VPT];
+    float c;
+  };
+  auto load = [&](int64_t row, Row& r) {
     const T* gyp = static_cast<const T*>(a.gy) + row * a.gy_stride;
     const T* hp = static_cast<const T*>(a.h) + row * a.h_stride;
-    typename V::raw_t gy[VPT], h[VPT], gh[VPT];
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
-      gy[v] = V::template load<true>(gyp, (v * THREADS + tid) * 8, a.cols);
-      h[v] = V::template load<true>(hp, (v * THREADS + tid) * 8, a.cols);
+      r.gy[v] = V::template load<true>(gyp, (v * THREADS + tid) * 8, a.cols);
+      r.h[v] = V::template load<true>(hp, (v * THREADS + tid) * 8, a.cols);
     }
     if (a.gh) {
       const T* ghp = static_cast<const T*>(a.gh) + row * a.gh_stride;
 #pragma unroll
       for (int v = 0; v < VPT; ++v)
-        gh[v] = V::template load<true>(ghp, (v * THREADS + tid) * 8, a.cols);
+        r.gh[v] = V::template load<true>(ghp, (v * THREADS + tid) * 8, a.cols);
     } else {
 #pragma unroll
-      for (int v = 0; v < VPT; ++v) gh[v] = V::zero();
+      for (int v = 0; v < VPT; ++v) r.gh[v] = V::zero();
     }
-    const float c = a.rstd[row];
+    r.c = a.rstd[row];
+  };
+  // The next row is asked for before this one's sum is joined, where the registers hold both.
+  constexpr bool kAhead = ElemInfo<T>::kBytes == 2 && THREADS <= 512;
+  Row now, next;
+  if (kAhead && unit < a.rows) load(unit, now);
+  int turn = 0;
+  for (int64_t row = unit; row < a.rows; row += a.units, turn ^= 1) {
+    if constexpr (!kAhead) load(row, now);
+    else if (row + a.units < a.rows) load(row + a.units, next);
     float sum = 0.f;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       float g[8], f[8];
-      V::V::cvt(gy[v], g);
-      V::V::cvt(h[v], f);
+      V::V::cvt(now.gy[v], g);
+      V::V::cvt(now.h[v], f);
 #pragma unroll
       for (int i = 0; i < 8; ++i) {
-        const float hat = f[i] * c;
+        const float hat = f[i] * now.c;
         gw[v][i] = __builtin_fmaf(g[i], hat, gw[v][i]);
         sum = __builtin_fmaf(g[i] * w[v][i], hat, sum);
       }
@@ -230,14 +245,15 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_norm_bwd(NormBwdAr
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
       float g[8], f[8], r[8];
-      V::V::cvt(gy[v], g);
-      V::V::cvt(h[v], f);
-      V::V::cvt(gh[v], r);
+      V::V::cvt(now.gy[v], g);
+      V::V::cvt(now.h[v], f);
+      V::V::cvt(now.gh[v], r);
 #pragma unroll
       for (int i = 0; i < 8; ++i)
-        r[i] = __builtin_fmaf(c, __builtin_fmaf(-(f[i] * c), m, g[i] * w[v][i]), r[i]);
+        r[i] = __builtin_fmaf(now.c, __builtin_fmaf(-(f[i] * now.c), m, g[i] * w[v][i]), r[i]);
       V::store(gx, (v * THREADS + tid) * 8, a.cols, V::V::pack(r));
     }
+    if constexpr (kAhead) now = next;
   }
   if (!a.partials) return;
   float* out = a.partials + (int64_t)blockIdx.x * a.cols;
@@ -420,7 +436,13 @@ using namespace fmoe;
 namespace {
 
 constexpr int kMaxRegCols = 16384;          // columns that the largest register variant holds
-constexpr int64_t kBwdGroups = 512;         // workgroups of the backward, as many parts of grad_w
+// Workgroups of the backward, as many parts of grad_w.  The large ones fill a CU: one for each (2048 x 7168:
+// 27 us, 31 with two; smaller ones 42 us with two at 16384 x 2048, 58 with one).
+constexpr int64_t kBwdGroups = 512;
+template <int THREADS> constexpr int64_t bwd_groups() { return THREADS >= 512 ? kBwdGroups / 2 : kBwdGroups; }
+// y is stored past the caches from the size at which the combine's output is: 4096 x 16384 takes 83
+// instead of 95 us.  (8192 x 4096, 64 MiB, takes 47 either way, and leaves y to its reader in the cache.)
+int streams_y(int64_t bytes) { return bytes >= FMOE_STREAM_OUT_BYTES; }
 constexpr int64_t kMaxCols = int64_t(1) << 30;
 
 // Calls f(threads, vectors) with the variant that holds a row of `cols` in at most four vectors a thread.
@@ -522,7 +544,8 @@ extern "C" int fmoe_add_rms_norm(const void* d_x, int64_t x_row_stride, const vo
     if (int rc = check_rows8(who, d_q, q_stride, d_scales, rows, cols)) return rc;
   if (rows == 0) return FMOE_OK;
   const NormArgs a{d_x, d_residual, d_weight, x_row_stride, residual_row_stride, rows, cols, eps,
-                   d_h, d_y, d_rstd, static_cast<uint8_t*>(d_q), q_stride,
+                   d_h, d_y, streams_y(rows * cols * fmoe_host::dtype_bytes(dtype)), d_rstd,
+                   static_cast<uint8_t*>(d_q), q_stride,
                    fmoe_host::round_up(cols, kRowsPitch), d_scales};
   hipStream_t s = static_cast<hipStream_t>(stream);
   by_weight(dtype, weight_dtype, [&](auto t, auto tw) {
@@ -586,7 +609,7 @@ extern "C" int fmoe_add_rms_norm_backward(const void* d_grad_y, int64_t gy_row_s
       }
       by_cols_backward<T>(cols, [&](auto th, auto v) {
         constexpr int kT = decltype(th)::value, kRows = rows_per_group<kT>();
-        parts = std::min((rows + kRows - 1) / kRows, kBwdGroups);
+        parts = std::min((rows + kRows - 1) / kRows, bwd_groups<kT>());
         a.units = parts * kRows;
         hipLaunchKernelGGL((k_norm_bwd<T, TW, kT, decltype(v)::value>), dim3((unsigned)parts),
                            dim3(group_threads<kT>()), 0, s, a);

@@ -54,14 +54,18 @@ template <typename T> struct Eight {
     }
     return r;
   }
+  // NT: past the caches, for results that would not stay in them.
+  template <bool NT = false>
   static __device__ __forceinline__ void store(T* row, int64_t col, int64_t n, raw_t r) {
     if (col + 8 <= n) {
       u32x4_any* p = reinterpret_cast<u32x4_any*>(row + col);
-      if constexpr (kWords == 4) {
-        *p = r;
-      } else {
-        p[0] = u32x4{r[0], r[1], r[2], r[3]};
-        p[1] = u32x4{r[4], r[5], r[6], r[7]};
+      const u32x4 a = {r[0], r[1], r[2], r[3]};
+      if constexpr (NT) __builtin_nontemporal_store(a, p);
+      else *p = a;
+      if constexpr (kWords == 8) {
+        const u32x4 b = {r[4], r[5], r[6], r[7]};
+        if constexpr (NT) __builtin_nontemporal_store(b, p + 1);
+        else p[1] = b;
       }
     } else if (col < n) {
       float f[8];
