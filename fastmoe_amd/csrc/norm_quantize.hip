@@ -443,7 +443,7 @@ template <int THREADS> constexpr int64_t bwd_groups() { return THREADS >= 512 ? 
 // y is stored past the caches from the size at which the combine's output is: 4096 x 16384 takes 83
 // instead of 95 us.  (8192 x 4096, 64 MiB, takes 47 either way, and leaves y to its reader in the cache.)
 int streams_y(int64_t bytes) { return bytes >= FMOE_STREAM_OUT_BYTES; }
-constexpr int64_t kMaxCols = int64_t(1) << 30;
+constexpr int64_t kMaxCols = int64_t(1) << 26;  // 2048 columns for each of a grid's 2^15 in y
 
 // Calls f(threads, vectors) with the variant that holds a row of `cols` in at most four vectors a thread.
 // Up to 2048 columns a row is a wave's: no barrier, and more of its loads in flight (GELU to 8 bits of

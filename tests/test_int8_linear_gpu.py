@@ -292,3 +292,58 @@ def test_refusals():
     with pytest.raises(ValueError, match="not empty"):
         fm.int8_linear(fm.QuantizedRows(x.data[:0], x.scales[:0], 256), w, off,
                        rows=torch.zeros(8, dtype=torch.int64, device="cuda"))
+
+
+def test_arrays_beyond_32_bits():
+    """Rows, weights and results whose offsets pass 4 GiB."""
+    K, N = 16384, 2048
+    x, w = make(4, K, 2, N)
+    want = reference(x, w, [2, 2])[0]
+    big = torch.zeros(270_000, K, dtype=torch.int8, device="cuda")  # 4.4e9 bytes
+    last = torch.arange(270_000 - 4, 270_000, device="cuda")
+    big[last] = x.data
+    scales = torch.zeros(270_000, device="cuda")
+    scales[last] = x.scales
+    heavy = torch.zeros(140, N, K, dtype=torch.int8, device="cuda")  # 4.7e9 bytes
+    heavy[-2:] = w.data
+    heavy_scales = torch.zeros(140, N, device="cuda")
+    heavy_scales[-2:] = w.scales
+    got = fm.int8_linear(fm.QuantizedRows(big, scales, K), fm.Int8Weights(heavy, heavy_scales, K),
+                         route([0] * 138 + [2, 2]), rows=last, out_dtype=torch.float32)
+    assert ((got.double() - want).abs() <= 6 * U * want.abs()).all()
+    del big, heavy
+    R, wide = 80_000, 32768
+    x, w = make(R, 128, 1, wide)
+    got = fm.int8_linear(x, w)  # 5.2e9 bytes
+    for at in (slice(0, 3), slice(R - 3, R)):
+        part = fm.QuantizedRows(x.data[at], x.scales[at], 128)
+        check(got[at], *reference(part, w, [3]), torch.bfloat16)
+
+
+def test_two_streams_at_once():
+    cases = []
+    for seed, counts in enumerate(([1, 0, 5], [300, 200, 77], [3000])):
+        x, w = make(sum(counts), 640, len(counts), 512, seed=seed)
+        cases.append((x, w, route(counts)))
+    want = [fm.int8_linear(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    for _ in range(10):
+        got = []
+        for s, c in zip(streams, cases):
+            with torch.cuda.stream(s):
+                got.append(fm.int8_linear(*c))
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+def test_indices_and_offsets_with_gaps():
+    """Every second element of a longer tensor is taken as it is."""
+    x, w = make(9, 200, 3, 40)
+    counts = [4, 0, 7]
+    rows, off = torch.randint(0, 9, (11,), device="cuda"), route(counts)
+    bias = torch.randn(3, 40, device="cuda")
+    gaps = [torch.stack([t, torch.full_like(t, 7)], -1)[..., 0] for t in (rows, off, bias)]
+    assert not any(t.is_contiguous() for t in gaps)
+    got = fm.int8_linear(x, w, gaps[1], rows=gaps[0], bias=gaps[2])
+    assert torch.equal(got, fm.int8_linear(x, w, off, rows=rows, bias=bias))

@@ -369,3 +369,75 @@ def test_refusals():
         fm.gelu_compressed_backward(held, x[:2])
     with pytest.raises(ValueError, match="features"):
         fm.restore_rows(held._replace(features=200), torch.float32)
+
+
+def test_outputs_past_the_caches_and_beyond_32_bits():
+    """Arrays above 4 GiB (their last rows lie beyond 32-bit offsets), whose y is also large enough to be
+    stored past the caches: each row is what the row alone gives."""
+    T, D = 140_000, 16384
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device="cuda")
+    at = [0, 1, 65_536, T - 2, T - 1]
+    x[at] = rand(len(at), D, dtype=torch.bfloat16, seed=3)
+    w = rand(D, dtype=torch.bfloat16, seed=4)
+    got = fm.add_rms_norm_int8(x, w)
+    want = fm.add_rms_norm_int8(x[at], w)
+    assert torch.equal(got.normed[at], want.normed)
+    assert torch.equal(got.rows.data[at], want.rows.data)
+    assert torch.equal(got.rows.scales[at], want.rows.scales)
+    assert not got.normed[2].any() and got.rows.scales[2] == 0
+    del got
+    held, some = fm.compress_rows(x), fm.compress_rows(x[at])
+    assert torch.equal(held.data[at], some.data) and torch.equal(held.scales[at], some.scales)
+    assert torch.equal(fm.restore_rows(held, torch.bfloat16)[at], fm.restore_rows(some, torch.bfloat16))
+    q = fm.quantize_rows(x, activation="gelu")
+    assert torch.equal(q.data[at], fm.quantize_rows(x[at], activation="gelu").data)
+
+
+def test_two_streams_at_once():
+    """No workspace is shared: interleaved calls on two streams give what each gives alone."""
+    sizes = [(700, 1001), (300, 4096)]
+    inputs = [(rand(T, D, dtype=torch.bfloat16, seed=T), rand(D, dtype=torch.bfloat16, seed=D),
+               rand(T, D, dtype=torch.bfloat16, seed=9)) for T, D in sizes]
+
+    def step(x, w, g):
+        leaves = [x.clone().requires_grad_(True), w.clone().requires_grad_(True)]
+        y, _ = fm.add_rms_norm(leaves[0], leaves[1])
+        grads = torch.autograd.grad(y, leaves, g)
+        a, held = fm.gelu_compress(x)
+        return [*grads, a, *fm.gelu_compressed_backward(held, g), fm.quantize_rows(x).data]
+
+    want = [step(*i) for i in inputs]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(5):
+        got = []
+        for s, i in zip(streams, inputs):
+            with torch.cuda.stream(s):
+                got.append(step(*i))
+        torch.cuda.synchronize()
+        for u, v in zip(want, got):
+            assert all(torch.equal(a, b) for a, b in zip(u, v))
+
+
+def test_the_norms_gradient_has_none():
+    x, w = rand(4, 32).requires_grad_(True), rand(32, seed=1).requires_grad_(True)
+    y, _ = fm.add_rms_norm(x, w)
+    seed = torch.ones_like(y, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        torch.autograd.grad(y, x, seed, create_graph=True)
+    y, _ = fm.add_rms_norm(x, w)
+    y.sum().backward()
+    with pytest.raises(RuntimeError):
+        y.sum().backward()  # freed, as with any node
+    with pytest.raises(RuntimeError, match="transforms"):
+        torch.func.vmap(lambda t: fm.add_rms_norm(t, w)[0])(rand(2, 4, 32))
+
+
+def test_inference_mode_and_parameters():
+    w = torch.nn.Parameter(rand(64, seed=1))
+    with torch.inference_mode():
+        x = rand(3, 64)
+        y, h = fm.add_rms_norm(x, w, x)
+        r = fm.add_rms_norm_int8(x, w, x)
+        assert torch.equal(r.normed, y) and not y.requires_grad
+        assert fm.quantize_rows(x).dequantize().shape == (3, 64)
