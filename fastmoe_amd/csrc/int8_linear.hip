@@ -198,8 +198,8 @@ __device__ __forceinline__ void zero_rows(const LinearArgs& a, const Tile& t, in
 // Few rows and few columns: 16 x 16 results in a workgroup, whose eight waves take 128-byte pieces of K
 // in turn, straight from memory to the matrix units' registers, and add their int32 parts in LDS.
 // Where even the smallest tile below leaves most CUs without work, splitting K over the waves is what is
-// left: 11.8 against 14.9 us for one row and [2048, 7168] weights, 32 workgroups of 32 x 64 (but 27.8
-// against 26.7 us with eight experts' weights, 256 workgroups).
+// left: 9.2 against 19 us for one row and [2048, 7168] weights, 32 workgroups of 32 x 64 (but 27.9
+// against 25.1 us with eight experts' weights, 256 workgroups).
 constexpr int kFewWaves = 8;
 template <typename TO> __global__ __launch_bounds__(kFewWaves * kWave) void k_int8_few(LinearArgs a) {
   __shared__ i32x4 part[kFewWaves][kWave];
@@ -253,10 +253,10 @@ template <typename TO> __global__ __launch_bounds__(kFewWaves * kWave) void k_in
 typedef int32_t i32x16 __attribute__((ext_vector_type(16)));
 #define FMOE_LDS __attribute__((address_space(3)))
 
-__device__ __forceinline__ void load_piece(const uint8_t* from, uint8_t* to) {
+template <int CPOL> __device__ __forceinline__ void load_piece(const uint8_t* from, uint8_t* to) {
   __builtin_amdgcn_global_load_lds(reinterpret_cast<const FMOE_GLOBAL uint32_t*>(
                                        reinterpret_cast<uintptr_t>(from)),
-                                   (FMOE_LDS uint32_t*)to, 16, 0, 0);
+                                   (FMOE_LDS uint32_t*)to, 16, 0, CPOL);
 }
 // All but the youngest `LOADS` loads of this wave have arrived, and all its LDS reads.
 template <int LOADS> __device__ __forceinline__ void wait_loads() {
@@ -272,7 +272,7 @@ __device__ __forceinline__ void barrier() {
 }
 template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, int CPOL>
 __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   constexpr int kWaves = WR * WC;
   constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 tiles of a wave
@@ -311,8 +311,8 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
             (lane % (KB / 16) ^ swizzle<KB>(r)) * 16;
   }
   auto load_one = [&](uint8_t* s, int64_t at, int i) {
-    if (i < PX) load_piece(xp[i < PX ? i : 0] + at, s + (wave * PX + i) * 1024);
-    else load_piece(wp[i < PX ? 0 : i - PX] + at, s + BM * KB + (wave * PW + i - PX) * 1024);
+    if (i < PX) load_piece<kCPolCached>(xp[i < PX ? i : 0] + at, s + (wave * PX + i) * 1024);
+    else load_piece<CPOL>(wp[i < PX ? 0 : i - PX] + at, s + BM * KB + (wave * PW + i - PX) * 1024);
   };
   auto load = [&](uint8_t* s, int64_t at) {
 #pragma unroll
@@ -521,11 +521,11 @@ template <typename TO> int launch_few(const char* who, LinearArgs a, hipStream_t
   return fmoe_host::check_launch(who);
 }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, int CPOL>
 int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
   const int64_t groups = grid_of(who, &a, BM, BN, WR * WC * kWave);
   if (groups < 0) return FMOE_ERANGE;
-  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES>), dim3((unsigned)groups),
+  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES, CPOL>), dim3((unsigned)groups),
                      dim3(WR * WC * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
@@ -533,14 +533,18 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 // The variant for these sizes: the largest tile that the experts' rows fill and that leaves no CU
 // without work.  `per` is the rows of an expert were the routing even, work(bm, bn) the workgroups then.
 // Times in us of 32 experts' [2048, 7168] weights / 128 experts' [1024, 2048] / 8 experts' [4096, 4096]:
-//   rows per expert      1              16             48             128            256
-//   32 x 64         58 / 38 / 24   91 / 58 / 34  123 / 86 / 45  214 / 148 / 72  360 / 246 / 115
-//   128 x 128       80 / 44 / 31   94 / 59 / 36  102 / 65 / 38   152 / 95 / 56  233 / 145 / 77
-//   128 x 256       63 / 45 / 35   83 / 55 / 40   88 / 61 / 42   141 / 85 / 47  191 / 124 / 77
-//   256 x 256       81 / 51 / 42   93 / 60 / 46  100 / 68 / 50   114 / 82 / 57  204 / 120 / 62
-// Long rows of few experts' rows each are streamed best 128 columns wide, where that leaves two workgroups
-// for every CU: 80 against 88 us for 4 rows of each of 32 experts ([2048, 7168]), 142 against 147 for 64 rows
-// over 256 experts, but 391 against 384 for 256 rows, and 43 against 38 at K = 2048.
+//   rows per expert     1              4              16             48              128            256
+//   16 x 16 (few)  70 / 58 / 27  110 / 83 / 37  191 / 137 / 60  431 / 300 / 136
+//   32 x 64        51 / 35 / 24   80 / 50 / 30   82 / 54 / 31   155 / 103 / 51  296 / 183 / 91  563 / 337 / 161
+//   32 x 128       55 / 39 / 30   72 / 46 / 33   73 / 53 / 33   118 / 89 / 37   259 / 158 / 88  487 / 290 / 147
+//   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
+//   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
+//   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
+// Long rows are streamed best 128 columns wide where that leaves two workgroups for every CU (64 rows
+// over 256 experts of [2048, 7168]: 129 us, 32 x 64 132; but 256 rows 358 against 346).
+// Weights that one tile of rows reads (few rows per expert) pass the caches: 32 experts at 48 rows 77
+// us, kept in them 88; with several tiles of rows they are shared through L2 (346 rows: 15.5 against
+// 17.7 us).
 enum Variant { kFew = 16016, k32x64 = 32064, k32x128 = 32128, k128x128 = 128128, k128x256 = 128256, k256x256 = 256256 };
 Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   const int64_t per = rows / E;
@@ -557,12 +561,14 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
 
 template <typename TO> int launch_linear(const char* who, const LinearArgs& a, hipStream_t s) {
   switch (pick(a.rows, a.E, a.N, a.Kp)) {
-    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4>(who, a, s);
-    case k128x256: return launch_tile<TO, 128, 256, 2, 4, 128, 3>(who, a, s);
-    case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4>(who, a, s);
-    case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3>(who, a, s);
+    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4, kCPolCached>(who, a, s);
+    case k128x256:
+      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, kCPol>(who, a, s);
+      return launch_tile<TO, 128, 256, 2, 4, 128, 3, kCPolCached>(who, a, s);
+    case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4, kCPolCached>(who, a, s);
+    case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3, kCPol>(who, a, s);
     case kFew: return launch_few<TO>(who, a, s);
-    default: return launch_tile<TO, 32, 64, 1, 2, 128, 4>(who, a, s);
+    default: return launch_tile<TO, 32, 64, 1, 2, 128, 4, kCPol>(who, a, s);
   }
 }
 
