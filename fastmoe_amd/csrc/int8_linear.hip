@@ -41,6 +41,14 @@ struct Tile {
   int count;
 };
 
+// Lane `lane`'s value, in scalar registers: what hangs on a tile is then the same for the whole wave to
+// the compiler too.
+__device__ __forceinline__ int64_t lane_value(int64_t v, int lane) {
+  const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, lane);
+  const uint32_t hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)((uint64_t)v >> 32), lane);
+  return (int64_t)((uint64_t)hi << 32 | lo);
+}
+
 __device__ __forceinline__ int64_t bounded(int64_t v, int64_t most) {
   return min(max(v, (int64_t)0), most);
 }
@@ -92,8 +100,8 @@ template <int BM> struct TileScan {
       if (!of && want < k) {
         of = k;
         expert += i;
-        first = __shfl(lo[i], at);
-        end = __shfl(lo[i + 1], at);
+        first = lane_value(lo[i], at);
+        end = lane_value(lo[i + 1], at);
       }
       if (!of) want -= k;
     }
