@@ -280,7 +280,7 @@ __device__ __forceinline__ void barrier() {
 }
 template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, int CPOL>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL>
 __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   constexpr int kWaves = WR * WC;
   constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 tiles of a wave
@@ -354,23 +354,30 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   auto at = [&](int piece) { return (int64_t)min(piece, pieces - 1) * KB; };
   // Step i multiplies piece i in buffer `cur`.  Before its last fragments are multiplied, each wave has
   // read all of the piece and waits until its loads of piece i + 1 have arrived; behind the barrier that
-  // holds for every wave, so `next` is read.  Meanwhile the piece before (its buffer `old` was read by
-  // every wave before the last step's barrier) is replaced by piece i + STAGES - 1.  Reads and
-  // loads stand between the products, one or two at a time: issued together they would hold the wave
-  // back while the matrix units run dry.
+  // holds for every wave, so `next` is read, and `cur` is free for piece i + STAGES.  EARLY: that piece's
+  // loads begin there and end before the next barrier (so step i first goes on with piece
+  // i + STAGES - 1 into `old`).  Else they begin with the next step, spread over all of it.  Tiles of 32
+  // rows wait for memory and gain by more in flight (128 rows over 256 experts of [2048, 7168], 32 x 128:
+  // 230 us, else 249; 8 rows, 32 x 64: 22.7 and 25.2), the larger ones nothing (256 x 256, all of
+  // 49152 rows over 64 experts of [2048, 4096]: 471 to 473 us either way).
+  // Reads and loads stand between the products, one or two at a time: issued together they would hold
+  // the wave back while the matrix units run dry.
+  constexpr auto part = [](int k) { return k * kLoads / kSteps; };  // loads before part k of a piece's
   auto step = [&](auto works, uint8_t* old, uint8_t* cur, const uint8_t* next, int i) {
-    const int64_t from = at(i + STAGES - 1);
+    const int64_t rest = at(i + STAGES - 1), from = at(i + STAGES);
 #pragma unroll
     for (int k = 0; k < kSteps; ++k) {
-      const bool last = k + 1 == kSteps;
+      const bool last = k + 1 == kSteps, ahead = EARLY && last;
       if (last) {
-        wait_loads<(STAGES - 3) * kLoads + (kSteps - 1) * kLoads / kSteps>();
+        wait_loads<EARLY ? (STAGES - 2) * kLoads : (STAGES - 3) * kLoads + part(kSteps - 1)>();
         barrier();
       }
-      constexpr int kOps = TM + TN;
-      const int more = (k + 1) * kLoads / kSteps - k * kLoads / kSteps;  // loads in this part
-      const int ops = kOps + more;
+      const int p = !EARLY ? k : last ? 0 : k + 1;
+      const int first = part(p), more = part(p + 1) - first;
+      auto load_next = [&](int o) { load_one(ahead ? cur : old, ahead ? from : rest, first + o); };
       if constexpr (decltype(works)::value) {
+        constexpr int kOps = TM + TN;
+        const int ops = kOps + more;
 #pragma unroll
         for (int j = 0; j < TM * TN; ++j) {
           acc[j / TM][j % TM] = __builtin_amdgcn_mfma_i32_32x32x32_i8(
@@ -378,13 +385,13 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
 #pragma unroll
           for (int o = j * ops / (TM * TN); o < (j + 1) * ops / (TM * TN); ++o) {
             if (o < kOps) read_one(last ? next : cur, last ? 0 : k + 1, (k + 1) & 1, o);
-            else load_one(old, from, k * kLoads / kSteps + o - kOps);
+            else load_next(o - kOps);
           }
           __builtin_amdgcn_sched_barrier(0);
         }
       } else {  // no rows for this wave: it only loads its share
 #pragma unroll
-        for (int o = kOps; o < ops; ++o) load_one(old, from, k * kLoads / kSteps + o - kOps);
+        for (int o = 0; o < more; ++o) load_next(o);
       }
     }
   };
@@ -429,7 +436,10 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
     col_scale[threadIdx.x] = my_col_scale;
     col_bias[threadIdx.x] = my_bias;
   }
-  wait_loads<(STAGES - 2) * kLoads>();
+  constexpr int kBegun = EARLY ? part(1) : 0;  // loads of piece STAGES - 1
+#pragma unroll
+  for (int i = 0; i < kBegun; ++i) load_one(STAGES > 3 ? stage3 : stage2, at(STAGES - 1), i);
+  wait_loads<(STAGES - 2) * kLoads + kBegun>();
   barrier();
 #pragma unroll
   for (int i = 0; i < TM + TN; ++i) read_one(stage0, 0, 0, i);
@@ -529,11 +539,11 @@ template <typename TO> int launch_few(const char* who, LinearArgs a, hipStream_t
   return fmoe_host::check_launch(who);
 }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, int CPOL>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL>
 int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
   const int64_t groups = grid_of(who, &a, BM, BN, WR * WC * kWave);
   if (groups < 0) return FMOE_ERANGE;
-  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES, CPOL>), dim3((unsigned)groups),
+  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES, EARLY, CPOL>), dim3((unsigned)groups),
                      dim3(WR * WC * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
@@ -543,13 +553,17 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 // Times in us of 32 experts' [2048, 7168] weights / 128 experts' [1024, 2048] / 8 experts' [4096, 4096]:
 //   rows per expert     1              4              16             48              128            256
 //   16 x 16 (few)  70 / 58 / 27  110 / 83 / 37  191 / 137 / 60  431 / 300 / 136
-//   32 x 64        51 / 35 / 24   80 / 50 / 30   82 / 54 / 31   155 / 103 / 51  296 / 183 / 91  563 / 337 / 161
-//   32 x 128       55 / 39 / 30   72 / 46 / 33   73 / 53 / 33   118 / 89 / 37   259 / 158 / 88  487 / 290 / 147
+//   32 x 64        52 / 35 / 24   78 / 51 / 31   82 / 55 / 31   156 / 104 / 50  301 / 181 / 90  582 / 327 / 159
+//   32 x 128       57 / 37 / 26   72 / 45 / 32   74 / 51 / 32   124 / 90 / 38   245 / 157 / 79  481 / 285 / 134
 //   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
-// Long rows are streamed best 128 columns wide where that leaves two workgroups for every CU (64 rows
-// over 256 experts of [2048, 7168]: 129 us, 32 x 64 132; but 256 rows 358 against 346).
+// Of the tiles of 32 rows, 512 workgroups of 128 columns run at once, or 768 of 64, in about 4 to 3 parts
+// of time: the sums of those rounds decide for short rows (4 rows of each of E experts of [2048, 2048],
+// 32 x 64 / 32 x 128: E = 24 19.6 / 20.7 us, 32 29.9 / 24.4, 48 38.0 / 39.5, 64 49.8 / 45.3).  Long rows
+// blur the rounds and 64 columns are as good or better (K = 7168: 24 55.9 / 60.4, 48 108 / 108, 96 204 /
+// 205; 256 rows over 64 experts, K = 4096: 105 / 110) but where 128 end in a single round and 64 do not
+// (32: 78 / 72; at one row each, with experts that got none, 52 / 57).
 // Weights that one tile of rows reads (few rows per expert) pass the caches: 32 experts at 48 rows 77
 // us, kept in them 88; with several tiles of rows they are shared through L2 (346 rows: 15.5 against
 // 17.7 us).
@@ -563,20 +577,21 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   if (per >= 16 && work(128, 256) >= 140) return k128x256;
   if (per >= 40 && work(128, 128) >= 128) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
-  if (K >= 4096 && work(32, 128) >= 512) return k32x128;
+  const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
+  if (K < 4096 ? wide <= narrow : rows >= 2 * E && wide == 4 && narrow > 3) return k32x128;
   return k32x64;
 }
 
 template <typename TO> int launch_linear(const char* who, const LinearArgs& a, hipStream_t s) {
   switch (pick(a.rows, a.E, a.N, a.Kp)) {
-    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4, kCPolCached>(who, a, s);
+    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k128x256:
-      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, kCPol>(who, a, s);
-      return launch_tile<TO, 128, 256, 2, 4, 128, 3, kCPolCached>(who, a, s);
-    case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4, kCPolCached>(who, a, s);
-    case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3, kCPol>(who, a, s);
+      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, false, kCPol>(who, a, s);
+      return launch_tile<TO, 128, 256, 2, 4, 128, 3, false, kCPolCached>(who, a, s);
+    case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4, false, kCPolCached>(who, a, s);
+    case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3, true, kCPol>(who, a, s);
     case kFew: return launch_few<TO>(who, a, s);
-    default: return launch_tile<TO, 32, 64, 1, 2, 128, 4, kCPol>(who, a, s);
+    default: return launch_tile<TO, 32, 64, 1, 2, 128, 4, true, kCPol>(who, a, s);
   }
 }
 

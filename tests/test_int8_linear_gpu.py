@@ -113,7 +113,8 @@ KS = [1, 130, 300, 500, 641, 1100]
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
 @pytest.mark.parametrize("tile,E,mean,N,K", [(*t, K) for t in TILES for K in KS] +
-                         [(32128, 130, 5, 500, K) for K in (4000, 4097, 4225)])
+                         [(32064, 130, 5, 500, K) for K in (4000, 4097, 4225)] +
+                         [(32128, 30, 5, 2000, K) for K in (1, 130, 300, 500, 1100, 4000, 4097, 4225)])
 def test_every_tile(tile, E, mean, N, K, dtype):
     """Every tile, with rings of every remainder of pieces, ragged experts and column ends."""
     counts = ragged(E, mean, seed=K)
