@@ -147,7 +147,8 @@ __device__ __forceinline__ Scale8 scale8(uint32_t top_bits) {
   const float top = __uint_as_float(top_bits);
   Scale8 s;
   s.bad = top_bits >= 0x7f800000u;
-  s.scale = s.bad ? __uint_as_float(0x7fc00000u) : top / 127.0f;
+  // the quotient of the largest fp32 number rounds up, and 127 of it are infinite: one step less
+  s.scale = s.bad ? __uint_as_float(0x7fc00000u) : fminf(top / 127.0f, 0x1.020406p+121f);
   // Below 2^-118 the scale would be denormal, and a little lower the quotient overflows: such rows
   // are held as zeros.
   const bool zero = top < 0x1p-118f;

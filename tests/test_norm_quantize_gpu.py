@@ -223,6 +223,18 @@ def test_rows_of_zeros_infinities_and_nan(dtype):
     assert (fm.quantize_rows(tiny * 2).data[0, :8] == 127).all()
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_the_largest_numbers_stay_finite(dtype):
+    top = torch.finfo(dtype).max
+    x = torch.tensor([[top, -top, top / 2, 0.0]], dtype=dtype, device="cuda")
+    # 127 steps are within the scale's rounding (one fp32 step, 2 u) of the largest value
+    for back in (fm.quantize_rows(x).dequantize(), fm.restore_rows(fm.compress_rows(x), torch.float32)):
+        close(back[:, :2], x[:, :2].double(), 3 * U, 0)
+        close(back[:, 2:], x[:, 2:].double(), 0, top / 127 * (0.5 + 127 * 8 * U))
+    again, _ = fm.gelu_compressed_backward(fm.compress_rows(x.float()), torch.ones(1, 4, device="cuda"))
+    assert again.isfinite().all()
+
+
 def test_rows_into_a_wider_buffer_leave_its_rest():
     """The C entry points write a row's own 128-column pieces and nothing of a wider pitch."""
     from fastmoe_amd import _abi
