@@ -137,8 +137,15 @@ bool is_float(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 ||
          t.scalar_type() == at::kHalf;
 }
-bool plain(const Tensor& t) { return t.is_cuda() && t.layout() == c10::kStrided && t.has_storage(); }
-bool recorded(const Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
+// A tensor whose memory holds its values: not a view that stands for their negatives.
+bool plain(const Tensor& t) {
+  return t.is_cuda() && t.layout() == c10::kStrided && t.has_storage() && !t.is_neg();
+}
+// A gradient, of either mode, would be recorded.
+bool recorded(const Tensor& t) {
+  return t.defined() &&
+         ((t.requires_grad() && at::GradMode::is_enabled()) || t._fw_grad(0).defined());
+}
 bool good_matrix(const Tensor& t) {
   return t.defined() && plain(t) && t.dim() == 2 && is_float(t) && t.size(1) >= 1 &&
          (t.size(1) == 1 || t.stride(1) == 1 || t.size(0) == 0);
@@ -154,7 +161,7 @@ bool good_norm(const Tensor& x, const Tensor& weight, const Tensor& residual, do
 }
 bool good_int8(const Tensor& q, const Tensor& s, int64_t features, int64_t dims) {
   return q.defined() && s.defined() && plain(q) && plain(s) && q.scalar_type() == at::kChar &&
-         q.dim() == dims && s.scalar_type() == at::kFloat && s.device() == q.device() &&
+         q.dim() == dims && s.scalar_type() == at::kFloat && s.device() == q.device() && !recorded(s) &&
          s.is_contiguous() && features >= 1 && features <= INT64_MAX - 127 &&
          q.size(dims - 1) == padded(features) &&
          (q.numel() == 0 ||
@@ -168,9 +175,9 @@ bool good_rows8(const Tensor& q, const Tensor& s, int64_t features, int64_t per_
                                     : q.stride(0) >= q.size(1) && q.stride(0) % 16 == 0));
 }
 
-// Rows with unit column stride.
+// Rows with unit column stride, as their memory stands.
 Tensor by_rows(const Tensor& t) {
-  return t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous();
+  return (t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous()).resolve_neg();
 }
 
 class AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {

@@ -31,9 +31,6 @@ import ctypes
 from typing import NamedTuple, Optional, Sequence, Tuple, Union
 
 import torch
-
-
-
 from torch.autograd import forward_ad
 
 from . import _abi, ops
@@ -147,7 +144,8 @@ def _float_code(dtype, what: str = "dtype") -> int:
 
 
 def _not_taken(what: str) -> None:
-    raise ValueError(f"fastmoe_amd: {what} does not take these tensors")
+    raise ValueError(f"fastmoe_amd: {what} does not take these tensors (forward-mode gradients, views that "
+                     "stand for negated memory, and tensors without memory of their own are not read)")
 
 
 class QuantizedRows(NamedTuple):
@@ -162,6 +160,7 @@ class QuantizedRows(NamedTuple):
         out = _call("restore", self.data, self.scales, False, self.features, _float_code(dtype))
         if out is NotImplemented:
             _check_rows8(self, "rows")
+            _no_gradient("dequantize", self.scales)
             _not_taken("dequantize")
         return out
 
@@ -389,7 +388,7 @@ def _check_linear(x, weights, expert_offsets, rows, bias, out_dtype) -> None:
             raise TypeError(f"fastmoe_amd: unsupported bias dtype {bias.dtype}")
         if tuple(bias.shape) != (E, N) and not (E == 1 and tuple(bias.shape) == (N,)):
             raise ValueError(f"fastmoe_amd: bias must be [{E}, {N}], got {tuple(bias.shape)}")
-        _no_gradient("int8_linear", bias)
+    _no_gradient("int8_linear", x.scales, weights.scales, bias)
     _same_device(x.data, weights=data, expert_offsets=expert_offsets, rows=rows, bias=bias)
 
 
@@ -439,6 +438,7 @@ def restore_rows(held: CompressedRows, dtype: torch.dtype) -> torch.Tensor:
     out = _call("restore", held.data, held.scales, True, held.features, _float_code(dtype))
     if out is NotImplemented:
         _check_held(held)
+        _no_gradient("restore_rows", held.scales)
         _not_taken("restore_rows")
     return out
 
@@ -463,6 +463,6 @@ def gelu_compressed_backward(held: CompressedRows, grad: torch.Tensor, *,
         if tuple(grad.shape) != (R, C):
             raise ValueError(f"fastmoe_amd: grad must be [{R}, {C}], got {tuple(grad.shape)}")
         _same_device(held.data, grad=grad)
-        _no_gradient("gelu_compressed_backward", grad)
+        _no_gradient("gelu_compressed_backward", held.scales, grad)
         _not_taken("gelu_compressed_backward")
     return out

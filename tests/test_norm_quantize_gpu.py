@@ -383,6 +383,37 @@ def test_refusals():
         fm.restore_rows(held._replace(features=200), torch.float32)
 
 
+def test_gradients_and_views_that_would_be_lost_are_refused():
+    x, w = rand(4, 64), rand(64, seed=1)
+    q, held = fm.quantize_rows(x), fm.compress_rows(x)
+    weights = fm.quantize_weights(rand(8, 64, seed=2))
+    grown = lambda t: t._replace(scales=t.scales.clone().requires_grad_(True))
+    for call in (lambda: grown(q).dequantize(), lambda: fm.restore_rows(grown(held), torch.float32),
+                 lambda: fm.gelu_compressed_backward(grown(held), x),
+                 lambda: fm.int8_linear(grown(q), weights), lambda: fm.int8_linear(q, grown(weights))):
+        with pytest.raises(RuntimeError, match="no gradient"):
+            call()
+        with torch.no_grad():
+            call()
+    negated = torch._neg_view(x)
+    grads = []
+    for hook in (torch.neg, torch._neg_view):
+        leaf = x.clone().requires_grad_(True)
+        y, _ = fm.add_rms_norm(leaf, w)
+        y.register_hook(hook)
+        y.backward(rand(4, 64, seed=3))
+        grads.append(leaf.grad)
+    assert torch.equal(*grads)
+    for call in (lambda t: fm.quantize_rows(t), lambda t: fm.add_rms_norm(t, w),
+                 lambda t: fm.add_rms_norm_int8(t, w), lambda t: fm.add_rms_norm(x, w, t),
+                 lambda t: fm.gelu_compress(t), lambda t: fm.gelu_compressed_backward(held, t)):
+        with pytest.raises(ValueError, match="negated"):
+            call(negated)
+        with torch.autograd.forward_ad.dual_level():
+            with pytest.raises((ValueError, RuntimeError), match="forward-mode"):
+                call(torch.autograd.forward_ad.make_dual(x, torch.ones_like(x)))
+
+
 def test_outputs_past_the_caches_and_beyond_32_bits():
     """Arrays above 4 GiB (their last rows lie beyond 32-bit offsets), whose y is also large enough to be
     stored past the caches: each row is what the row alone gives."""
