@@ -218,7 +218,10 @@ class _HeldExperts(torch.autograd.Function):
             n1, nb1, n2, nb2 = needs[4 * e:4 * e + 4]
             live = counts[e] > 0 and g is not None
             if dx is not None and counts[e]:
-                torch.mm(he, w1, out=dxs[e])
+                if live:
+                    torch.mm(he, w1, out=dxs[e])
+                else:  # zeros, whatever its rows held
+                    dxs[e].zero_()
             out += [torch.mm(he.t(), x[e]) if n1 and live else None,
                     he.sum(0) if nb1 and live else None,
                     torch.mm(g.t(), a[e]) if n2 and live else None,

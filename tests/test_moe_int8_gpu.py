@@ -313,6 +313,15 @@ def test_held_experts_parts_of_the_gradient():
         assert not fm.compute_experts(moe.experts, x, counts, checkpoint="int8")[0].requires_grad
 
 
+def test_an_expert_without_part_in_the_loss_passes_no_nan_on():
+    moe = layer(64, 96, 2, 1, torch.float32)
+    x = rand(8, 64)
+    x[1, 5] = float("nan")
+    x.requires_grad_(True)
+    fm.compute_experts(moe.experts, x, [4, 4], checkpoint="int8")[1].sum().backward()
+    assert not x.grad[:4].any() and x.grad[4:].isfinite().all() and x.grad[4:].any()
+
+
 def test_held_experts_refusals():
     moe = layer(64, 96, 2, 1, torch.float32)
     x = rand(8, 64)
