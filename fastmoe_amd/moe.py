@@ -104,22 +104,34 @@ def compute_experts(experts: Sequence[nn.Module], recv_data: torch.Tensor,
     return out
 
 
+_HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_pre_hooks")
+
+
+def _computes_as(module: nn.Module, kind: type) -> bool:
+    """``module`` is a ``kind`` whose forward is that class's own."""
+    return (isinstance(module, kind) and type(module).forward is kind.forward
+            and "forward" not in vars(module))
+
+
+def _hooked(*modules: nn.Module) -> bool:
+    return any(getattr(m, hooks, None) for m in modules for hooks in _HOOKS)
+
+
 def _mlp_parameters(experts: Sequence[nn.Module]):
     """[(w1, b1, w2, b2), ...] of experts Sequential(Linear, GELU(), Linear); biases may be None."""
     out = []
     for e, expert in enumerate(experts):
-        parts = list(expert.children()) if isinstance(expert, nn.Sequential) else []
-        if (len(parts) != 3 or not isinstance(parts[0], nn.Linear)
-                or not isinstance(parts[1], nn.GELU) or not isinstance(parts[2], nn.Linear)):
+        parts = list(expert) if _computes_as(expert, nn.Sequential) else []
+        if len(parts) != 3 or not all(
+                _computes_as(p, k) for p, k in zip(parts, (nn.Linear, nn.GELU, nn.Linear))):
             raise TypeError(f"fastmoe_amd: expert {e} is not Sequential(Linear, GELU, Linear)")
         if parts[1].approximate != "none":
             raise ValueError(f"fastmoe_amd: expert {e} has a GELU approximation "
                              f"({parts[1].approximate!r}); the 8-bit operators compute the exact form")
         out.append((parts[0].weight, parts[0].bias, parts[2].weight, parts[2].bias))
-        if any(getattr(p, "_forward_hooks", None) or getattr(p, "_forward_pre_hooks", None)
-               for p in (expert, *parts)):
-            raise ValueError(f"fastmoe_amd: expert {e} has forward hooks, which the 8-bit operators "
-                             "would not call")
+        if _hooked(expert, *parts):
+            raise ValueError(f"fastmoe_amd: expert {e} has hooks, which the 8-bit operators would not "
+                             "call")
     if not out:
         raise ValueError("fastmoe_amd: no experts")
     return out
@@ -343,6 +355,8 @@ class Int8MoEFeedForward(nn.Module):
                  eps: float = 1e-6) -> None:
         super().__init__()
         params = _mlp_parameters(moe.experts)
+        if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
+            raise TypeError("fastmoe_amd: the router is not a Linear without hooks")
         self.dim, self.num_experts, self.top_k, self.eps = moe.dim, moe.num_experts, moe.top_k, eps
         self.hidden = params[0][0].shape[0]
         self.router = nn.Linear(moe.dim, moe.num_experts, bias=moe.router.bias is not None,

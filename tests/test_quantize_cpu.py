@@ -112,3 +112,46 @@ def test_int8_linear_entry_point_refuses():
     assert call(rows=1 << 31) == _abi.ERANGE
     assert call(N=1 << 25, os_=1 << 25) == _abi.ERANGE
     assert call(rows=0, x=None) == _abi.OK
+
+
+def test_modules_that_compute_something_else_are_refused():
+    """The experts' parameters are read without calling the modules."""
+    nn = torch.nn
+
+    class Scaled(nn.Linear):
+        def forward(self, x):
+            return super().forward(x) * 2
+
+    class Named(nn.Linear):  # a subclass that computes the same
+        pass
+
+    class Residual(nn.Sequential):
+        def forward(self, x):
+            return x + super().forward(x)
+
+    def experts(first=nn.Linear, outer=nn.Sequential, act=nn.GELU):
+        return [outer(first(8, 16), act(), nn.Linear(16, 8)) for _ in range(2)]
+
+    x = torch.zeros(4, 8)
+    run = lambda e: fm.compute_experts(e, x, [2, 2], checkpoint="int8")
+    for wrong in (experts(Scaled), experts(outer=Residual), experts(act=nn.SiLU)):
+        with pytest.raises(TypeError, match="Sequential"):
+            run(wrong)
+    for right in (experts(), experts(Named)):
+        with pytest.raises(RuntimeError, match="only on the GPU"):
+            run(right)
+    patched = experts()
+    patched[1][0].forward = lambda x: x
+    with pytest.raises(TypeError, match="Sequential"):
+        run(patched)
+    shared = nn.Linear(8, 8)  # the same module twice: its weight has two gradients
+    with pytest.raises(RuntimeError, match="only on the GPU"):
+        run([nn.Sequential(shared, nn.GELU(), shared) for _ in range(2)])
+    hooked = experts()
+    hooked[0][2].register_full_backward_hook(lambda *a: None)
+    with pytest.raises(ValueError, match="hooks"):
+        run(hooked)
+    layer = fm.MoEFeedForward(8, 16, 2, 1)
+    layer.router = Scaled(8, 2, bias=False)
+    with pytest.raises(TypeError, match="router"):
+        layer.int8()
