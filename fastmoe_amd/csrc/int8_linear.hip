@@ -356,10 +356,11 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   // read all of the piece and waits until its loads of piece i + 1 have arrived; behind the barrier that
   // holds for every wave, so `next` is read, and `cur` is free for piece i + STAGES.  EARLY: that piece's
   // loads begin there and end before the next barrier (so step i first goes on with piece
-  // i + STAGES - 1 into `old`).  Else they begin with the next step, spread over all of it.  Tiles of 32
-  // rows wait for memory and gain by more in flight (128 rows over 256 experts of [2048, 7168], 32 x 128:
-  // 230 us, else 249; 8 rows, 32 x 64: 22.7 and 25.2), the larger ones nothing (256 x 256, all of
-  // 49152 rows over 64 experts of [2048, 4096]: 471 to 473 us either way).
+  // i + STAGES - 1 into `old`).  Else they begin with the next step, spread over all of it.  Tiles that
+  // wait for memory gain by more in flight (128 rows over 256 experts of [2048, 7168], 32 x 128: 230 us,
+  // else 249; 8 rows, 32 x 64: 22.7 and 25.2; 2048 rows over 32 experts of [7168, 2048], 128 x 256: 107.2
+  // and 109.7), the others nothing (128 x 128: 37.7 and 37.4 at 384 rows over 8 experts of
+  // [4096, 4096]; 256 x 256: 471 to 473 us either way at 49152 rows over 64 experts of [2048, 4096]).
   // Reads and loads stand between the products, one or two at a time: issued together they would hold
   // the wave back while the matrix units run dry.
   constexpr auto part = [](int k) { return k * kLoads / kSteps; };  // loads before part k of a piece's
@@ -586,8 +587,8 @@ template <typename TO> int launch_linear(const char* who, const LinearArgs& a, h
   switch (pick(a.rows, a.E, a.N, a.Kp)) {
     case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k128x256:
-      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, false, kCPol>(who, a, s);
-      return launch_tile<TO, 128, 256, 2, 4, 128, 3, false, kCPolCached>(who, a, s);
+      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPol>(who, a, s);
+      return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPolCached>(who, a, s);
     case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3, true, kCPol>(who, a, s);
     case kFew: return launch_few<TO>(who, a, s);
