@@ -185,9 +185,11 @@ __device__ __forceinline__ void unpack8(u32x2 q, float scale, float* v) {
 // fitted here by reweighted least squares up to |x| = T; beyond, both stay positive and x * P(x^2)
 // rises, so Phi goes to 0 or 1.  With degree 8 and T = 5.5, x * Phi is within 4e-7 of the true value,
 // and relatively within 2e-5 down to x = -T; with degree 6 and T = 5 within 3e-6, relatively 2.4e-4:
-// a sixteenth of bf16's half step, a seventeenth of half an 8-bit step.  13 and 11 instructions and
-// two quarter-rate ones (2^x, 1 / x) an element, where erf takes about 50: at 2 bytes an element
-// those bound the kernels instead of HBM.
+// a sixteenth of bf16's half step.  13 and 11 instructions and two quarter-rate ones (2^x, 1 / x) an
+// element, where erf takes about 50: at 2 bytes an element those bound the kernels instead of HBM
+// (49152 x 2048 to 8 bits: 59 us with degree 6, 64 with 8).  In 8 bits an error moves values near a
+// border to the next whole number: that shows beside fp16's rounding (error of the restored rows
+// against 64 bits 4.2e-4 with degree 6, 2.5e-4 with 8, 2.3e-4 with erf), not beside bf16's (1.6e-3).
 // fp32 values take erfc, which is exact to its last bits.
 template <typename T> __device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (ElemInfo<T>::kBytes == 4) {
@@ -222,9 +224,6 @@ template <typename T> __device__ __forceinline__ float gelu(float x) {
   x = __builtin_elementwise_maximum(x, -3.402823466e38f);
   return x * normal_cdf<T>(x);
 }
-// The type whose GELU is close enough for a result of 8 bits.
-template <typename T> struct Gelu8 { using type = bf16_t; };
-template <> struct Gelu8<float> { using type = float; };
 // d gelu / dx = Phi(x) + x * phi(x)
 template <typename T> __device__ __forceinline__ float gelu_slope(float x, float cdf) {
   const float e = __builtin_amdgcn_exp2f(-0.72134752f * x * x);

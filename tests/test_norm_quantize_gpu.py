@@ -223,6 +223,19 @@ def test_rows_of_zeros_infinities_and_nan(dtype):
     assert (fm.quantize_rows(tiny * 2).data[0, :8] == 127).all()
 
 
+def test_gelu_of_half_precision_rows():
+    """GELU's error moves values near a border to the next whole number: for fp16 it is the one that its
+    own results have, 4e-7, not the larger one that bf16's rounding covers."""
+    x = rand(64, 2048, dtype=torch.float16, seed=9) * 3
+    v = x.double() * cdf64(x.double())
+    e = 4e-7 + 16 * U * float(x.double().abs().max())
+    g = fm.quantize_rows(x, activation="gelu")
+    close(g.scales, v.abs().amax(-1) / 127, 8 * U, e / 127)
+    step = g.scales.double().unsqueeze(-1)
+    err = (g.data[:, :2048].double() * step - v).abs()
+    assert (err <= 0.5 * step + 2 * e + 64 * U * v.abs()).all()
+
+
 @pytest.mark.parametrize("dtype", TYPES)
 def test_the_largest_numbers_stay_finite(dtype):
     top = torch.finfo(dtype).max
