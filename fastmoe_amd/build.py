@@ -105,7 +105,7 @@ def _host_ext_command(cxx: str, name: str, source: str):
     cmd = [cxx, *CXX_FLAGS, "-shared", f"-D_GLIBCXX_USE_CXX11_ABI={abi}", "-D__HIP_PLATFORM_AMD__",
            str(CSRC / source), "-o", str(tmp), *[f"-I{i}" for i in incs],
            *[f"-L{d}" for d in libdirs], *[f"-Wl,-rpath,{d}" for d in libdirs], "-lc10", "-lc10_hip",
-           "-ltorch", "-ltorch_cpu", "-ltorch_python"]
+           "-ltorch", "-ltorch_cpu", "-ltorch_hip", "-ltorch_python"]
     return cmd, tmp, path
 
 
