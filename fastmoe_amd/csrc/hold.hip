@@ -14,12 +14,17 @@
 
 namespace fmoe {
 
-// A workgroup is `1 << tx` vectors of eight columns wide and kGroup >> tx rows high; `chunks`
-// workgroups side by side cover a row.
+// Rows of a thread, which asks for all of them first: 32768 x 2048 in bf16 take 59.3 us (GELU and 8 bits), 34.5
+// (8 bits) and 32.1 (back), with one row 62.2, 36.8 and 35.1, with four 60.4, 34.3 and 31.8; GELU's
+// backward 85 either way.  In fp32 restoring two takes 78 us, one 60.
+template <typename T> constexpr int hold_rows() { return ElemInfo<T>::kBytes == 2 ? 2 : 1; }
+
+// A workgroup is `1 << tx` vectors of eight columns wide and step = kGroup >> tx rows high, and goes
+// on to the next `step` rows `each` times; `chunks` workgroups side by side cover a row.
 struct HoldGrid {
-  int tx, chunks;
+  int tx, chunks, step, each;
   __device__ __forceinline__ bool place(int64_t rows, int64_t* row, int64_t* col) const {
-    *row = (int64_t)(blockIdx.x / (unsigned)chunks) * (kGroup >> tx) + (threadIdx.x >> tx);
+    *row = (int64_t)(blockIdx.x / (unsigned)chunks) * step * each + (threadIdx.x >> tx);
     *col = ((int64_t)(blockIdx.x % (unsigned)chunks) * (1 << tx) + (threadIdx.x & ((1 << tx) - 1))) * 8;
     return *row < rows;
   }
@@ -38,55 +43,87 @@ struct HoldArgs {
 };
 
 template <typename T, bool GELU> __global__ __launch_bounds__(kGroup) void k_compress(HoldArgs a) {
+  constexpr int ROWS = hold_rows<T>();
   int64_t row, col;
   using V = Eight<T>;
   // the lanes of a block stay together: a row's vectors beyond its last block are whole DPP rows
   if (!a.grid.place(a.rows, &row, &col) || col >= a.blocks * kHoldBlock) return;
-  const typename V::raw_t raw =
-      V::template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols);
-  float f[8];
-  V::V::cvt(raw, f);
-  float top = 0.f;
+  typename V::raw_t raw[ROWS];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
-  const Scale8 s = scale8(row_max(abs_bits(top)));
-  if (col % kHoldBlock == 0) a.scales[row * a.blocks + col / kHoldBlock] = s.scale;
-  *reinterpret_cast<u32x2*>(a.q + row * a.q_stride + col) = pack8(f, s);
-  if constexpr (GELU) {
+  for (int r = 0; r < ROWS; ++r)
+    raw[r] = V::template load<true>(
+        static_cast<const T*>(a.x) + min(row + r * a.grid.step, a.rows - 1) * a.x_stride, col, a.cols);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) f[i] = gelu<T>(f[i]);
-    V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(f));
+  for (int r = 0; r < ROWS; ++r, row += a.grid.step) {
+    if (row >= a.rows) return;
+    float f[8];
+    V::V::cvt(raw[r], f);
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
+    const Scale8 s = scale8(row_max(abs_bits(top)));
+    if (col % kHoldBlock == 0) a.scales[row * a.blocks + col / kHoldBlock] = s.scale;
+    *reinterpret_cast<u32x2*>(a.q + row * a.q_stride + col) = pack8(f, s);
+    if constexpr (GELU) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) f[i] = gelu<T>(f[i]);
+      V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(f));
+    }
   }
 }
 
 template <typename T> __global__ __launch_bounds__(kGroup) void k_restore(HoldArgs a) {
+  constexpr int ROWS = hold_rows<T>();
   int64_t row, col;
   using V = Eight<T>;
   if (!a.grid.place(a.rows, &row, &col) || col >= a.cols) return;
-  const u32x2 q = *reinterpret_cast<const u32x2*>(a.q + row * a.q_stride + col);
-  float f[8];
-  unpack8(q, a.scales[row * a.blocks + (a.blocks > 1 ? col / kHoldBlock : 0)], f);
-  V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(f));
+  u32x2 q[ROWS];
+  float scale[ROWS];
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t at = min(row + r * a.grid.step, a.rows - 1);
+    q[r] = *reinterpret_cast<const u32x2*>(a.q + at * a.q_stride + col);
+    scale[r] = a.scales[at * a.blocks + (a.blocks > 1 ? col / kHoldBlock : 0)];
+  }
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r, row += a.grid.step) {
+    if (row >= a.rows) return;
+    float f[8];
+    unpack8(q[r], scale[r], f);
+    V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(f));
+  }
 }
 
 template <typename T> __global__ __launch_bounds__(kGroup) void k_gelu_backward(HoldArgs a) {
+  constexpr int ROWS = hold_rows<T>();
   int64_t row, col;
   using V = Eight<T>;
   if (!a.grid.place(a.rows, &row, &col) || col >= a.cols) return;
-  const u32x2 q = *reinterpret_cast<const u32x2*>(a.q + row * a.q_stride + col);
-  const typename V::raw_t raw =
-      V::template load<true>(static_cast<const T*>(a.x) + row * a.x_stride, col, a.cols);
-  float f[8], g[8];
-  unpack8(q, a.scales[row * a.blocks + col / kHoldBlock], f);
-  V::V::cvt(raw, g);
+  u32x2 q[ROWS];
+  float scale[ROWS];
+  typename V::raw_t raw[ROWS];
 #pragma unroll
-  for (int i = 0; i < 8; ++i) {
-    const float cdf = normal_cdf<T>(f[i]);
-    g[i] *= gelu_slope<T>(f[i], cdf);
-    f[i] *= cdf;
+  for (int r = 0; r < ROWS; ++r) {
+    const int64_t at = min(row + r * a.grid.step, a.rows - 1);
+    q[r] = *reinterpret_cast<const u32x2*>(a.q + at * a.q_stride + col);
+    raw[r] = V::template load<true>(static_cast<const T*>(a.x) + at * a.x_stride, col, a.cols);
+    scale[r] = a.scales[at * a.blocks + col / kHoldBlock];
   }
-  if (a.again) V::store(static_cast<T*>(a.again) + row * a.cols, col, a.cols, V::V::pack(f));
-  V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(g));
+#pragma unroll
+  for (int r = 0; r < ROWS; ++r, row += a.grid.step) {
+    if (row >= a.rows) return;
+    float f[8], g[8];
+    unpack8(q[r], scale[r], f);
+    V::V::cvt(raw[r], g);
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      const float cdf = normal_cdf<T>(f[i]);
+      g[i] *= gelu_slope<T>(f[i], cdf);
+      f[i] *= cdf;
+    }
+    if (a.again) V::store(static_cast<T*>(a.again) + row * a.cols, col, a.cols, V::V::pack(f));
+    V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(g));
+  }
 }
 
 }  // namespace fmoe
@@ -110,7 +147,10 @@ int hold_args(const char* who, int64_t rows, int64_t cols, int dtype, const void
   a->grid.tx = 4;  // 16 lanes: one block
   while (a->grid.tx < 8 && (1 << a->grid.tx) < vectors) ++a->grid.tx;
   const int64_t chunks = (vectors + (1 << a->grid.tx) - 1) >> a->grid.tx;
-  const int64_t high = (rows + (kGroup >> a->grid.tx) - 1) / (kGroup >> a->grid.tx);
+  a->grid.step = kGroup >> a->grid.tx;
+  a->grid.each = dtype == FMOE_F32 ? hold_rows<float>() : hold_rows<bf16_t>();
+  const int64_t rows_of_group = a->grid.step * a->grid.each;
+  const int64_t high = (rows + rows_of_group - 1) / rows_of_group;
   // a launch has fewer than 2^32 threads
   if (cols > (int64_t(1) << 30) || rows > (int64_t(1) << 34) ||
       high > ((int64_t(1) << 24) - 1) / chunks) {
