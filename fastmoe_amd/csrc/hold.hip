@@ -118,7 +118,7 @@ template <typename T> __global__ __launch_bounds__(kGroup) void k_gelu_backward(
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
       const float cdf = normal_cdf<T>(f[i]);
-      g[i] *= gelu_slope<T>(f[i], cdf);
+      g[i] *= gelu_slope(f[i], cdf);
       f[i] *= cdf;
     }
     if (a.again) V::store(static_cast<T*>(a.again) + row * a.cols, col, a.cols, V::V::pack(f));

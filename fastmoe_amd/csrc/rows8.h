@@ -224,10 +224,10 @@ template <typename T> __device__ __forceinline__ float gelu(float x) {
   x = __builtin_elementwise_maximum(x, -3.402823466e38f);
   return x * normal_cdf<T>(x);
 }
-// d gelu / dx = Phi(x) + x * phi(x)
-template <typename T> __device__ __forceinline__ float gelu_slope(float x, float cdf) {
-  const float e = __builtin_amdgcn_exp2f(-0.72134752f * x * x);
-  return cdf + (e == 0.f ? 0.f : 0.39894228f * x * e);
+// d gelu / dx = Phi(x) + x * phi(x), for a finite x (or NaN).
+__device__ __forceinline__ float gelu_slope(float x, float cdf) {
+  const float e = __builtin_amdgcn_exp2f(-0.72134752f * (x * x));
+  return __builtin_fmaf(0.39894228f * x, e, cdf);
 }
 
 }  // namespace fmoe
