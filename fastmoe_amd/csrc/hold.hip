@@ -15,8 +15,8 @@
 namespace fmoe {
 
 // Rows of a thread, which asks for all of them first: 32768 x 2048 in bf16 take 59.3 us (GELU and 8 bits), 34.5
-// (8 bits) and 32.1 (back), with one row 62.2, 36.8 and 35.1, with four 60.4, 34.3 and 31.8; GELU's
-// backward 85 either way.  In fp32 restoring two takes 78 us, one 60.
+// (8 bits) and 32.1 (back, through the caches), with one row 62.2, 36.8 and 35.1, with four 60.4, 34.3 and
+// 31.8; GELU's backward 85 either way.  In fp32 restoring two takes 78 us, one 60.
 template <typename T> constexpr int hold_rows() { return ElemInfo<T>::kBytes == 2 ? 2 : 1; }
 
 // A workgroup is `1 << tx` vectors of eight columns wide and step = kGroup >> tx rows high, and goes
@@ -39,8 +39,17 @@ struct HoldArgs {
   float* scales;      // packed [rows, blocks]
   void* out;          // compress: a; restore: x; backward: grad.  Packed.
   void* again;        // backward: gelu of the held rows, packed, or null
+  int past;           // restore, backward: outputs go past the caches
   HoldGrid grid;
 };
+
+template <typename T>
+__device__ __forceinline__ void put(const HoldArgs& a, void* to, int64_t row, int64_t col,
+                                    typename Eight<T>::raw_t v) {
+  T* p = static_cast<T*>(to) + row * a.cols;
+  if (a.past) Eight<T>::template store<true>(p, col, a.cols, v);
+  else Eight<T>::store(p, col, a.cols, v);
+}
 
 template <typename T, bool GELU> __global__ __launch_bounds__(kGroup) void k_compress(HoldArgs a) {
   constexpr int ROWS = hold_rows<T>();
@@ -90,7 +99,7 @@ template <typename T> __global__ __launch_bounds__(kGroup) void k_restore(HoldAr
     if (row >= a.rows) return;
     float f[8];
     unpack8(q[r], scale[r], f);
-    V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(f));
+    put<T>(a, a.out, row, col, V::V::pack(f));
   }
 }
 
@@ -121,8 +130,8 @@ template <typename T> __global__ __launch_bounds__(kGroup) void k_gelu_backward(
       g[i] *= gelu_slope(f[i], cdf);
       f[i] *= cdf;
     }
-    if (a.again) V::store(static_cast<T*>(a.again) + row * a.cols, col, a.cols, V::V::pack(f));
-    V::store(static_cast<T*>(a.out) + row * a.cols, col, a.cols, V::V::pack(g));
+    if (a.again) put<T>(a, a.again, row, col, V::V::pack(f));
+    put<T>(a, a.out, row, col, V::V::pack(g));
   }
 }
 
@@ -167,6 +176,14 @@ int hold_args(const char* who, int64_t rows, int64_t cols, int dtype, const void
   a->q_stride = q_stride;
   a->scales = static_cast<float*>(const_cast<void*>(scales));
   return FMOE_OK;
+}
+
+// Outputs go past the caches from the size at which the combine's does: 32768 x 2048 in bf16, backward 73.5 us
+// and 83, restoring 29.2 and 32.2.  Two 16-byte stores a lane, as fp32's, leave lines that are written in
+// two parts: restoring takes 97 us so and 60 through the caches (the backward, which also computes,
+// 159 and 170).
+int goes_past(const HoldArgs& a, int dtype) {
+  return a.rows * a.cols * fmoe_host::dtype_bytes(dtype) >= FMOE_STREAM_OUT_BYTES;
 }
 
 template <typename F> void by_float(int dtype, F&& f) {
@@ -217,6 +234,7 @@ extern "C" int fmoe_restore_rows(const void* d_q, int64_t q_stride, const float*
   if (rows == 0) return FMOE_OK;
   a.blocks = scales_per_row;
   a.out = d_out;
+  a.past = dtype != FMOE_F32 && goes_past(a, dtype);
   by_float(dtype, [&](auto t) {
     hipLaunchKernelGGL((k_restore<decltype(t)>), dim3((unsigned)groups), dim3(kGroup), 0,
                        static_cast<hipStream_t>(stream), a);
@@ -240,6 +258,7 @@ extern "C" int fmoe_gelu_compressed_backward(const void* d_q, int64_t q_stride,
   a.x_stride = grad_row_stride;
   a.out = d_grad;
   a.again = d_again;
+  a.past = goes_past(a, dtype);
   by_float(dtype, [&](auto t) {
     hipLaunchKernelGGL((k_gelu_backward<decltype(t)>), dim3((unsigned)groups), dim3(kGroup), 0,
                        static_cast<hipStream_t>(stream), a);

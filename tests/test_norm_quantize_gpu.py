@@ -449,6 +449,22 @@ def test_outputs_past_the_caches_and_beyond_32_bits():
     assert torch.equal(q.data[at], fm.quantize_rows(x[at], activation="gelu").data)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+def test_held_outputs_past_the_caches(dtype):
+    """Outputs above 96 MiB, of rows that start anywhere: bit for bit what the rows give in small calls."""
+    C = 1001
+    R = 100 * 2 ** 20 // (C * dtype.itemsize) + 5
+    x, g = rand(R, C, dtype=dtype), rand(R, C, dtype=dtype, seed=1)
+    a, held = fm.gelu_compress(x)
+    back, (again, grad) = fm.restore_rows(held, dtype), fm.gelu_compressed_backward(held, g)
+    for at in (slice(0, 3), slice(R // 2, R // 2 + 129), slice(R - 70, R)):
+        a1, h1 = fm.gelu_compress(x[at])
+        b1, (g1, d1) = fm.restore_rows(h1, dtype), fm.gelu_compressed_backward(h1, g[at])
+        for got, want in ((a, a1), (held.data, h1.data), (held.scales, h1.scales), (back, b1),
+                          (again, g1), (grad, d1)):
+            assert torch.equal(got[at], want)
+
+
 def test_two_streams_at_once():
     """No workspace is shared: interleaved calls on two streams give what each gives alone."""
     sizes = [(700, 1001), (300, 4096)]
