@@ -559,6 +559,10 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
+// With many rows larger tiles pay on fewer CUs: 128 workgroups of 128 x 256 from 105 rows (16 experts
+// of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 64
+// of 128 x 128 from 192 (2 experts of [2048, 7168] at 350 rows 32.0, 32 x 64 44.0; 3 of [1024, 2048] 14.4
+// and 15.4).
 // Of the tiles of 32 rows, 512 workgroups of 128 columns run at once, or 768 of 64, in about 4 to 3 parts
 // of time: the sums of those rounds decide for short rows (4 rows of each of E experts of [2048, 2048],
 // 32 x 64 / 32 x 128: E = 24 19.6 / 20.7 us, 32 29.9 / 24.4, 48 38.0 / 39.5, 64 49.8 / 45.3).  Long rows
@@ -575,8 +579,8 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
     return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
   };
   if (per >= 112 && work(256, 256) >= 192) return k256x256;
-  if (per >= 16 && work(128, 256) >= 140) return k128x256;
-  if (per >= 40 && work(128, 128) >= 128) return k128x128;
+  if (per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
+  if (per >= 40 && work(128, 128) >= (per >= 192 ? 64 : 128)) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
   const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
   if (K < 4096 ? wide <= narrow : rows >= 2 * E && wide == 4 && narrow > 3) return k32x128;
