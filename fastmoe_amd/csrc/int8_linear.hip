@@ -563,6 +563,11 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 // of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 64
 // of 128 x 128 from 192 (2 experts of [2048, 7168] at 350 rows 32.0, 32 x 64 44.0; 3 of [1024, 2048] 14.4
 // and 15.4).
+// The host does not know how uneven the routing is.  Where 128 x 256 costs little on an even one, because there
+// are many workgroups, it is taken from 4 rows on: 2048 rows over 256 experts of [2048, 7168] take 577 us
+// instead of 559 if they are even, but 125 instead of 187 if a few experts have most.  With 512
+// workgroups it would lose either way (64 experts of [2048, 4096] at 8 rows: even 125 and 106, uneven 41
+// and 41).
 // Of the tiles of 32 rows, 512 workgroups of 128 columns run at once, or 768 of 64, in about 4 to 3 parts
 // of time: the sums of those rounds decide for short rows (4 rows of each of E experts of [2048, 2048],
 // 32 x 64 / 32 x 128: E = 24 19.6 / 20.7 us, 32 29.9 / 24.4, 48 38.0 / 39.5, 64 49.8 / 45.3).  Long rows
@@ -580,6 +585,7 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   };
   if (per >= 112 && work(256, 256) >= 192) return k256x256;
   if (per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
+  if (per >= 4 && work(128, 256) >= 1024) return k128x256;
   if (per >= 40 && work(128, 128) >= (per >= 192 ? 64 : 128)) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
   const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
