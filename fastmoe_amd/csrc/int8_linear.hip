@@ -566,9 +566,9 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
 // With many rows larger tiles pay on fewer CUs: 128 workgroups of 128 x 256 from 105 rows (16 experts
-// of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 64
+// of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 72
 // of 128 x 128 from 192 (2 experts of [2048, 7168] at 350 rows 32.0, 32 x 64 44.0; 3 of [1024, 2048] 14.4
-// and 15.4).
+// and 15.4; but 64 of them 21.3 and 20.3, 256 rows and one [4096, 4096]).
 // The host does not know how uneven the routing is.  Where 128 x 256 costs little on an even one, because there
 // are many workgroups, it is taken from 4 rows on: 2048 rows over 256 experts of [2048, 7168] take 577 us
 // instead of 559 if they are even, but 125 instead of 187 if a few experts have most.  With 512
@@ -592,7 +592,7 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   if (per >= 112 && work(256, 256) >= 192) return k256x256;
   if (per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
   if (per >= 4 && work(128, 256) >= 1024) return k128x256;
-  if (per >= 40 && work(128, 128) >= (per >= 192 ? 64 : 128)) return k128x128;
+  if (per >= 40 && work(128, 128) >= (per >= 192 ? 72 : 128)) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
   const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
   if (K < 4096 ? wide <= narrow : rows >= 2 * E && wide == 4 && narrow > 3) return k32x128;
