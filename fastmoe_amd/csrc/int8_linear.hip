@@ -565,6 +565,9 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
+// 256 columns need more than 128 (256 experts of [64, 4096] at 64 rows: 128 x 128 23.9 us, 128 x 256 33.3; of
+// [128, 4096] 37.1 and 39.0), and a workgroup a CU should not take a round more than 128 x 128's two
+// (100 experts of [640, 2048] at 64 rows, 300 workgroups of 128 x 256: 41.3, 128 x 128 30.8).
 // With many rows larger tiles pay on fewer CUs: 128 workgroups of 128 x 256 from 105 rows (16 experts
 // of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 72
 // of 128 x 128 from 192 (2 experts of [2048, 7168] at 350 rows 32.0, 32 x 64 44.0; 3 of [1024, 2048] 14.4
@@ -589,9 +592,12 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   auto work = [&](int64_t bm, int64_t bn) {
     return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
   };
-  if (per >= 112 && work(256, 256) >= 192) return k256x256;
-  if (per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
-  if (per >= 4 && work(128, 256) >= 1024) return k128x256;
+  if (N > 128) {
+    if (per >= 112 && work(256, 256) >= 192) return k256x256;
+    const bool more = (work(128, 256) + 255) / 256 > (work(128, 128) + 511) / 512;
+    if (!more && per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
+    if (!more && per >= 4 && work(128, 256) >= 1024) return k128x256;
+  }
   if (per >= 40 && work(128, 128) >= (per >= 192 ? 72 : 128)) return k128x128;
   if (per <= 16 && work(32, 64) <= 128) return kFew;
   const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
