@@ -14,6 +14,7 @@
 #include "rows8.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace fmoe {
 
@@ -565,13 +566,16 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
-// 256 columns need more than 128 (256 experts of [64, 4096] at 64 rows: 128 x 128 23.9 us, 128 x 256 33.3; of
+// From 112 rows on the large tiles differ by how they fill the CUs: rounds of 256 workgroups of 256 x 256 or of
+// 128 x 256, or 512 of 128 x 128, that take about 8, 5.5 and 5.8 parts of time, counted over the tiles that
+// random routing makes.  In us, 256 x 256 / 128 x 256 / 128 x 128: 8 experts of [4096, 4096] at 256 rows 60 / 72 /
+// -, 160 of [160, 1024] at 160 18.5 / 25.7 / 23.6, 100 of [256, 2048] at 160 26.9 / 20.1 / 24.5, 160 of [384, 1024] at
+// 160 37.4 / 40.0 / 31.2, 194 of [373, 888] at 306 84 / - / 54.5.
+// Below, 256 columns need more than 128 (256 experts of [64, 4096] at 64 rows: 128 x 128 23.9, 128 x 256 33.3; of
 // [128, 4096] 37.1 and 39.0), and a workgroup a CU should not take a round more than 128 x 128's two
 // (100 experts of [640, 2048] at 64 rows, 300 workgroups of 128 x 256: 41.3, 128 x 128 30.8).
-// With many rows larger tiles pay on fewer CUs: 128 workgroups of 128 x 256 from 105 rows (16 experts
-// of [2048, 2048] at 128 rows 20.2 us, 128 x 128 25.8, but at 48 rows of [2048, 1024] 14.4 and 11.8), 72
-// of 128 x 128 from 192 (2 experts of [2048, 7168] at 350 rows 32.0, 32 x 64 44.0; 3 of [1024, 2048] 14.4
-// and 15.4; but 64 of them 21.3 and 20.3, 256 rows and one [4096, 4096]).
+// Where even 16 x 16 leave little work, they are best whatever the rows (2 experts of [95, 6798] at 111 rows
+// 10.9, 32 x 64 17.3; 5 of [46, 4040] at 184 8.2 and 12.7; but 500 workgroups at 20 rows 10.5 and 9.3).
 // The host does not know how uneven the routing is.  Where 128 x 256 costs little on an even one, because there
 // are many workgroups, it is taken from 4 rows on: 2048 rows over 256 experts of [2048, 7168] take 577 us
 // instead of 559 if they are even, but 125 instead of 187 if a few experts have most.  With 512
@@ -592,14 +596,29 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   auto work = [&](int64_t bm, int64_t bn) {
     return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
   };
-  if (N > 128) {
-    if (per >= 112 && work(256, 256) >= 192) return k256x256;
+  if (work(16, 16) <= (per <= 16 ? 512 : 400)) return kFew;
+  if (per >= 112 && N >= 64) {
+    // an expert's tiles of bm rows, on the average over random routing: a last one for some of them
+    auto tiles = [&](double bm) {
+      const double spread = E > 1 ? 2 * std::sqrt((double)per) : 0, least = std::ceil((per - spread) / bm);
+      return E * (least + (E > 1 ? std::clamp((per + spread - least * bm) / (2 * spread), 0.0, 1.0) : 0));
+    };
+    const double g = (double)((N + 255) / 256), t256 = tiles(256) * g, t128 = tiles(128) * g,
+                 t64 = tiles(128) * (double)((N + 127) / 128);
+    auto rounds = [](double t, double at_once) { return t <= 4 * at_once ? std::ceil(t / at_once) : t / at_once + 0.5; };
+    const double c256 = N > 128 && t256 >= 144 ? 8 * rounds(t256, 256) : HUGE_VAL,
+                 c128 = N > 128 && t128 >= 144 ? 5.5 * rounds(t128, 256) : HUGE_VAL,
+                 c64 = t64 >= (per >= 192 ? 72 : 100) ? 5.8 * rounds(t64, 512) : HUGE_VAL;
+    if (c256 < HUGE_VAL && c256 <= c128 && c256 <= c64) return k256x256;
+    if (c128 < HUGE_VAL && c128 <= c64) return k128x256;
+    if (c64 < HUGE_VAL) return k128x128;
+  }
+  if (N > 128 && per < 112) {
     const bool more = (work(128, 256) + 255) / 256 > (work(128, 128) + 511) / 512;
     if (!more && per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
     if (!more && per >= 4 && work(128, 256) >= 1024) return k128x256;
   }
-  if (per >= 40 && work(128, 128) >= (per >= 192 ? 72 : 128)) return k128x128;
-  if (per <= 16 && work(32, 64) <= 128) return kFew;
+  if (per >= 40 && work(128, 128) >= 128) return k128x128;
   const int64_t wide = (work(32, 128) + 511) / 512 * 4, narrow = (work(32, 64) + 767) / 768 * 3;
   if (K < 4096 ? wide <= narrow : rows >= 2 * E && wide == 4 && narrow > 3) return k32x128;
   return k32x64;
