@@ -6,7 +6,8 @@
 // norm's backward runs in the engine's thread without the interpreter.
 //
 // Each function but bind checks its arguments and returns NotImplemented where something is not as it
-// takes it; the caller (quantize.py) then goes through the checks one by one and says what is wrong.
+// takes it, and under tracing; the caller (quantize.py) then goes through the checks one by one and says
+// what is wrong.
 //
 //   bind({name: address}) once, with the library's entry points
 //   norm(x, weight, residual | None, eps, want_y, want_rows8) -> (stream, y | None, data | None, scales | None)
@@ -22,10 +23,12 @@
 #include <ATen/ATen.h>
 #include <ATen/hip/EmptyTensor.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 
 #include <cmath>
 #include <cstring>
@@ -288,6 +291,14 @@ PyObject* attribute(const char* module, const char* name) {
   return PyExc_RuntimeError;
 }
 
+// torch.jit.trace or make_fx records the program: results that come straight from the allocator would
+// enter the record as constants, whatever the inputs.
+bool traced() {
+  using Modes = c10::impl::TorchDispatchModeTLS;
+  return torch::jit::tracer::isTracing() ||
+         Modes::get_mode(c10::impl::TorchDispatchModeKey::PROXY).has_value();
+}
+
 // Runs f with its `want` arguments; no C++ exception leaves it.
 template <Py_ssize_t want, typename F> PyObject* guarded(Py_ssize_t given, F&& f) {
   if (given != want) {
@@ -298,6 +309,7 @@ template <Py_ssize_t want, typename F> PyObject* guarded(Py_ssize_t given, F&& f
     PyErr_SetString(PyExc_RuntimeError, "fastmoe_amd._rows: bind() has not been called");
     return nullptr;
   }
+  if (traced()) return not_taken();
   try {
     return f();
   } catch (const StatusError& e) {

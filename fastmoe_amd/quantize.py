@@ -143,7 +143,20 @@ def _float_code(dtype, what: str = "dtype") -> int:
     return code
 
 
+def _refuse_transforms(what: str) -> None:
+    """These calls are opaque to functorch's transforms, forward-mode gradients and tracing (which would
+    record their results as constants)."""
+    if torch.compiler.is_compiling():  # first: the compiler does not trace the others
+        return
+    if (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
+            or torch._C._get_tracing_state() is not None
+            or torch._C._get_dispatch_mode(torch._C._TorchDispatchModeKey.PROXY) is not None):
+        raise RuntimeError(f"fastmoe_amd: {what} does not run under functorch transforms, "
+                           "forward-mode gradients or tracing")
+
+
 def _not_taken(what: str) -> None:
+    _refuse_transforms(what)
     raise ValueError(f"fastmoe_amd: {what} does not take these tensors (forward-mode gradients, views that "
                      "stand for negated memory, and tensors without memory of their own are not read)")
 
@@ -218,16 +231,6 @@ def _check_norm(x, weight, residual, eps) -> None:
     _same_device(x, weight=weight, residual=residual)
     if not 0.0 <= float(eps) < float("inf"):
         raise ValueError(f"fastmoe_amd: eps must be finite and not negative, got {eps}")
-
-
-def _refuse_transforms(what: str) -> None:
-    """These calls are opaque to functorch's transforms, forward-mode gradients and tracing."""
-    if torch.compiler.is_compiling():  # first: the compiler does not trace the others
-        return
-    if (torch._C._are_functorch_transforms_active() or forward_ad._current_level >= 0
-            or torch._C._get_tracing_state() is not None):
-        raise RuntimeError(f"fastmoe_amd: {what} does not run under functorch transforms, "
-                           "forward-mode gradients or tracing")
 
 
 def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch.Tensor] = None, *,

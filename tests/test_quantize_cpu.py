@@ -155,3 +155,15 @@ def test_modules_that_compute_something_else_are_refused():
     layer.router = Scaled(8, 2, bias=False)
     with pytest.raises(TypeError, match="router"):
         layer.int8()
+
+
+def test_recording_is_refused():
+    """make_fx and torch.jit.trace would keep the example's results as constants."""
+    from torch.fx.experimental.proxy_tensor import make_fx
+
+    w = torch.ones(8)
+    norm = lambda x: fm.add_rms_norm(x, w)[0]
+    for record in (lambda: make_fx(norm)(torch.zeros(2, 8)),
+                   lambda: torch.jit.trace(norm, (torch.zeros(2, 8),))):
+        with pytest.raises(RuntimeError, match="tracing"):
+            record()
