@@ -110,11 +110,20 @@ _HOOKS = ("_forward_hooks", "_forward_pre_hooks", "_backward_hooks", "_backward_
 def _computes_as(module: nn.Module, kind: type) -> bool:
     """``module`` is a ``kind`` whose forward is that class's own."""
     return (isinstance(module, kind) and type(module).forward is kind.forward
-            and "forward" not in vars(module))
+            and type(module).__call__ is kind.__call__ and "forward" not in vars(module))
 
 
 def _hooked(*modules: nn.Module) -> bool:
     return any(getattr(m, hooks, None) for m in modules for hooks in _HOOKS)
+
+
+def _check_layer(layer: nn.Module, kind: type) -> None:
+    """What ``int8`` reads of a layer is all that its call computes."""
+    if not _computes_as(layer, kind):
+        raise TypeError(f"fastmoe_amd: {type(layer).__name__} is not a {kind.__name__} with that class's "
+                        "forward; int8() would lose what it adds")
+    if _hooked(layer):
+        raise ValueError(f"fastmoe_amd: the {kind.__name__} has hooks, which its 8-bit form would not call")
 
 
 def _mlp_parameters(experts: Sequence[nn.Module]):
@@ -312,7 +321,8 @@ class MoEFeedForward(nn.Module):
 
     def int8(self) -> "Int8MoEFeedForward":
         """This layer for serving, its experts' weights in 8 bits (a copy: later changes of this layer
-        do not reach it)."""
+        do not reach it).  A layer with hooks, or a subclass with a forward of its own, is refused: what
+        they add would be lost."""
         return Int8MoEFeedForward(self)
 
 
@@ -335,6 +345,7 @@ class NormedMoEFeedForward(nn.Module):
 
     def int8(self) -> "Int8MoEFeedForward":
         """As :meth:`MoEFeedForward.int8`, the norm included."""
+        _check_layer(self, NormedMoEFeedForward)
         return Int8MoEFeedForward(self.moe, self.norm_weight, self.eps)
 
 
@@ -354,6 +365,7 @@ class Int8MoEFeedForward(nn.Module):
     def __init__(self, moe: MoEFeedForward, norm_weight: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> None:
         super().__init__()
+        _check_layer(moe, MoEFeedForward)
         params = _mlp_parameters(moe.experts)
         if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
             raise TypeError("fastmoe_amd: the router is not a Linear without hooks")

@@ -167,3 +167,48 @@ def test_recording_is_refused():
                    lambda: torch.jit.trace(norm, (torch.zeros(2, 8),))):
         with pytest.raises(RuntimeError, match="tracing"):
             record()
+
+
+def test_layers_that_compute_something_else_are_refused():
+    """The 8-bit layer reads a layer's parts without calling the layer."""
+    class Shared(fm.MoEFeedForward):
+        def __init__(self, *args):
+            super().__init__(*args)
+            self.shared = torch.nn.Linear(args[0], args[0])
+
+        def forward(self, x):
+            return super().forward(x) + self.shared(x)
+
+    class Scaled(fm.NormedMoEFeedForward):
+        def forward(self, x, residual=None):
+            out, stream = super().forward(x, residual)
+            return out * 0.5, stream
+
+    class Called(fm.MoEFeedForward):
+        def __call__(self, x):
+            return super().__call__(x) * 2
+
+    class Named(fm.MoEFeedForward):  # a subclass that computes the same
+        pass
+
+    sizes = (8, 16, 2, 1)
+    for wrong in (Shared(*sizes), Called(*sizes), fm.NormedMoEFeedForward(Shared(*sizes)),
+                  Scaled(fm.MoEFeedForward(*sizes))):
+        with pytest.raises(TypeError, match="forward"):
+            wrong.int8()
+    with pytest.raises(TypeError, match="forward"):
+        fm.Int8MoEFeedForward(Shared(*sizes))
+    patched = fm.MoEFeedForward(*sizes)
+    patched.forward = lambda x: x
+    with pytest.raises(TypeError, match="forward"):
+        patched.int8()
+    for hook in ("register_forward_hook", "register_forward_pre_hook", "register_full_backward_hook"):
+        plain, normed = fm.MoEFeedForward(*sizes), fm.NormedMoEFeedForward(fm.MoEFeedForward(*sizes))
+        inner = fm.NormedMoEFeedForward(fm.MoEFeedForward(*sizes))
+        for module, layer in ((plain, plain), (normed, normed), (inner.moe, inner)):
+            getattr(module, hook)(lambda *a: None)
+            with pytest.raises(ValueError, match="hooks"):
+                layer.int8()
+    for right in (Named(*sizes), fm.NormedMoEFeedForward(Named(*sizes))):
+        with pytest.raises(RuntimeError, match="only on the GPU"):  # the weights are next
+            right.int8()
