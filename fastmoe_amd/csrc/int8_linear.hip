@@ -6,7 +6,10 @@
 // through an index (the dispatch's reverse map: the rows of a token are never copied for its
 // experts), else r.  The sums are int32 and exact (K <= 131071 keeps them in range: 128 * 128 * K <
 // 2^31), so neither the order nor a split of K changes a bit; each is then converted to fp32 once
-// (2^-24), scaled and rounded to the output's type.
+// (2^-24), scaled and rounded to the output's type.  A row's scale below one is multiplied first and
+// a larger one last: then no step overflows or vanishes unless the result does (rows near the largest
+// numbers have scales up to 2^121, which times the sum would be infinite whatever the weights').  The last
+// factor comes with the bias' addition, in one instruction.
 //
 // Rows and weights lie with K innermost, padded with zeros to whole pieces of 128 bytes, so no
 // product needs a tail in K.  Rows of a tile beyond its expert's last repeat that last one, columns
@@ -169,10 +172,17 @@ __device__ __forceinline__ int64_t source_row(const LinearArgs& a, int64_t r) {
   return i >= 0 && i < a.x_rows ? i : -1;
 }
 
+// A row's scale as the factors before and after the output's scale.
+struct RowScale {
+  float before, after;
+  __device__ __forceinline__ explicit RowScale(float s)
+      : before(s < 1.f ? s : 1.f), after(s < 1.f ? 1.f : s) {}  // NaN: after
+};
+
 // Four neighbouring columns of one output row.
 template <typename TO>
 __device__ __forceinline__ void store4(const LinearArgs& a, const Tile& t, int64_t r, int64_t n,
-                                       i32x4 acc, float sx) {
+                                       i32x4 acc, RowScale sx) {
   if (n >= a.N) return;
   TO* p = static_cast<TO*>(a.out) + r * a.out_stride + n;
   float f[4];
@@ -182,8 +192,8 @@ __device__ __forceinline__ void store4(const LinearArgs& a, const Tile& t, int64
   for (int i = 0; i < 4; ++i) {
     f[i] = 0.f;
     if (i < left) {
-      f[i] = (float)acc[i] * sx * sw[i];
-      if (a.bias) f[i] += load_weight(a.bias, a.bias_dtype, t.expert * a.N + n + i);
+      const float bias = a.bias ? load_weight(a.bias, a.bias_dtype, t.expert * a.N + n + i) : 0.f;
+      f[i] = __builtin_fmaf((float)acc[i] * sx.before * sw[i], sx.after, bias);
     }
   }
   if (left == 4) {
@@ -249,7 +259,7 @@ template <typename TO> __global__ __launch_bounds__(kFewWaves * kWave) void k_in
 #pragma unroll
   for (int v = 1; v < kFewWaves; ++v) acc += part[v][lane];
   // lane l of a 16 x 16 result has row l % 16 and columns 4 * (l / 16) + 0..3
-  store4<TO>(a, t, t.row + l16, n0 + quad * 4, acc, row >= 0 ? a.sx[row] : 0.f);
+  store4<TO>(a, t, t.row + l16, n0 + quad * 4, acc, RowScale(row >= 0 ? a.sx[row] : 0.f));
 }
 
 // BM x BN results of one expert in a workgroup of WR x WC waves, each wave (BM / WR) x (BN / WC) of them in
@@ -472,7 +482,7 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   for (int m = 0; m < TM; ++m) {
     const int first = m0 + m * 32;
     if (first >= t.count) break;
-    const float sx = row_scale[first + l32];
+    const RowScale sx(row_scale[first + l32]);
     // lane l of a 32 x 32 result has row l % 32 and columns 8 * q + 4 * (l / 32) + 0..3, q = 0..3
 #pragma unroll
     for (int base = 0; base < TN; base += CT) {
@@ -485,8 +495,8 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
           float f[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            f[j] = (float)acc[base + n][m][4 * q + j] * sx * col_scale[at_col + j] +
-                   col_bias[at_col + j];
+            f[j] = __builtin_fmaf((float)acc[base + n][m][4 * q + j] * sx.before * col_scale[at_col + j],
+                                  sx.after, col_bias[at_col + j]);
           *reinterpret_cast<typename Vec<TO, 4>::raw_t*>(mine + l32 * kPitch + c * kSize) =
               Vec<TO, 4>::pack(f);
         }
