@@ -289,6 +289,12 @@ __device__ __forceinline__ void barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// Between what a wave's lanes write to LDS and what its other lanes read there: LDS serves a wave in order,
+// so no wait is needed, but the compiler, which sees one lane's addresses, must keep that order.
+__device__ __forceinline__ void wave_order() {
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+  __builtin_amdgcn_wave_barrier();
+}
 template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
 
 template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL>
@@ -501,6 +507,7 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
               Vec<TO, 4>::pack(f);
         }
       constexpr int kLanes = CT * 32 * kSize / 16;  // lanes of a row
+      wave_order();
 #pragma unroll
       for (int p = 0; p < 32 * kLanes / kWave; ++p) {
         const int r = p * (kWave / kLanes) + lane / kLanes, c = lane % kLanes * (16 / kSize);
@@ -521,6 +528,7 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
             }
         }
       }
+      wave_order();  // the next tiles' results go where these lay
     }
   }
 }
