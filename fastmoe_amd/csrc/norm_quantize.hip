@@ -385,7 +385,7 @@ __global__ __launch_bounds__(group_threads<THREADS>()) void k_rows8(RowsArgs a) 
     V::V::cvt(raw[v], f[v]);
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
-      if constexpr (GELU) f[v][i] = gelu<T>(f[v][i]);
+      if constexpr (GELU) f[v][i] = gelu8<T>(f[v][i]);
       top = larger(top, f[v][i]);
     }
   }
@@ -410,7 +410,7 @@ __global__ __launch_bounds__(1024) void k_rows8_long(RowsArgs a) {
     V::V::cvt(V::template load<false>(x, col, a.cols), f);
     if constexpr (GELU) {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[i] = gelu<T>(f[i]);
+      for (int i = 0; i < 8; ++i) f[i] = gelu8<T>(f[i]);
     }
   };
   float top = 0.f;

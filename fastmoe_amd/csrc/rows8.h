@@ -187,10 +187,13 @@ __device__ __forceinline__ void unpack8(u32x2 q, float scale, float* v) {
 // and relatively within 2e-5 down to x = -T; with degree 6 and T = 5 within 3e-6, relatively 2.4e-4:
 // a sixteenth of bf16's half step.  13 and 11 instructions and two quarter-rate ones (2^x, 1 / x) an
 // element, where erf takes about 50: at 2 bytes an element those bound the kernels instead of HBM
-// (49152 x 2048 to 8 bits: 59 us with degree 6, 64 with 8).  In 8 bits an error moves values near a
-// border to the next whole number: that shows beside fp16's rounding (error of the restored rows
-// against 64 bits 4.2e-4 with degree 6, 2.5e-4 with 8, 2.3e-4 with erf), not beside bf16's (1.6e-3).
-// fp32 values take erfc, which is exact to its last bits.
+// (49152 x 2048 to 8 bits: 58.5 us with degree 6, 61.5 with 8).  A result of bf16 takes degree 6, one of fp16
+// degree 8, and so do rows that go to 8 bits, whatever their type: there an error moves values near a border to
+// the next whole number, which shows even beside bf16's rounding (restored rows of a prompt against 64
+// bits: 1.61e-3 with degree 6, 1.56e-3 with 8, 1.56e-3 with erf).
+// fp32 values take erfc.  Its argument is rounded to within 2^-23 of itself, which the tail amplifies: the
+// result's relative error is up to (x^2 + 2) * 2^-23 for a negative x (1e-5 at x = -10, where 1 + erf has no
+// bits left), and a few half steps around and above zero.
 template <typename T> __device__ __forceinline__ float normal_cdf(float x) {
   if constexpr (ElemInfo<T>::kBytes == 4) {
     return 0.5f * erfcf(-0.70710678118654752f * x);
@@ -223,6 +226,10 @@ template <typename T> __device__ __forceinline__ float normal_cdf(float x) {
 template <typename T> __device__ __forceinline__ float gelu(float x) {
   x = __builtin_elementwise_maximum(x, -3.402823466e38f);
   return x * normal_cdf<T>(x);
+}
+// The same of a value that goes to 8 bits.
+template <typename T> __device__ __forceinline__ float gelu8(float x) {
+  return gelu<std::conditional_t<std::is_same<T, bf16_t>::value, f16_t, T>>(x);
 }
 // d gelu / dx = Phi(x) + x * phi(x), for a finite x (or NaN).
 __device__ __forceinline__ float gelu_slope(float x, float cdf) {
