@@ -196,7 +196,7 @@ class _HeldExperts(torch.autograd.Function):
             if xe.shape[0]:
                 _mm(xe, w1.t(), b1, he)
         a, held_h = _compress(h, True)
-        del h
+        del h, he  # he: the last expert's part of it
         outs = []
         for ae, (_, _, w2, b2) in zip(a.split(counts), params):
             y = a.new_empty((ae.shape[0], w2.shape[0]))
@@ -227,7 +227,7 @@ class _HeldExperts(torch.autograd.Function):
             elif de.shape[0]:
                 torch.mm(g, w2, out=de)
         a, dh = gelu_compressed_backward(CompressedRows(hd, hs, hidden), da, again=any(needs[2::4]))
-        del da
+        del da, de
         x = None
         if any(needs[0::4]):
             x = restore_rows(CompressedRows(xd, xs, D), ctx.dtype).split(counts)
