@@ -2,7 +2,7 @@
 //
 // Every block of 128 columns of a row has a scale of its own (rows8.h): 1.03 bytes an element
 // instead of 2 or 4, each value within 1/254 of its block's largest.
-//   compress        q, s of x; with GELU also a = gelu(x) of the exact x
+//   compress        q, s of x; with GELU also a = gelu(x) of the exact x, or a alone
 //   restore         q * s
 //   GELU's backward held = q * s;  again = gelu(held);  grad = grad_a * gelu'(held)
 //
@@ -35,7 +35,7 @@ struct HoldArgs {
   const void* x;      // compress: the rows; backward: grad_a
   int64_t x_stride;   // elements
   int64_t rows, cols, blocks;
-  uint8_t* q;         // rows of q_stride bytes
+  uint8_t* q;         // rows of q_stride bytes; null (compress) where only a is wanted
   int64_t q_stride;
   float* scales;      // packed [rows, blocks]
   void* out;          // compress: a; restore: x; backward: grad.  Packed.
@@ -52,7 +52,7 @@ __device__ __forceinline__ void put(const HoldArgs& a, void* to, int64_t row, in
   else Eight<T>::store(p, col, a.cols, v);
 }
 
-template <typename T, bool GELU> __global__ __launch_bounds__(kGroup) void k_compress(HoldArgs a) {
+template <typename T, bool HOLD, bool GELU> __global__ __launch_bounds__(kGroup) void k_compress(HoldArgs a) {
   constexpr int ROWS = hold_rows<T>();
   int64_t row, col;
   using V = Eight<T>;
@@ -68,12 +68,14 @@ template <typename T, bool GELU> __global__ __launch_bounds__(kGroup) void k_com
     if (row >= a.rows) return;
     float f[8];
     V::V::cvt(raw[r], f);
-    float top = 0.f;
+    if constexpr (HOLD) {
+      float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
-    const Scale8 s = scale8(row_max(abs_bits(top)));
-    if (col % kHoldBlock == 0) a.scales[row * a.blocks + col / kHoldBlock] = s.scale;
-    *reinterpret_cast<u32x2*>(a.q + row * a.q_stride + col) = pack8(f, s);
+      for (int i = 0; i < 8; ++i) top = larger(top, f[i]);
+      const Scale8 s = scale8(row_max(abs_bits(top)));
+      if (col % kHoldBlock == 0) a.scales[row * a.blocks + col / kHoldBlock] = s.scale;
+      *reinterpret_cast<u32x2*>(a.q + row * a.q_stride + col) = pack8(f, s);
+    }
     if constexpr (GELU) {
 #pragma unroll
       for (int i = 0; i < 8; ++i) f[i] = gelu<T>(f[i]);
@@ -142,15 +144,16 @@ using namespace fmoe;
 
 namespace {
 
-// Fills in the grid and checks what every call has; *groups = 0 where there is nothing to do.
+// Fills in the grid and checks what every call has; *groups = 0 where there is nothing to do.  `held`: there
+// are rows in 8 bits.
 int hold_args(const char* who, int64_t rows, int64_t cols, int dtype, const void* q,
-              int64_t q_stride, const void* scales, HoldArgs* a, int64_t* groups) {
+              int64_t q_stride, const void* scales, HoldArgs* a, int64_t* groups, bool held = true) {
   FMOE_REQUIRE(rows >= 0 && cols >= 1, "%s: bad sizes rows=%lld columns=%lld", who, (long long)rows,
                (long long)cols);
   FMOE_REQUIRE(fmoe_host::is_float_dtype(dtype), "%s: bad dtype %d", who, dtype);
-  FMOE_REQUIRE(rows == 0 || (q && scales), "%s: null device pointer", who);
-  FMOE_REQUIRE(reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 16 == 0 &&
-                   q_stride >= fmoe_host::round_up(cols, kHoldBlock),
+  FMOE_REQUIRE(rows == 0 || !held || (q && scales), "%s: null device pointer", who);
+  FMOE_REQUIRE(!held || (reinterpret_cast<uintptr_t>(q) % 16 == 0 && q_stride % 16 == 0 &&
+                         q_stride >= fmoe_host::round_up(cols, kHoldBlock)),
                "%s: 8-bit rows must start at multiples of 16 bytes and have room for whole blocks",
                who);
   const int64_t vectors = fmoe_host::round_up(cols, kHoldBlock) / 8;
@@ -202,7 +205,8 @@ extern "C" int fmoe_compress_rows(const void* d_x, int64_t x_row_stride, int64_t
   const char* who = "fmoe_compress_rows";
   HoldArgs a{};
   int64_t groups;
-  if (int rc = hold_args(who, rows, cols, dtype, d_q, q_stride, d_scales, &a, &groups)) return rc;
+  const bool held = d_q || d_scales || !d_gelu;
+  if (int rc = hold_args(who, rows, cols, dtype, d_q, q_stride, d_scales, &a, &groups, held)) return rc;
   FMOE_REQUIRE(rows == 0 || d_x, "%s: null device pointer", who);
   FMOE_REQUIRE(x_row_stride >= 0, "%s: negative row stride", who);
   if (rows == 0) return FMOE_OK;
@@ -212,10 +216,10 @@ extern "C" int fmoe_compress_rows(const void* d_x, int64_t x_row_stride, int64_t
   by_float(dtype, [&](auto t) {
     using T = decltype(t);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (d_gelu)
-      hipLaunchKernelGGL((k_compress<T, true>), dim3((unsigned)groups), dim3(kGroup), 0, s, a);
-    else
-      hipLaunchKernelGGL((k_compress<T, false>), dim3((unsigned)groups), dim3(kGroup), 0, s, a);
+    const dim3 grid((unsigned)groups), group(kGroup);
+    if (!held) hipLaunchKernelGGL((k_compress<T, false, true>), grid, group, 0, s, a);
+    else if (d_gelu) hipLaunchKernelGGL((k_compress<T, true, true>), grid, group, 0, s, a);
+    else hipLaunchKernelGGL((k_compress<T, true, false>), grid, group, 0, s, a);
   });
   return fmoe_host::check_launch(who);
 }

@@ -13,7 +13,7 @@
 //   norm(x, weight, residual | None, eps, want_y, want_rows8) -> (stream, y | None, data | None, scales | None)
 //   norm_recorded(x, weight, residual | None, eps) -> (y, stream): records its backward
 //   quantize(x, activation) -> (data, scales)
-//   compress(x, gelu) -> (gelu(x) | None, data, scales)
+//   compress(x, gelu, hold) -> (gelu(x) | None, data | None, scales | None)
 //   restore(data, scales, a scale for every 128 columns, features, dtype code) -> values
 //   gelu_backward(data, scales, features, grad, again) -> (gelu | None, grad)
 //   linear(x data, x scales, features, weights, their scales, offsets | None, rows | None, bias | None,
@@ -394,14 +394,17 @@ PyObject* quantize(PyObject*, PyObject* const* a, Py_ssize_t n) {
 }
 
 PyObject* compress(PyObject*, PyObject* const* a, Py_ssize_t n) {
-  return guarded<2>(n, [&] {
+  return guarded<3>(n, [&] {
     if (!tensors({a[0]})) return not_taken();
     const Tensor x = tensor(a[0]);
     if (!good_matrix(x) || recorded(x)) return not_taken();
     const int64_t pad = padded(x.size(1)), R = x.size(0), C = x.size(1);
     Place place(x);
-    const Tensor q = empty({R, pad}, x, at::kChar), s = empty({R, pad / 128}, x, at::kFloat);
-    Tensor g;
+    Tensor g, q, s;
+    if (a[2] == Py_True) {
+      q = empty({R, pad}, x, at::kChar);
+      s = empty({R, pad / 128}, x, at::kFloat);
+    }
     if (a[1] == Py_True) g = empty({R, C}, x);
     if (R)
       check(api.fmoe_compress_rows(data(x), pitch(x), R, C, code(x.scalar_type()), data(q), pad,
@@ -504,7 +507,7 @@ PyMethodDef kMethods[] = {
     {"norm", FMOE_FAST(norm), "norm(x, weight, residual, eps, want_y, want_rows8)"},
     {"norm_recorded", FMOE_FAST(norm_recorded), "norm_recorded(x, weight, residual, eps)"},
     {"quantize", FMOE_FAST(quantize), "quantize(x, activation)"},
-    {"compress", FMOE_FAST(compress), "compress(x, gelu)"},
+    {"compress", FMOE_FAST(compress), "compress(x, gelu, hold)"},
     {"restore", FMOE_FAST(restore), "restore(data, scales, blocks, features, dtype)"},
     {"gelu_backward", FMOE_FAST(gelu_backward), "gelu_backward(data, scales, features, grad, again)"},
     {"linear", FMOE_FAST(linear),

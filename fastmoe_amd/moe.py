@@ -86,7 +86,8 @@ def compute_experts(experts: Sequence[nn.Module], recv_data: torch.Tensor,
     rows and the first product in 8 bits, a scale for every 128 columns, instead of the rows, the
     first product and GELU's output in their own type: about D + F bytes a row instead of 2 D + 4 F at 16
     bits.  The forward is exact; the gradients are those of the held values (each within 1/254 of
-    its block's largest).  Rows and weights share one dtype (autocast's, where it is on).
+    its block's largest).  Without a backward to record nothing is held.  Rows and weights share one
+    dtype (autocast's, where it is on).
     """
     if checkpoint is not None:
         if checkpoint != "int8":
@@ -173,7 +174,7 @@ def _compute_experts_held(experts, recv_data, counts) -> List[torch.Tensor]:
     _refuse_autograd_capture("the experts with held activations", recv_data, records)
     # autocast has done its casts: the products below run in the rows' type
     with torch.autocast("cuda", enabled=False):
-        return list(_HeldExperts.apply(counts, recv_data, *flat))
+        return list(_HeldExperts.apply((counts, records), recv_data, *flat))
 
 
 def _mm(x, w, bias, out):
@@ -186,16 +187,19 @@ def _mm(x, w, bias, out):
 
 class _HeldExperts(torch.autograd.Function):
     """Every expert's Linear, GELU, Linear over the packed rows; what the backward needs of the
-    activations is held in 8 bits.  One launch each way holds or restores all experts' rows."""
+    activations is held in 8 bits.  One launch each way holds or restores all experts' rows.  The first
+    argument is the experts' rows and whether a backward is recorded: ctx.needs_input_grad does not
+    say so (under no_grad it is still true of parameters)."""
 
     @staticmethod
-    def forward(ctx, counts, x, *flat):
+    def forward(ctx, plan, x, *flat):
+        counts, records = plan
         params = [flat[i:i + 4] for i in range(0, len(flat), 4)]
         h = x.new_empty((x.shape[0], params[0][0].shape[0]))
         for xe, he, (w1, b1, _, _) in zip(x.split(counts), h.split(counts), params):
             if xe.shape[0]:
                 _mm(xe, w1.t(), b1, he)
-        a, held_h = _compress(h, True)
+        a, held_h = _compress(h, True, hold=records)
         del h, he  # he: the last expert's part of it
         outs = []
         for ae, (_, _, w2, b2) in zip(a.split(counts), params):
@@ -203,6 +207,8 @@ class _HeldExperts(torch.autograd.Function):
             if ae.shape[0]:
                 _mm(ae, w2.t(), b2, y)
             outs.append(y)
+        if not records:
+            return tuple(outs)
         held_x = _compress(x, False)[1] if any(ctx.needs_input_grad[2::4]) else None
         ctx.counts, ctx.dtype = counts, x.dtype
         ctx.features = (x.shape[1], a.shape[1])

@@ -419,8 +419,9 @@ def _check_held(held: CompressedRows) -> None:
         raise ValueError("fastmoe_amd: held data must be contiguous")
 
 
-def _compress(x: torch.Tensor, gelu: bool, what: str = "compress_rows"):
-    out = _call("compress", x, gelu)
+def _compress(x: torch.Tensor, gelu: bool, what: str = "compress_rows", hold: bool = True):
+    """(gelu(x) or None, x held in 8 bits, or nothing in it without ``hold``)."""
+    out = _call("compress", x, gelu, hold)
     if out is NotImplemented:
         _check_matrix(x, "x")
         _no_gradient(what, x)

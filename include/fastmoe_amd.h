@@ -470,7 +470,8 @@ FMOE_API int fmoe_quantize_rows(const void* d_x, int64_t x_row_stride, int64_t r
 
 /*
  * Rows to 8 bits with a scale for every 128 columns (d_scales: fp32[rows, ceil(cols / 128)]), and, where
- * d_gelu is not null, gelu(x) of the exact x (packed, in `dtype`).
+ * d_gelu is not null, gelu(x) of the exact x (packed, in `dtype`).  With d_gelu, d_q and d_scales may both
+ * be null: GELU alone, in the same bits.
  */
 FMOE_API int fmoe_compress_rows(const void* d_x, int64_t x_row_stride, int64_t rows, int64_t cols,
                                 int dtype, void* d_q, int64_t q_stride, float* d_scales,

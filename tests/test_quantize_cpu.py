@@ -212,3 +212,17 @@ def test_layers_that_compute_something_else_are_refused():
     for right in (Named(*sizes), fm.NormedMoEFeedForward(Named(*sizes))):
         with pytest.raises(RuntimeError, match="only on the GPU"):  # the weights are next
             right.int8()
+
+
+def test_gelu_without_held_rows_at_the_entry_point():
+    lib = _abi.lib()
+
+    def call(q=None, qs=0, sc=None, gelu=DEV, x=DEV, rows=4):
+        return lib.fmoe_compress_rows(x, 8, rows, 8, _abi.F16, q, qs, sc, gelu, None)
+
+    assert call(gelu=None) == _abi.EINVAL             # nothing to write
+    assert call(q=DEV, qs=128) == _abi.EINVAL         # rows without scales
+    assert call(sc=DEV, qs=128) == _abi.EINVAL        # scales without rows
+    assert call(x=None) == _abi.EINVAL
+    assert call(rows=1 << 40) == _abi.ERANGE
+    assert call(rows=0, x=None) == _abi.OK
