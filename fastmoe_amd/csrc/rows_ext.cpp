@@ -27,6 +27,8 @@
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 
@@ -185,6 +187,8 @@ Tensor by_rows(const Tensor& t) {
   return (t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous()).resolve_neg();
 }
 
+constexpr const char* kNoSecond = "fastmoe_amd: the norm's gradient has no gradient of its own";
+
 class AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
  public:
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, Tensor x,
@@ -205,7 +209,7 @@ class AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
     Tensor gy = grads[0], gh = grads.size() > 1 ? grads[1] : Tensor();
     if (at::GradMode::is_enabled() && ((gy.defined() && gy.requires_grad()) ||
                                        (gh.defined() && gh.requires_grad())))
-      throw std::runtime_error("fastmoe_amd: the norm's gradient has no gradient of its own");
+      throw std::runtime_error(kNoSecond);
     // the third input is counted only where there was a residual, which has an output of its own
     const bool need_x = ctx->needs_input_grad(0), need_w = ctx->needs_input_grad(1),
                need_r = grads.size() > 1 && ctx->needs_input_grad(2);
@@ -236,6 +240,15 @@ class AddRmsNorm : public torch::autograd::Function<AddRmsNorm> {
                 data(weight), code(weight.scalar_type()), static_cast<const float*>(data(rstd)), T,
                 D, code(h.scalar_type()), data(gx), data(gw), data(ws), bytes, place.stream),
             "fmoe_add_rms_norm_backward");
+      // Under create_graph the results depend on h and the weight too: who differentiates them is told, and
+      // does not get a part of the derivative.
+      if (at::GradMode::is_enabled() && (h.requires_grad() || weight.requires_grad()))
+        for (Tensor* g : {&gx, &gw})
+          if (g->defined())
+            torch::autograd::set_history(
+                *g, std::shared_ptr<torch::autograd::Node>(
+                        new torch::autograd::Error(kNoSecond, torch::autograd::collect_next_edges(h, weight)),
+                        torch::autograd::deleteNode));
     }
     return {need_x ? gx : Tensor(), need_w ? gw : Tensor(), need_r ? gx : Tensor(), Tensor()};
   }
