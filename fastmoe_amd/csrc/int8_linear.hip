@@ -177,7 +177,16 @@ struct RowScale {
   float before, after;
   __device__ __forceinline__ explicit RowScale(float s)
       : before(s < 1.f ? s : 1.f), after(s < 1.f ? 1.f : s) {}  // NaN: after
+  __device__ __forceinline__ float scaled(int32_t sum, float sw, float bias) const {
+    return __builtin_fmaf((float)sum * before * sw, after, bias);
+  }
 };
+
+// fp32 values before their rounding to fp16.  The compiler would take the last addition and the rounding as
+// one instruction, which is no faster, and whose results are not always the fp32 ones' nearest.
+template <typename TO> __device__ __forceinline__ void apart(float* f) {
+  if constexpr (std::is_same<TO, f16_t>::value) asm("" : "+v"(f[0]), "+v"(f[1]), "+v"(f[2]), "+v"(f[3]));
+}
 
 // Four neighbouring columns of one output row.
 template <typename TO>
@@ -193,9 +202,10 @@ __device__ __forceinline__ void store4(const LinearArgs& a, const Tile& t, int64
     f[i] = 0.f;
     if (i < left) {
       const float bias = a.bias ? load_weight(a.bias, a.bias_dtype, t.expert * a.N + n + i) : 0.f;
-      f[i] = __builtin_fmaf((float)acc[i] * sx.before * sw[i], sx.after, bias);
+      f[i] = sx.scaled(acc[i], sw[i], bias);
     }
   }
+  apart<TO>(f);
   if (left == 4) {
     if constexpr (ElemInfo<TO>::kBytes == 4)
       *reinterpret_cast<u32x4_any*>(p) = Vec<TO, 4>::pack(f);
@@ -501,8 +511,8 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
           float f[4];
 #pragma unroll
           for (int j = 0; j < 4; ++j)
-            f[j] = __builtin_fmaf((float)acc[base + n][m][4 * q + j] * sx.before * col_scale[at_col + j],
-                                  sx.after, col_bias[at_col + j]);
+            f[j] = sx.scaled(acc[base + n][m][4 * q + j], col_scale[at_col + j], col_bias[at_col + j]);
+          apart<TO>(f);
           *reinterpret_cast<typename Vec<TO, 4>::raw_t*>(mine + l32 * kPitch + c * kSize) =
               Vec<TO, 4>::pack(f);
         }

@@ -10,7 +10,7 @@ import torch
 import fastmoe_amd as fm
 from fastmoe_amd import _abi
 
-from .test_int8_linear_gpu import TILES, U, make, ragged, reference, route
+from .test_int8_linear_gpu import TILES, U, check, make, ragged, reference, route
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +49,16 @@ def test_rows_near_the_largest_numbers():
         want = x.double() @ w.double().t()
         # both are their rows' largest: 127 steps of a scale, a few u off
         assert ((got.double() - want).abs() <= (torch.finfo(dtype).eps / 2 + 16 * U) * want).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tile,E,mean,N", [(256256, 50, 130, 1024), (256256, 50, 130, 1025), (128256, 40, 40, 1024),
+                                           (128256, 40, 40, 992)])
+def test_rows_that_start_with_a_line_of_memory_and_inside_one(tile, E, mean, N, dtype):
+    K = 300
+    counts = ragged(E, mean)
+    R = sum(counts)
+    assert _abi.lib().fmoe_int8_linear_tile(R, E, N, K) == tile
+    x, w = make(R, K, E, N, seed=3)
+    got = fm.int8_linear(x, w, route(counts), out_dtype=dtype)
+    check(got, *reference(x, w, counts), dtype)
