@@ -307,7 +307,7 @@ __device__ __forceinline__ void wave_order() {
 }
 template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL, bool PAST>
 __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   constexpr int kWaves = WR * WC;
   constexpr int TM = BM / WR / 32, TN = BN / WC / 32;  // 32 x 32 tiles of a wave
@@ -478,11 +478,6 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
   // Each wave turns its results, 32 rows at a time, into rows of the output's type in LDS and stores
   // them 16 bytes a lane: whole lines of the output.
   constexpr int kSize = ElemInfo<TO>::kBytes;
-  // Tiles of 256 columns store past the caches, which leaves those to rows and weights: 2048 rows over 32 experts
-  // of [7168, 2048] 97 us instead of 109, and 113 instead of 124 with the GELU that reads the results; 16
-  // experts of [2048, 2048] at 128 rows 19.6 and 20.8.  Narrower tiles write parts of lines and lose (13
-  // experts of [900, 1001] at 128 rows 12.6 and 12.0).
-  constexpr bool kPast = BN >= 256;
   // column tiles at a time: as many as the stages hold for every wave
   constexpr auto fits = [](int tiles) {
     return kStage / (32 * (tiles * 32 * kSize + 16)) * STAGES >= kWaves;
@@ -526,7 +521,7 @@ __global__ __launch_bounds__(WR * WC * kWave) void k_int8_tile(LinearArgs a) {
         if (first + r >= t.count || n >= a.N) continue;
         TO* to = static_cast<TO*>(a.out) + (t.row + first + r) * a.out_stride + n;
         if (n + 16 / kSize <= a.N) {
-          if constexpr (kPast) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(to));
+          if constexpr (PAST) __builtin_nontemporal_store(v, reinterpret_cast<u32x4_any*>(to));
           else *reinterpret_cast<u32x4_any*>(to) = v;
         } else {
           const int left = (int)(a.N - n);
@@ -575,12 +570,13 @@ template <typename TO> int launch_few(const char* who, LinearArgs a, hipStream_t
   return fmoe_host::check_launch(who);
 }
 
-template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL>
+template <typename TO, int BM, int BN, int WR, int WC, int KB, int STAGES, bool EARLY, int CPOL,
+          bool PAST = (BN >= 256)>
 int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
   const int64_t groups = grid_of(who, &a, BM, BN, WR * WC * kWave);
   if (groups < 0) return FMOE_ERANGE;
-  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES, EARLY, CPOL>), dim3((unsigned)groups),
-                     dim3(WR * WC * kWave), 0, s, a);
+  hipLaunchKernelGGL((k_int8_tile<TO, BM, BN, WR, WC, KB, STAGES, EARLY, CPOL, PAST>),
+                     dim3((unsigned)groups), dim3(WR * WC * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
@@ -652,9 +648,25 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   return k32x64;
 }
 
+// Tiles of 256 columns store past the caches, which leaves those to rows and weights: 2048 rows over 32 experts
+// of [7168, 2048] 97 us instead of 109, and 113 instead of 124 with the GELU that reads the results; 16
+// experts of [2048, 2048] at 128 rows 19.6 and 20.8.  Narrower tiles write parts of lines and lose (13
+// experts of [900, 1001] at 128 rows 12.6 and 12.0).  Rows that start inside a line have parts of lines at
+// every wave's ends.  16-bit results gain all the same or lose little (N = 7167, 64 rows of 32 experts,
+// K = 2048: 100 and 111; N = 1001, 2048 rows of 8: 65.6 and 62.7).  fp32 ones of 256 x 256, each line of which
+// two of a lane's stores write, lose much (346 rows of 32 experts, K = 512: N = 1001 31 and 23, 7167 169
+// and 147), and gain as much where rows start with a line (N = 4096: 68 and 89).
+bool starts_with_lines(const LinearArgs& a, int64_t bytes) {
+  return reinterpret_cast<uintptr_t>(a.out) % 128 == 0 && a.out_stride * bytes % 128 == 0;
+}
+
 template <typename TO> int launch_linear(const char* who, const LinearArgs& a, hipStream_t s) {
   switch (pick(a.rows, a.E, a.N, a.Kp)) {
-    case k256x256: return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached>(who, a, s);
+    case k256x256:
+      if constexpr (ElemInfo<TO>::kBytes == 4)
+        if (!starts_with_lines(a, 4))
+          return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached, false>(who, a, s);
+      return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k128x256:
       if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPol>(who, a, s);
       return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPolCached>(who, a, s);

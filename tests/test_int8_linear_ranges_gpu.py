@@ -62,3 +62,16 @@ def test_rows_that_start_with_a_line_of_memory_and_inside_one(tile, E, mean, N, 
     x, w = make(R, K, E, N, seed=3)
     got = fm.int8_linear(x, w, route(counts), out_dtype=dtype)
     check(got, *reference(x, w, counts), dtype)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("tile,E,mean,N", [(256256, 50, 130, 1024), (256256, 50, 130, 1025), (128256, 40, 40, 1024),
+                                           (128256, 40, 40, 992)])
+def test_rows_that_start_with_a_line_of_memory_and_inside_one(tile, E, mean, N, dtype):
+    K = 300
+    counts = ragged(E, mean)
+    R = sum(counts)
+    assert _abi.lib().fmoe_int8_linear_tile(R, E, N, K) == tile
+    x, w = make(R, K, E, N, seed=3)
+    got = fm.int8_linear(x, w, route(counts), out_dtype=dtype)
+    check(got, *reference(x, w, counts), dtype)
