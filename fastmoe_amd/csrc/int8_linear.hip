@@ -590,11 +590,16 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 //   128 x 128      80 / 45 / 31   90 / 56 / 36   94 / 59 / 36   102 / 65 / 37   151 / 95 / 56   234 / 144 / 76
 //   128 x 256      58 / 42 / 35   72 / 47 / 37   73 / 50 / 38    77 / 58 / 40   139 / 83 / 46   189 / 123 / 76
 //   256 x 256      81 / 52 / 42   92 / 58 / 45   93 / 60 / 46   100 / 68 / 49   113 / 80 / 56   203 / 120 / 63
-// From 112 rows on the large tiles differ by how they fill the CUs: rounds of 256 workgroups of 256 x 256 or of
-// 128 x 256, or 512 of 128 x 128, that take about 8, 5.5 and 5.8 parts of time, counted over the tiles that
-// random routing makes.  In us, 256 x 256 / 128 x 256 / 128 x 128: 8 experts of [4096, 4096] at 256 rows 60 / 72 /
+// Above 104 rows, from where 128 x 256 keeps its weights in the caches, the large tiles differ by how they fill the
+// CUs: rounds of 256 workgroups of 256 x 256 or of 128 x 256, or 512 of 128 x 128, that take about 8, 5.5 and 5.8
+// parts of time (5.4 where 128 x 128 has a CU for each), counted over the tiles that random routing makes.
+// 256 x 256 is not taken below 144 workgroups, 128 x 256 below 128, and 128 x 128 where those of 32 x 64 are at
+// most two on a CU.  In us, 256 x 256 / 128 x 256 / 128 x 128: 8 experts of [4096, 4096] at 256 rows 60 / 72 /
 // -, 160 of [160, 1024] at 160 18.5 / 25.7 / 23.6, 100 of [256, 2048] at 160 26.9 / 20.1 / 24.5, 160 of [384, 1024] at
-// 160 37.4 / 40.0 / 31.2, 194 of [373, 888] at 306 84 / - / 54.5.
+// 160 37.4 / 40.0 / 31.2, 194 of [373, 888] at 306 84 / - / 54.5; 8 of [4096, 4096] at 106 55.0 / 45.1 / 39.8, 16 of
+// [2048, 2048] 23.4 / 17.5 / 18.3, and at 116, where some have two tiles, 24.9 / 17.9 / 23.0; 32 x 64 against 128 x 128:
+// 8 of [768, 4096] at 132, 440 workgroups of 32 x 64, 19.9 / 24.1, at 160, 528, 26.1 / 20.6; 1 of [5120, 4096] at 192,
+// 480, 20.8 / 20.6, at 224, 560, 25.9 / 21.0; 1 of [4096, 4096] at 256, 512, 20.1 / 21.1.
 // Below, 256 columns need more than 128 (256 experts of [64, 4096] at 64 rows: 128 x 128 23.9, 128 x 256 33.3; of
 // [128, 4096] 37.1 and 39.0), and a workgroup a CU should not take a round more than 128 x 128's two
 // (100 experts of [640, 2048] at 64 rows, 300 workgroups of 128 x 256: 41.3, 128 x 128 30.8).
@@ -615,31 +620,36 @@ int launch_tile(const char* who, LinearArgs a, hipStream_t s) {
 // us, kept in them 88; with several tiles of rows they are shared through L2 (346 rows: 15.5 against
 // 17.7 us).
 enum Variant { kFew = 16016, k32x64 = 32064, k32x128 = 32128, k128x128 = 128128, k128x256 = 128256, k256x256 = 256256 };
+// Rows of an expert up to which one tile of 128 reads its weights, which then pass the caches.
+constexpr int64_t kReadOnce = 104;
 Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   const int64_t per = rows / E;
   auto work = [&](int64_t bm, int64_t bn) {
     return ((N + bn - 1) / bn) * std::max(std::min(E, rows), (rows + bm - 1) / bm);
   };
   if (work(16, 16) <= (per <= 16 ? 512 : 400)) return kFew;
-  if (per >= 112 && N >= 64) {
+  if (per > kReadOnce && N >= 64) {
     // an expert's tiles of bm rows, on the average over random routing: a last one for some of them
     auto tiles = [&](double bm) {
       const double spread = E > 1 ? 2 * std::sqrt((double)per) : 0, least = std::ceil((per - spread) / bm);
       return E * (least + (E > 1 ? std::clamp((per + spread - least * bm) / (2 * spread), 0.0, 1.0) : 0));
     };
     const double g = (double)((N + 255) / 256), t256 = tiles(256) * g, t128 = tiles(128) * g,
-                 t64 = tiles(128) * (double)((N + 127) / 128);
-    auto rounds = [](double t, double at_once) { return t <= 4 * at_once ? std::ceil(t / at_once) : t / at_once + 0.5; };
+                 t64 = tiles(128) * (double)((N + 127) / 128), t32 = tiles(32) * (double)((N + 63) / 64);
+    // an average of a hundredth of a round more is no round more yet
+    auto rounds = [](double t, double at_once) {
+      return t <= 4 * at_once ? std::ceil(t / at_once - 0.01) : t / at_once + 0.5;
+    };
     const double c256 = N > 128 && t256 >= 144 ? 8 * rounds(t256, 256) : HUGE_VAL,
-                 c128 = N > 128 && t128 >= 144 ? 5.5 * rounds(t128, 256) : HUGE_VAL,
-                 c64 = t64 >= (per >= 192 ? 72 : 100) ? 5.8 * rounds(t64, 512) : HUGE_VAL;
+                 c128 = N > 128 && t128 >= 128 ? 5.5 * rounds(t128, 256) : HUGE_VAL,
+                 c64 = t32 <= 512 ? HUGE_VAL : t64 <= 256 ? 5.4 : 5.8 * rounds(t64, 512);
     if (c256 < HUGE_VAL && c256 <= c128 && c256 <= c64) return k256x256;
     if (c128 < HUGE_VAL && c128 <= c64) return k128x256;
     if (c64 < HUGE_VAL) return k128x128;
   }
-  if (N > 128 && per < 112) {
+  if (N > 128 && per <= kReadOnce) {
     const bool more = (work(128, 256) + 255) / 256 > (work(128, 128) + 511) / 512;
-    if (!more && per >= 16 && work(128, 256) >= (per > 104 ? 128 : 140)) return k128x256;
+    if (!more && per >= 16 && work(128, 256) >= 140) return k128x256;
     if (!more && per >= 4 && work(128, 256) >= 1024) return k128x256;
   }
   if (per >= 40 && work(128, 128) >= 128) return k128x128;
@@ -668,7 +678,7 @@ template <typename TO> int launch_linear(const char* who, const LinearArgs& a, h
           return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached, false>(who, a, s);
       return launch_tile<TO, 256, 256, 4, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k128x256:
-      if (a.rows / a.E <= 104) return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPol>(who, a, s);
+      if (a.rows / a.E <= kReadOnce) return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPol>(who, a, s);
       return launch_tile<TO, 128, 256, 2, 4, 128, 3, true, kCPolCached>(who, a, s);
     case k128x128: return launch_tile<TO, 128, 128, 2, 2, 64, 4, false, kCPolCached>(who, a, s);
     case k32x128: return launch_tile<TO, 32, 128, 1, 4, 128, 3, true, kCPol>(who, a, s);

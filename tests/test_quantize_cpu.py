@@ -226,3 +226,21 @@ def test_gelu_without_held_rows_at_the_entry_point():
     assert call(x=None) == _abi.EINVAL
     assert call(rows=1 << 40) == _abi.ERANGE
     assert call(rows=0, x=None) == _abi.OK
+
+
+def test_the_tile_does_not_alternate_with_the_rows():
+    """One row more per expert does not change the tile there and back: at these sizes (none of which is a
+    tie of two tiles' rounds) a choice between two equal ones lasts three row counts at least."""
+    tile = _abi.lib().fmoe_int8_linear_tile
+    for E in (1, 4, 8, 13, 16, 20, 32, 50, 64, 128, 160, 256):
+        for N in (16, 100, 256, 640, 1003, 2048, 3000, 4096, 8192):
+            for K in (128, 2048, 7168):
+                runs = []  # (tile, row counts that it lasts)
+                for per in range(1, 420):
+                    t = tile(per * E, E, N, K)
+                    if runs and runs[-1][0] == t:
+                        runs[-1][1] += 1
+                    else:
+                        runs.append([t, 1])
+                for a, b, c in zip(runs, runs[1:], runs[2:]):
+                    assert a[0] != c[0] or b[1] >= 3, (E, N, K, runs)
