@@ -332,6 +332,13 @@ class MoEFeedForward(nn.Module):
         return Int8MoEFeedForward(self)
 
 
+def _check_residual(x: torch.Tensor, residual: Optional[torch.Tensor]) -> None:
+    """Before both become rows: [T, B, D] would pass for [B, T, D] there."""
+    if residual is not None and residual.shape != x.shape:
+        raise ValueError(f"fastmoe_amd: residual must be {tuple(x.shape)}, got "
+                         f"{tuple(residual.shape)}")
+
+
 class NormedMoEFeedForward(nn.Module):
     """A :class:`MoEFeedForward` behind the root-mean-square norm of a pre-norm block: the residual's
     addition and the norm are one kernel (``add_rms_norm``).  ``forward(x, residual=None)`` returns
@@ -345,6 +352,7 @@ class NormedMoEFeedForward(nn.Module):
                                                    device=moe.router.weight.device))
 
     def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        _check_residual(x, residual)
         flat = None if residual is None else residual.reshape(-1, x.shape[-1])
         y, stream = add_rms_norm(x.reshape(-1, x.shape[-1]), self.norm_weight, flat, eps=self.eps)
         return self.moe(y.view(x.shape)), stream.view(x.shape)
@@ -407,9 +415,7 @@ class Int8MoEFeedForward(nn.Module):
                 raise ValueError("fastmoe_amd: a residual needs the norm (NormedMoEFeedForward.int8)")
             rows, y = quantize_rows(flat), flat
         else:
-            if residual is not None and residual.shape != x.shape:
-                raise ValueError(f"fastmoe_amd: residual must be {tuple(x.shape)}, got "
-                                 f"{tuple(residual.shape)}")
+            _check_residual(x, residual)
             rows, y, stream = add_rms_norm_int8(
                 flat, self.norm_weight, None if residual is None else residual.reshape(-1, D),
                 eps=self.eps)

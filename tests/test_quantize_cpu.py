@@ -244,3 +244,14 @@ def test_the_tile_does_not_alternate_with_the_rows():
                         runs.append([t, 1])
                 for a, b, c in zip(runs, runs[1:], runs[2:]):
                     assert a[0] != c[0] or b[1] >= 3, (E, N, K, runs)
+
+
+def test_a_residual_of_another_shape_is_refused():
+    """Of as many rows, but in another order: batch and tokens exchanged."""
+    layer = fm.NormedMoEFeedForward(fm.MoEFeedForward(8, 16, 2, 1))
+    x = torch.zeros(2, 3, 8)
+    for wrong in (torch.zeros(3, 2, 8), torch.zeros(6, 8), torch.zeros(1, 3, 8)):
+        with pytest.raises(ValueError, match="residual must be"):
+            layer(x, wrong)
+    with pytest.raises(RuntimeError, match="only on the GPU"):
+        layer(x, torch.zeros(2, 3, 8))
