@@ -302,6 +302,7 @@ def quantize_weights(weight: Union[torch.Tensor, Sequence[torch.Tensor]]) -> Int
         parts = list(weight)
         if not parts:
             raise ValueError("fastmoe_amd: no weights")
+    _need_gpu(parts[0], "weight 0")
     N, K = parts[0].shape if parts[0].dim() == 2 else (0, 0)
     for i, p in enumerate(parts):
         _check_matrix(p, f"weight {i}")

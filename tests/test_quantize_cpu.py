@@ -255,3 +255,11 @@ def test_a_residual_of_another_shape_is_refused():
             layer(x, wrong)
     with pytest.raises(RuntimeError, match="only on the GPU"):
         layer(x, torch.zeros(2, 3, 8))
+
+
+def test_weights_that_are_no_tensors_are_refused():
+    for wrong in ([1.0, 2.0], [[1.0]], [None]):
+        with pytest.raises(TypeError, match="weight 0 must be a tensor"):
+            fm.quantize_weights(wrong)
+    with pytest.raises(ValueError, match="no weights"):
+        fm.quantize_weights([])
