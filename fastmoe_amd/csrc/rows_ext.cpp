@@ -26,6 +26,7 @@
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
@@ -325,6 +326,8 @@ template <Py_ssize_t want, typename F> PyObject* guarded(Py_ssize_t given, F&& f
   if (traced()) return not_taken();
   try {
     return f();
+  } catch (python_error& e) {  // Python's own, from a hook on saved tensors: activation checkpointing's way out
+    e.restore();
   } catch (const StatusError& e) {
     PyObject* type = e.code == FMOE_EINVAL    ? PyExc_ValueError
                      : e.code == FMOE_ERANGE ? PyExc_OverflowError
