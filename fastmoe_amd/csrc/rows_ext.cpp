@@ -145,9 +145,12 @@ bool is_float(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 ||
          t.scalar_type() == at::kHalf;
 }
-// A tensor whose memory holds its values: not a view that stands for their negatives.
+// A tensor whose memory holds its values: neither a view that stands for their negatives nor a subclass that
+// answers in Python and has no memory of its own (its null address would pass for an absent residual,
+// bias or index).
 bool plain(const Tensor& t) {
-  return t.is_cuda() && t.layout() == c10::kStrided && t.has_storage() && !t.is_neg();
+  return t.is_cuda() && t.layout() == c10::kStrided && t.has_storage() && !t.is_neg() &&
+         !t.key_set().has(c10::DispatchKey::Python);
 }
 // A gradient, of either mode, would be recorded.
 bool recorded(const Tensor& t) {

@@ -263,3 +263,19 @@ def test_weights_that_are_no_tensors_are_refused():
             fm.quantize_weights(wrong)
     with pytest.raises(ValueError, match="no weights"):
         fm.quantize_weights([])
+
+
+def test_tensors_that_only_stand_for_memory_are_refused():
+    """Fake tensors say that they are on the GPU, and have no memory anywhere."""
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    with FakeTensorMode():
+        x, w = torch.empty(2, 8, device="cuda"), torch.empty(8, device="cuda")
+        q = fm.QuantizedRows(torch.empty(2, 128, dtype=torch.int8, device="cuda"),
+                             torch.empty(2, device="cuda"), 8)
+        held = fm.CompressedRows(q.data, torch.empty(2, 1, device="cuda"), 8)
+    for call in (lambda: fm.add_rms_norm_int8(x, w), lambda: fm.quantize_rows(x),
+                 lambda: fm.compress_rows(x), lambda: fm.gelu_compress(x), lambda: q.dequantize(), lambda: fm.restore_rows(held, torch.float32),
+                 lambda: fm.gelu_compressed_backward(held, x)):
+        with pytest.raises(ValueError, match="memory of their own"):
+            call()
