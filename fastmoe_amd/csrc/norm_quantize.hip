@@ -9,8 +9,8 @@
 //   grad_x = grad_residual = grad_h + c * t - h * c^3 / D * sum(t * h)
 //   grad_w = sum over rows of grad_y * h * c
 //
-// Sums, the norm's factor and the scales are fp32; a mean of squares above fp32's range gives zeros,
-// as it does in the unfused formula.
+// Sums, the norm's factor and the scales are fp32; a row whose sum of squares passes fp32's range (finite
+// values of 1.5e17 in 16384 columns, 1.5e18 in 150) gives zeros, as it does in the unfused fp32 formula.
 #include "rows8.h"
 
 #include <algorithm>
@@ -461,7 +461,8 @@ template <typename F> void by_cols(int64_t cols, F&& f) {
   else go(integral_constant<int, 512>{}, integral_constant<int, 4>{});
 }
 // The backward holds three inputs, the weight and its gradient's part: two vectors each (four take 250
-// registers).  fp32 rows above 8192 columns take four all the same: two with 1024 threads spill.
+// registers).  Above 8192 columns none fits: with 1024 threads and two vectors 16-bit rows spill 5 registers (23
+// with an fp32 weight), fp32 rows 55, and 53 with 512 and four, which they take.
 template <typename T, typename F> void by_cols_backward(int64_t cols, F&& f) {
   using std::integral_constant;
   const int64_t v = (cols + 7) / 8;

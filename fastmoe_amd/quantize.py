@@ -240,7 +240,7 @@ def add_rms_norm(x: torch.Tensor, weight: torch.Tensor, residual: Optional[torch
     ``x`` and ``residual`` [T, D] (unit column stride), ``weight`` [D] in x's type or float32.  h is
     rounded to x's type, as the tensors' sum is, and y is computed from it in float32 and rounded
     once.  Without a residual, h is ``x`` itself.  Differentiable in all three; the gradient of the
-    weight sums the rows in a fixed order.
+    weight sums the rows in a fixed order.  A row whose sum of squares passes float32's range gives zeros.
     """
     _refuse_transforms("add_rms_norm")
     out = _call("norm", x, weight, residual, eps, True, False)
