@@ -145,12 +145,12 @@ bool is_float(const Tensor& t) {
   return t.scalar_type() == at::kFloat || t.scalar_type() == at::kBFloat16 ||
          t.scalar_type() == at::kHalf;
 }
-// A tensor whose memory holds its values: neither a view that stands for their negatives nor a subclass that
-// answers in Python and has no memory of its own (its null address would pass for an absent residual,
-// bias or index).
+// A tensor whose memory holds its values: neither a view that stands for their negatives, nor a subclass that
+// answers in Python, nor one that stands for zeros, which have no memory of their own (their null
+// address would pass for an absent residual, bias or index).
 bool plain(const Tensor& t) {
   return t.is_cuda() && t.layout() == c10::kStrided && t.has_storage() && !t.is_neg() &&
-         !t.key_set().has(c10::DispatchKey::Python);
+         !t.key_set().has(c10::DispatchKey::Python) && !t._is_zerotensor();
 }
 // A gradient, of either mode, would be recorded.
 bool recorded(const Tensor& t) {
@@ -186,9 +186,13 @@ bool good_rows8(const Tensor& q, const Tensor& s, int64_t features, int64_t per_
                                     : q.stride(0) >= q.size(1) && q.stride(0) % 16 == 0));
 }
 
-// Rows with unit column stride, as their memory stands.
-Tensor by_rows(const Tensor& t) {
-  return (t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous()).resolve_neg();
+// A gradient's rows with unit column stride, as their memory stands.
+Tensor by_rows(Tensor t) {
+  if (t._is_zerotensor()) t = at::zeros_like(t);
+  t = (t.size(1) <= 1 || t.stride(1) == 1 ? t : t.contiguous()).resolve_neg();
+  if (!plain(t))
+    throw std::runtime_error("fastmoe_amd: the norm's backward does not take a gradient without memory of its own");
+  return t;
 }
 
 constexpr const char* kNoSecond = "fastmoe_amd: the norm's gradient has no gradient of its own";

@@ -54,3 +54,39 @@ def test_subclasses_with_memory_are_taken():
     x, w = torch.randn(4, 64, device="cuda"), torch.randn(64, device="cuda")
     y, _ = fm.add_rms_norm(x.as_subclass(Named), torch.nn.Parameter(w), x)
     assert torch.equal(y.as_subclass(torch.Tensor), fm.add_rms_norm(x, w, x)[0])
+
+
+def test_zeros_without_memory_are_refused():
+    """What forward-mode and complex views make for zeros: no memory, a null address."""
+    x, w = torch.randn(4, 256, device="cuda"), torch.randn(256, device="cuda")
+    zero = torch._efficientzerotensor((4, 256), device="cuda")
+    assert zero.is_cuda and not zero.any()
+    q, weights = fm.quantize_rows(x), fm.quantize_weights(torch.randn(8, 256, device="cuda"))
+    for call in (lambda: fm.add_rms_norm(x, w, zero), lambda: fm.add_rms_norm_int8(x, w, zero),
+                 lambda: fm.quantize_rows(zero), lambda: fm.gelu_compressed_backward(fm.compress_rows(x), zero),
+                 lambda: fm.int8_linear(q, weights, bias=torch._efficientzerotensor((8,), device="cuda"))):
+        with pytest.raises((ValueError, RuntimeError)):
+            call()
+
+
+def test_gradients_of_every_kind():
+    """Zeros without memory count as zeros; wrappers and batched gradients raise."""
+    x, w, r = (torch.randn(*s, device="cuda").requires_grad_(True) for s in ((4, 32), (32,), (4, 32)))
+    g, gh = torch.randn(4, 32, device="cuda"), torch.randn(4, 32, device="cuda")
+
+    def grads(of_y, of_h, **kw):
+        y, h = fm.add_rms_norm(x, w, r)
+        return torch.autograd.grad([y, h], [x, w, r], [of_y, of_h], **kw)
+
+    zero = torch._efficientzerotensor((4, 32), device="cuda")
+    for a, b in ((g, zero), (zero, gh)):
+        plain = [torch.zeros_like(g) if t is zero else t for t in (a, b)]
+        assert all(torch.equal(u, v) for u, v in zip(grads(a, b), grads(*plain)))
+    for which in range(2):
+        y, h = fm.add_rms_norm(x, w, r)
+        (y, h)[which].register_hook(Wrapper)
+        with pytest.raises((ValueError, RuntimeError, NotImplementedError, TypeError)):
+            torch.autograd.grad([y, h], [x, w, r], [g, gh])
+    with pytest.raises(RuntimeError):
+        grads(torch.stack([g, g]), torch.stack([gh, gh]), is_grads_batched=True)
+    assert all(t.isfinite().all() for t in grads(g, gh))  # and leaves nothing behind
