@@ -176,7 +176,7 @@ __device__ __forceinline__ int64_t source_row(const LinearArgs& a, int64_t r) {
 struct RowScale {
   float before, after;
   __device__ __forceinline__ explicit RowScale(float s)
-      : before(s < 1.f ? s : 1.f), after(s < 1.f ? 1.f : s) {}  // NaN: after
+      : before(__builtin_fabsf(s) < 1.f ? s : 1.f), after(__builtin_fabsf(s) < 1.f ? 1.f : s) {}  // NaN: after
   __device__ __forceinline__ float scaled(int32_t sum, float sw, float bias) const {
     return __builtin_fmaf((float)sum * before * sw, after, bias);
   }
@@ -661,11 +661,11 @@ Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
 // Tiles of 256 columns store past the caches, which leaves those to rows and weights: 2048 rows over 32 experts
 // of [7168, 2048] 97 us instead of 109, and 113 instead of 124 with the GELU that reads the results; 16
 // experts of [2048, 2048] at 128 rows 19.6 and 20.8.  Narrower tiles write parts of lines and lose (13
-// experts of [900, 1001] at 128 rows 12.6 and 12.0).  Rows that start inside a line have parts of lines at
-// every wave's ends.  16-bit results gain all the same or lose little (N = 7167, 64 rows of 32 experts,
-// K = 2048: 100 and 111; N = 1001, 2048 rows of 8: 65.6 and 62.7).  fp32 ones of 256 x 256, each line of which
-// two of a lane's stores write, lose much (346 rows of 32 experts, K = 512: N = 1001 31 and 23, 7167 169
-// and 147), and gain as much where rows start with a line (N = 4096: 68 and 89).
+// experts of [900, 1001] at 128 rows 12.6 and 12.0).  Rows that start inside a line have parts of lines wherever a
+// wave's part of a row ends.  16-bit results gain all the same or lose little (346 rows of 32 experts, N = 2047:
+// K = 256 33.9 and 32.2, 2048 71.6 and 76.3); fp32 ones of 256 x 256, where a wave writes its columns in two parts,
+// one after the other, lose much (52.0 and 33.3, 87.8 and 77.5), and gain where rows start with a line
+// (N = 4096: K = 512 67 and 79, 2048 140 and 153).
 bool starts_with_lines(const LinearArgs& a, int64_t bytes) {
   return reinterpret_cast<uintptr_t>(a.out) % 128 == 0 && a.out_stride * bytes % 128 == 0;
 }

@@ -86,8 +86,8 @@ def compute_experts(experts: Sequence[nn.Module], recv_data: torch.Tensor,
     rows and the first product in 8 bits, a scale for every 128 columns, instead of the rows, the
     first product and GELU's output in their own type: about D + F bytes a row instead of 2 D + 4 F at 16
     bits.  The forward computes with the rows as they are (GELU within the results' rounding); the
-    gradients are those of the held values (each within 1/254 of its block's largest).  Without a backward to record nothing is held.  Rows and weights share one
-    dtype (autocast's, where it is on).
+    gradients are those of the held values (each within 1/254 of its block's largest).  Without a
+    backward to record nothing is held.  Rows and weights share one dtype (autocast's, where it is on).
     """
     if checkpoint is not None:
         if checkpoint != "int8":

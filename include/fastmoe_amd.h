@@ -499,7 +499,7 @@ FMOE_API int fmoe_gelu_compressed_backward(const void* d_q, int64_t q_stride, co
  * [E, N, Kp] with Kp = K rounded up to 128, zeros from K on, d_w_scales fp32[E, N]; d_bias [E, N] or null.
  * d_offsets: int64[E + 1] on the device, or null for one expert.  Sums are exact int32 (K <= 131071).
  * Rows at or beyond offsets[E] are written as zero; a row whose index lies outside [0, x_rows) has
- * a product of zero (of NaN for outputs whose weights' scale is).
+ * a product of zero (NaN for an output whose weights' scale is NaN).
  */
 FMOE_API int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows,
                               const float* d_x_scales, const void* d_index, int index_dtype,

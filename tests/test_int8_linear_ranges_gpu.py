@@ -75,3 +75,18 @@ def test_rows_that_start_with_a_line_of_memory_and_inside_one(tile, E, mean, N, 
     x, w = make(R, K, E, N, seed=3)
     got = fm.int8_linear(x, w, route(counts), out_dtype=dtype)
     check(got, *reference(x, w, counts), dtype)
+
+
+@pytest.mark.parametrize("tile,E,mean,N", TILES)
+def test_scales_of_either_sign(tile, E, mean, N):
+    """A scale may be negative; its size alone says which factor comes first."""
+    counts = ragged(E, mean)
+    R = sum(counts)
+    x, w = make(R, 300, E, N, seed=3)
+    g = torch.Generator(device="cuda").manual_seed(5)
+    sign = lambda *s: torch.randint(0, 2, s, generator=g, device="cuda") * 2.0 - 1
+    x = x._replace(scales=sign(R) * 1e36)
+    w = w._replace(scales=sign(E, N) * 1e-36)
+    want, _ = reference(x, w, counts)
+    got = fm.int8_linear(x, w, route(counts), out_dtype=torch.float32).double()
+    assert ((got - want).abs() <= 6 * U * want.abs()).all()
