@@ -38,6 +38,7 @@ from .quantize import (
     quantize_weights,
     restore_rows,
 )
+from .routing import RoutedTokens, Routing, route_tokens
 
 __all__ = [
     "CompressedRows",
@@ -51,6 +52,8 @@ __all__ = [
     "NormedMoEFeedForward",
     "PermutedTokens",
     "QuantizedRows",
+    "RoutedTokens",
+    "Routing",
     "add_rms_norm",
     "add_rms_norm_int8",
     "compress_rows",
@@ -63,6 +66,7 @@ __all__ = [
     "quantize_rows",
     "quantize_weights",
     "restore_rows",
+    "route_tokens",
     "unpermute",
     "build_plan",
     "grouped_weighted_scatter_add",

@@ -20,6 +20,8 @@ F32, BF16, F16, I64, I32 = 0, 1, 2, 3, 4
 MODE_DET, MODE_ATOMIC, MODE_ATOMIC_PACKED, MODE_DET_STEP = 0, 1, 2, 3
 STREAM_OUT_BYTES = 96 << 20  # FMOE_STREAM_OUT_BYTES
 ACT_NONE, ACT_GELU = 0, 1  # enum fmoe_activation
+SCORE_SOFTMAX, SCORE_SIGMOID = 0, 1  # enum fmoe_score
+GROUP_MAX, GROUP_TOP2 = 0, 1  # enum fmoe_group_score
 OK, EINVAL, EHIP, ERANGE = 0, -1, -2, -3
 
 _c_i64 = ctypes.c_int64
@@ -139,6 +141,16 @@ SIGNATURES: dict[str, tuple] = {
         _c_int,
         [_c_vp, _c_i64, _c_i64, _c_vp, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_i64,
          _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_vp],
+    ),
+    "fmoe_route": (
+        _c_int,
+        [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_i64, _c_int, _c_i64, _c_i64, _c_int, _c_int,
+         _c_f32, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_route_backward": (
+        _c_int,
+        [_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
+         _c_int, _c_f32, _c_vp, _c_vp],
     ),
 }
 

@@ -22,12 +22,13 @@ LIB_PATH = PKG / LIB_NAME
 
 # The operator layer's host helper modules (CPython extensions built against the installed torch, not
 # part of the C ABI): fastmoe_amd._host reads tensor properties in C++, fastmoe_amd._rows allocates
-# for and calls the entry points of the 8-bit operators and the norm.
-HOST_EXT_SOURCES = {"_host": "host_ext.cpp", "_rows": "rows_ext.cpp"}
+# for and calls the entry points of the 8-bit operators and the norm, fastmoe_amd._block those of the
+# router, the 4-bit products and the norms around a block.
+HOST_EXT_SOURCES = {"_host": "host_ext.cpp", "_rows": "rows_ext.cpp", "_block": "block_ext.cpp"}
 
 HIP_SOURCES = ["metadata.hip", "plan.hip", "plan_bucket.hip", "plan_radix.hip", "combine_fwd.hip",
                "combine_bwd.hip", "permute.hip", "noalloc.hip", "norm_quantize.hip", "hold.hip",
-               "int8_linear.hip"]
+               "int8_linear.hip", "route.hip"]
 HOST_SOURCES = ["abi.cpp"]
 
 ARCH = "gfx950"
@@ -112,7 +113,7 @@ def _host_ext_command(cxx: str, name: str, source: str):
 def build(verbose: bool = True, jobs: int | None = None, defines: list[str] | None = None,
           out: Path | None = None, build_dir: Path | None = None) -> Path:
     """Compile every translation unit and link ``libfastmoe_amd.so``; returns its path.  The
-    in-tree build also compiles the host helper modules ``fastmoe_amd._host`` and ``_rows``.
+    in-tree build also compiles the host helper modules ``fastmoe_amd._host``, ``_rows`` and ``_block``.
 
     ``defines`` (e.g. ``["FMOE_BWD_WAVES=8"]``) set the kernels' compile-time knobs; ``out`` and
     ``build_dir`` redirect the result (tuning builds), by default the in-tree library.

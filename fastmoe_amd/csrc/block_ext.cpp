@@ -1,0 +1,190 @@
+// fastmoe_amd._block: the host side of the router (not part of the C ABI): as in fastmoe_amd._rows, a call allocates its results and calls the C entry point in one go, and
+// a backward runs in the engine's thread without the interpreter.
+//
+// Each function but bind checks its arguments and returns NotImplemented where something is not as it
+// takes it, and under tracing; the caller then goes through the checks one by one and says what is wrong.
+//
+//   bind({name: address}) once, with the library's entry points
+//   route(logits, bias | None, top_k, score, groups, top_groups, group score, renormalize, scale, dtype code of
+//         the weights, recorded) -> (weights, ids): records its backward if `recorded`
+constexpr const char* kModuleName = "fastmoe_amd._block";
+#include "host_tensors.h"
+
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+
+namespace {
+
+#define FMOE_ENTRIES(X) \
+  X(fmoe_last_error)    \
+  X(fmoe_route)         \
+  X(fmoe_route_backward)
+
+struct Api {
+#define FMOE_DECLARE(name) decltype(&::name) name = nullptr;
+  FMOE_ENTRIES(FMOE_DECLARE)
+#undef FMOE_DECLARE
+} api;
+
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+void refuse_capture(const char* what) {
+  if (capturing())
+    throw std::runtime_error(
+        std::string("fastmoe_amd: ") + what +
+        " under HIP graph capture is not supported (a captured autograd step once crashed the host in "
+        "CUDAGraph.capture_end).  Run the autograd step eagerly.");
+}
+
+// A backward under create_graph: gradients that would need one of their own are refused, and results that
+// depend on `inputs` say so to whoever differentiates them.
+void refuse_second(const variable_list& grads, const char* message) {
+  if (!at::GradMode::is_enabled()) return;
+  for (const Tensor& g : grads)
+    if (g.defined() && g.requires_grad()) throw std::runtime_error(message);
+}
+void mark_second(std::initializer_list<Tensor*> results, const variable_list& inputs, const char* message) {
+  if (!at::GradMode::is_enabled()) return;
+  bool any = false;
+  for (const Tensor& t : inputs) any |= t.defined() && t.requires_grad();
+  if (!any) return;
+  for (Tensor* g : results)
+    if (g->defined())
+      torch::autograd::set_history(
+          *g, std::shared_ptr<torch::autograd::Node>(
+                  new torch::autograd::Error(message, torch::autograd::collect_next_edges(inputs)),
+                  torch::autograd::deleteNode));
+}
+
+// ---- the router -----------------------------------------------------------------------------------
+
+struct Routing {
+  Tensor bias;
+  int64_t k, groups, top_groups;
+  int score, group_score, renormalize, w_dtype;
+  float scale;
+};
+
+struct Routed {
+  Tensor weights, ids, share, rest, norm;
+};
+
+Routed run_route(const Tensor& logits, const Routing& o, bool keep) {
+  Place place(logits);
+  const int64_t T = logits.size(0), E = logits.size(1);
+  Routed r;
+  r.weights = empty({T, o.k}, logits, type_of(o.w_dtype));
+  r.ids = empty({T, o.k}, logits, at::kLong);
+  if (keep) {
+    r.share = empty({T, o.k}, logits, at::kFloat);
+    if (o.score == FMOE_SCORE_SIGMOID) r.rest = empty({T, o.k}, logits, at::kFloat);
+    else if (!o.renormalize) r.norm = empty({T, 2}, logits, at::kFloat);
+  }
+  check(api.fmoe_route(data(logits), pitch(logits), T, E, code(logits.scalar_type()),
+                       static_cast<const float*>(data(o.bias)), o.k, o.score, o.groups, o.top_groups,
+                       o.group_score, o.renormalize, o.scale, data(r.weights), o.w_dtype,
+                       static_cast<int64_t*>(data(r.ids)), static_cast<float*>(data(r.share)),
+                       static_cast<float*>(data(r.rest)), static_cast<float*>(data(r.norm)), place.stream),
+        "fmoe_route");
+  return r;
+}
+
+constexpr const char* kNoSecondRoute = "fastmoe_amd: the router's gradient has no gradient of its own";
+
+class Route : public torch::autograd::Function<Route> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor logits, Routing o) {
+    Routed r = run_route(logits, o, true);
+    // the logits are kept where a gradient reads them, and for what depends on them under create_graph
+    ctx->save_for_backward({logits, r.ids, r.share, r.rest, r.norm});
+    ctx->saved_data["renormalize"] = (int64_t)o.renormalize;
+    ctx->saved_data["scale"] = (double)o.scale;
+    ctx->mark_non_differentiable({r.ids});
+    ctx->set_materialize_grads(false);
+    return {r.weights, r.ids};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &logits = saved[0], &ids = saved[1], &share = saved[2], &rest = saved[3], &norm = saved[4];
+    if (!grads[0].defined()) return {Tensor(), Tensor()};
+    refuse_second(grads, kNoSecondRoute);
+    Place place(share);
+    refuse_capture("the router's backward");
+    const Tensor g = by_rows(grads[0]).contiguous();
+    const int64_t T = logits.size(0), E = logits.size(1);
+    Tensor out = empty({T, E}, logits);
+    check(api.fmoe_route_backward(data(g), code(g.scalar_type()), static_cast<const int64_t*>(data(ids)),
+                                  static_cast<const float*>(data(share)), static_cast<const float*>(data(rest)),
+                                  static_cast<const float*>(data(norm)), data(logits), pitch(logits), T, E,
+                                  ids.size(1), code(logits.scalar_type()),
+                                  (int)ctx->saved_data["renormalize"].toInt(),
+                                  (float)ctx->saved_data["scale"].toDouble(), data(out), place.stream),
+          "fmoe_route_backward");
+    mark_second({&out}, {logits}, kNoSecondRoute);
+    return {out, Tensor()};
+  }
+};
+
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded<11>(n, [&] {
+    if (!tensors({a[0], a[1]})) return not_taken();
+    const Tensor logits = tensor(a[0]);
+    Routing o;
+    o.bias = tensor(a[1]);
+    o.k = integer(a[2]);
+    o.score = (int)integer(a[3]);
+    o.groups = integer(a[4]);
+    o.top_groups = integer(a[5]);
+    o.group_score = (int)integer(a[6]);
+    o.renormalize = a[7] == Py_True;
+    o.scale = (float)real(a[8]);
+    o.w_dtype = (int)integer(a[9]);
+    const bool records = a[10] == Py_True;
+    if (!good_matrix(logits) || (recorded(logits) && !records) || o.k < 1 || o.k > logits.size(1) ||
+        (o.bias.defined() &&
+         (!plain(o.bias) || o.bias.device() != logits.device() || o.bias.scalar_type() != at::kFloat ||
+          o.bias.dim() != 1 || o.bias.size(0) != logits.size(1) || !o.bias.is_contiguous() || recorded(o.bias))))
+      return not_taken();
+    if (records) {
+      const auto r = Route::apply(logits, o);
+      return tuple(r[0], r[1]);
+    }
+    const Routed r = run_route(logits, o, false);
+    return tuple(r.weights, r.ids);
+  });
+}
+
+PyObject* bind(PyObject*, PyObject* dict) {
+  Api found;
+#define FMOE_FIND(name)                                                                         \
+  {                                                                                             \
+    PyObject* v = PyDict_Check(dict) ? PyDict_GetItemString(dict, #name) : nullptr;             \
+    void* p = v ? PyLong_AsVoidPtr(v) : nullptr;                                                \
+    if (!p) {                                                                                   \
+      if (!PyErr_Occurred()) PyErr_SetString(PyExc_ValueError, "fastmoe_amd._block: no " #name); \
+      return nullptr;                                                                           \
+    }                                                                                           \
+    std::memcpy(&found.name, &p, sizeof(p));                                                    \
+  }
+  FMOE_ENTRIES(FMOE_FIND)
+#undef FMOE_FIND
+  api = found;
+  last_error = found.fmoe_last_error;
+  Py_RETURN_NONE;
+}
+
+PyMethodDef kMethods[] = {
+    {"bind", bind, METH_O, "bind({name: address}): the library's entry points"},
+    {"route", FMOE_FAST(route),
+     "route(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale, dtype, recorded)"},
+    {nullptr, nullptr, 0, nullptr}};
+
+PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_block",
+                       "Host side of fastmoe_amd's router", -1, kMethods};
+
+}  // namespace
+
+PyMODINIT_FUNC PyInit__block(void) { return PyModule_Create(&kModule); }

@@ -89,6 +89,16 @@ enum fmoe_activation {
   FMOE_ACT_GELU = 1 /* x * Phi(x), the exact form (not the tanh approximation) */
 };
 
+/* What a router's logits are turned into, and what a group of experts is ranked by. */
+enum fmoe_score {
+  FMOE_SCORE_SOFTMAX = 0, /* over all experts */
+  FMOE_SCORE_SIGMOID = 1
+};
+enum fmoe_group_score {
+  FMOE_GROUP_MAX = 0, /* its highest choice */
+  FMOE_GROUP_TOP2 = 1 /* the sum of its two highest */
+};
+
 enum fmoe_status {
   FMOE_OK = 0,
   FMOE_EINVAL = -1,   /* bad argument (null pointer, size, dtype, alignment, layout) */
@@ -510,6 +520,37 @@ FMOE_API int fmoe_int8_linear(const void* d_x, int64_t x_row_stride, int64_t x_r
 
 /* The tile that fmoe_int8_linear chooses by size, as 1000 * rows + columns (introspection). */
 FMOE_API int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_t N, int64_t K);
+
+/*
+ * Routing of tokens to experts: for each row of logits[T, E] (row_stride elements apart, of `dtype`),
+ *     s = softmax(l) over all experts, or sigmoid(l)             (score: fmoe_score)
+ *     c = s + bias, both in fp32 (s rounded from 64 bits), with a bias or groups ranked by a sum; else l
+ *     the top_groups of `groups` equal groups of neighbouring experts, by their highest c or the sum of
+ *     their two highest in fp32                                  (group_score: fmoe_group_score)
+ *     ids = the top_k highest c of those groups, highest first, the lowest index first among equals
+ *     weights = scale * s[ids], divided by sum(s[ids]) with renormalize
+ * d_bias: fp32[E] or null.  d_weights [T, top_k] in weight_dtype, d_ids int64[T, top_k].  A masked expert
+ * (-inf) has no weight; where every expert that counts is masked, the ids are still different experts and the
+ * weights zero.  A NaN ranks highest.  For the backward, null where none follows: d_share fp32[T, top_k], the
+ * weights before the scale; d_rest fp32[T, top_k], 1 - s (a sigmoid); d_norm fp32[T, 2], maximum and 1 / sum
+ * of e^(l - maximum) (a softmax without renormalize; written for that alone).
+ * top_k <= 64 and at most top_groups * E / groups, E <= 4096, with groups E <= 1024 and groups <= 64.
+ */
+FMOE_API int fmoe_route(const void* d_logits, int64_t row_stride, int64_t num_tokens, int64_t num_experts,
+                        int dtype, const float* d_bias, int64_t top_k, int score, int64_t groups,
+                        int64_t top_groups, int group_score, int renormalize, float scale, void* d_weights,
+                        int weight_dtype, int64_t* d_ids, float* d_share, float* d_rest, float* d_norm,
+                        void* stream);
+
+/*
+ * Its backward: d_grad_logits[T, E] (packed, in `dtype`) from d_grad[T, top_k], the weights' gradient, and
+ * what the forward kept: d_rest for a sigmoid, d_norm and the logits for a softmax without renormalize, null
+ * otherwise.
+ */
+FMOE_API int fmoe_route_backward(const void* d_grad, int grad_dtype, const int64_t* d_ids, const float* d_share,
+                                 const float* d_rest, const float* d_norm, const void* d_logits,
+                                 int64_t row_stride, int64_t num_tokens, int64_t num_experts, int64_t top_k,
+                                 int dtype, int renormalize, float scale, void* d_grad_logits, void* stream);
 
 #ifdef __cplusplus
 }
