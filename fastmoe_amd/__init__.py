@@ -38,6 +38,7 @@ from .quantize import (
     quantize_weights,
     restore_rows,
 )
+from .norms import sandwich_norm
 from .routing import RoutedTokens, Routing, route_tokens
 
 __all__ = [
@@ -67,6 +68,7 @@ __all__ = [
     "quantize_weights",
     "restore_rows",
     "route_tokens",
+    "sandwich_norm",
     "unpermute",
     "build_plan",
     "grouped_weighted_scatter_add",

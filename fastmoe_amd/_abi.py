@@ -152,6 +152,17 @@ SIGNATURES: dict[str, tuple] = {
         [_c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_i64, _c_i64, _c_i64, _c_int,
          _c_int, _c_f32, _c_vp, _c_vp],
     ),
+    "fmoe_sandwich_norm": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_i64, _c_i64, _c_i64,
+         _c_int, _c_f32, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_sandwich_norm_backward_workspace_bytes": (_c_i64, [_c_i64, _c_i64, _c_i64]),
+    "fmoe_sandwich_norm_backward": (
+        _c_int,
+        [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_i64,
+         _c_vp, _c_i64, _c_i64, _c_int, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp],
+    ),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -1,5 +1,6 @@
-// fastmoe_amd._block: the host side of the router (not part of the C ABI): as in fastmoe_amd._rows, a call allocates its results and calls the C entry point in one go, and
-// a backward runs in the engine's thread without the interpreter.
+// fastmoe_amd._block: the host side of the router and the norms around a block (not part of the C ABI): as in
+// fastmoe_amd._rows, a call allocates its results and calls the C entry point in one go, and a backward runs
+// in the engine's thread without the interpreter.
 //
 // Each function but bind checks its arguments and returns NotImplemented where something is not as it
 // takes it, and under tracing; the caller then goes through the checks one by one and says what is wrong.
@@ -7,6 +8,7 @@
 //   bind({name: address}) once, with the library's entry points
 //   route(logits, bias | None, top_k, score, groups, top_groups, group score, renormalize, scale, dtype code of
 //         the weights, recorded) -> (weights, ids): records its backward if `recorded`
+//   sandwich(x, post, residual, pre | None, gate | None, scale, eps, recorded) -> (y | None, stream)
 constexpr const char* kModuleName = "fastmoe_amd._block";
 #include "host_tensors.h"
 
@@ -16,10 +18,13 @@ constexpr const char* kModuleName = "fastmoe_amd._block";
 
 namespace {
 
-#define FMOE_ENTRIES(X) \
-  X(fmoe_last_error)    \
-  X(fmoe_route)         \
-  X(fmoe_route_backward)
+#define FMOE_ENTRIES(X)                          \
+  X(fmoe_last_error)                             \
+  X(fmoe_route)                                  \
+  X(fmoe_route_backward)                         \
+  X(fmoe_sandwich_norm)                          \
+  X(fmoe_sandwich_norm_backward)                 \
+  X(fmoe_sandwich_norm_backward_workspace_bytes)
 
 struct Api {
 #define FMOE_DECLARE(name) decltype(&::name) name = nullptr;
@@ -157,6 +162,123 @@ PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- the norms around a block -------------------------------------------------------------------------
+
+struct Sandwich {
+  Tensor x, post, residual, pre, gate;  // pre, gate: or undefined
+  double scale, eps;
+  int64_t gate_rows() const { return !gate.defined() ? 0 : gate.dim() == 1 ? 1 : gate.size(0); }
+};
+
+bool good_param(const Tensor& t, const Tensor& x, bool matrix) {
+  return plain(t) && t.is_contiguous() && t.device() == x.device() &&
+         (t.dim() == 1 || (matrix && t.dim() == 2)) && t.size(-1) == x.size(1) &&
+         (t.scalar_type() == x.scalar_type() || t.scalar_type() == at::kFloat);
+}
+
+bool good_sandwich(const Sandwich& s) {
+  return good_matrix(s.x) && good_matrix(s.residual) && s.residual.sizes() == s.x.sizes() &&
+         s.residual.scalar_type() == s.x.scalar_type() && s.residual.device() == s.x.device() &&
+         s.post.defined() && good_param(s.post, s.x, false) &&
+         (!s.pre.defined() || (good_param(s.pre, s.x, false) && s.pre.scalar_type() == s.post.scalar_type())) &&
+         (!s.gate.defined() ||
+          (good_param(s.gate, s.x, true) && s.gate_rows() >= 1 && s.x.size(0) % s.gate_rows() == 0)) &&
+         std::isfinite(s.scale) && s.eps >= 0 && s.eps < HUGE_VAL;
+}
+
+struct Sandwiched {
+  Tensor y, h, rstd;
+};
+
+Sandwiched run_sandwich(const Sandwich& s, bool keep) {
+  Place place(s.x);
+  const int64_t T = s.x.size(0), D = s.x.size(1);
+  Sandwiched r;
+  r.h = empty({T, D}, s.x);
+  if (s.pre.defined()) r.y = empty({T, D}, s.x);
+  if (keep) r.rstd = empty({T, 2}, s.x, at::kFloat);
+  if (T)
+    check(api.fmoe_sandwich_norm(data(s.x), pitch(s.x), data(s.residual), pitch(s.residual), data(s.post),
+                                 data(s.pre), code(s.post.scalar_type()), data(s.gate),
+                                 s.gate.defined() ? code(s.gate.scalar_type()) : FMOE_F32, s.gate_rows(), T, D,
+                                 code(s.x.scalar_type()), (float)s.scale, (float)s.eps, data(r.h), data(r.y),
+                                 static_cast<float*>(data(r.rstd)), place.stream),
+          "fmoe_sandwich_norm");
+  return r;
+}
+
+constexpr const char* kNoSecondSandwich =
+    "fastmoe_amd: the gradient of the norms around a block has no gradient of its own";
+
+class SandwichNorm : public torch::autograd::Function<SandwichNorm> {
+ public:
+  static variable_list forward(AutogradContext* ctx, Tensor x, Tensor post, Tensor residual,
+                               std::optional<Tensor> pre, std::optional<Tensor> gate, double scale, double eps) {
+    const Sandwich s{x, post, residual, pre.value_or(Tensor()), gate.value_or(Tensor()), scale, eps};
+    const Sandwiched r = run_sandwich(s, true);
+    ctx->save_for_backward({x, r.h, post, s.pre, s.gate, r.rstd});
+    ctx->saved_data["scale"] = scale;
+    ctx->set_materialize_grads(false);
+    if (!s.pre.defined()) return {r.h};
+    return {r.h, r.y};
+  }
+
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &h = saved[1], &post = saved[2], &pre = saved[3], &gate = saved[4],
+                 &rstd = saved[5];
+    Tensor gh = grads[0], gy = grads.size() > 1 ? grads[1] : Tensor();
+    variable_list out(7);
+    if (!gh.defined() && !gy.defined()) return out;
+    refuse_second(grads, kNoSecondSandwich);
+    Place place(h);
+    refuse_capture("the backward of the norms around a block");
+    if (gh.defined()) gh = by_rows(gh);
+    if (gy.defined()) gy = by_rows(gy);
+    // inputs that were not given are not counted
+    const bool has_pre = pre.defined(), has_gate = gate.defined();
+    const bool need_pre = has_pre && ctx->needs_input_grad(3),
+               need_gate = has_gate && ctx->needs_input_grad(has_pre ? 4 : 3);
+    const int64_t T = h.size(0), D = h.size(1),
+                  runs = !has_gate ? 0 : gate.dim() == 1 ? 1 : gate.size(0);
+    if (ctx->needs_input_grad(0)) out[0] = empty({T, D}, h);
+    if (ctx->needs_input_grad(1)) out[1] = empty({D}, post);
+    if (ctx->needs_input_grad(2)) out[2] = empty({T, D}, h);
+    if (need_pre) out[3] = gy.defined() ? empty({D}, pre) : at::zeros_like(pre);
+    if (need_gate) out[4] = T ? empty(gate.sizes(), gate) : at::zeros_like(gate);
+    const int64_t bytes = api.fmoe_sandwich_norm_backward_workspace_bytes(T, D, runs);
+    const Tensor ws = empty({bytes}, h, at::kByte);
+    check(api.fmoe_sandwich_norm_backward(
+              data(gy), gy.defined() ? pitch(gy) : 0, data(gh), gh.defined() ? pitch(gh) : 0, data(x), pitch(x),
+              data(h), data(post), data(pre), code(post.scalar_type()), data(gate),
+              has_gate ? code(gate.scalar_type()) : FMOE_F32, runs, static_cast<const float*>(data(rstd)), T, D,
+              code(h.scalar_type()), (float)ctx->saved_data["scale"].toDouble(), data(out[0]), data(out[2]),
+              data(out[1]), gy.defined() ? data(out[3]) : nullptr, T ? data(out[4]) : nullptr, data(ws), bytes,
+              place.stream),
+          "fmoe_sandwich_norm_backward");
+    mark_second({&out[0], &out[1], &out[2], &out[3], &out[4]}, {x, post, h, pre, gate}, kNoSecondSandwich);
+    return out;
+  }
+};
+
+PyObject* sandwich(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded<8>(n, [&] {
+    if (!tensors({a[0], a[1], a[2], a[3], a[4]})) return not_taken();
+    const Sandwich s{tensor(a[0]), tensor(a[1]), tensor(a[2]), tensor(a[3]), tensor(a[4]), real(a[5]), real(a[6])};
+    const bool records = a[7] == Py_True;
+    if (!good_sandwich(s)) return not_taken();
+    if (records) {
+      auto maybe = [](const Tensor& t) { return t.defined() ? std::make_optional(t) : std::nullopt; };
+      const auto r = SandwichNorm::apply(s.x, s.post, s.residual, maybe(s.pre), maybe(s.gate), s.scale, s.eps);
+      return tuple(r.size() > 1 ? r[1] : Tensor(), r[0]);
+    }
+    for (const Tensor* t : {&s.x, &s.post, &s.residual, &s.pre, &s.gate})
+      if (recorded(*t)) return not_taken();
+    const Sandwiched r = run_sandwich(s, false);
+    return tuple(r.y, r.h);
+  });
+}
+
 PyObject* bind(PyObject*, PyObject* dict) {
   Api found;
 #define FMOE_FIND(name)                                                                         \
@@ -180,10 +302,11 @@ PyMethodDef kMethods[] = {
     {"bind", bind, METH_O, "bind({name: address}): the library's entry points"},
     {"route", FMOE_FAST(route),
      "route(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale, dtype, recorded)"},
+    {"sandwich", FMOE_FAST(sandwich), "sandwich(x, post, residual, pre, gate, scale, eps, recorded)"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_block",
-                       "Host side of fastmoe_amd's router", -1, kMethods};
+                       "Host side of fastmoe_amd's router and norms around a block", -1, kMethods};
 
 }  // namespace
 

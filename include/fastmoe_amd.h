@@ -552,6 +552,39 @@ FMOE_API int fmoe_route_backward(const void* d_grad, int grad_dtype, const int64
                                  int64_t row_stride, int64_t num_tokens, int64_t num_experts, int64_t top_k,
                                  int dtype, int renormalize, float scale, void* d_grad_logits, void* stream);
 
+/*
+ * The norms between two blocks, of `rows` rows of `dtype`:
+ *     a = x * post / sqrt(mean(x^2) + eps)               (x: the block's output)
+ *     h = residual + scale * gate * a, rounded to `dtype`
+ *     y = h * pre / sqrt(mean(h^2) + eps)                (d_pre and d_y null: not wanted)
+ * d_post and d_pre [cols] in weight_dtype (`dtype` or FMOE_F32); d_gate [gate_rows, cols] in gate_dtype (`dtype` or
+ * FMOE_F32), each row for rows / gate_rows neighbouring rows, or null with gate_rows 0.  h and y are packed.  d_rstd:
+ * fp32[rows, 2], the factors of the two norms for the backward, or null.  Strides in elements.  d_h may be d_x's or
+ * d_residual's own memory if that is packed.
+ */
+FMOE_API int fmoe_sandwich_norm(const void* d_x, int64_t x_row_stride, const void* d_residual,
+                                int64_t residual_row_stride, const void* d_post, const void* d_pre,
+                                int weight_dtype, const void* d_gate, int gate_dtype, int64_t gate_rows,
+                                int64_t rows, int64_t cols, int dtype, float scale, float eps, void* d_h,
+                                void* d_y, float* d_rstd, void* stream);
+
+/*
+ * Its backward from the gradients of y and h (one of them may be null): d_grad_x and d_grad_residual (packed),
+ * d_grad_post and d_grad_pre in weight_dtype, d_grad_gate in gate_dtype (rows > 0); each null where not wanted.
+ * d_h: the forward's, packed.  Where a parameter's gradient is wanted or the rows are long, d_workspace holds at least
+ * fmoe_sandwich_norm_backward_workspace_bytes(rows, cols, gate_rows) bytes at a multiple of 16.  Sums run in
+ * a fixed order.
+ */
+FMOE_API int64_t fmoe_sandwich_norm_backward_workspace_bytes(int64_t rows, int64_t cols, int64_t gate_rows);
+FMOE_API int fmoe_sandwich_norm_backward(const void* d_grad_y, int64_t gy_row_stride, const void* d_grad_h,
+                                         int64_t gh_row_stride, const void* d_x, int64_t x_row_stride,
+                                         const void* d_h, const void* d_post, const void* d_pre, int weight_dtype,
+                                         const void* d_gate, int gate_dtype, int64_t gate_rows,
+                                         const float* d_rstd, int64_t rows, int64_t cols, int dtype, float scale,
+                                         void* d_grad_x, void* d_grad_residual, void* d_grad_post,
+                                         void* d_grad_pre, void* d_grad_gate, void* d_workspace,
+                                         int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
