@@ -5,6 +5,7 @@ The operator API mirrors ``fastmoe.kernels.ops``; the work runs in hand-written 
 """
 from .consts import MoEImplementation
 from .dispatch import PermutedTokens, permute_tokens
+from .fp4 import Fp4Weights, fp4_linear, quantize_weights_fp4
 from .moe import (
     Int8MoEFeedForward,
     MoEFeedForward,
@@ -43,6 +44,7 @@ from .routing import RoutedTokens, Routing, route_tokens
 
 __all__ = [
     "CompressedRows",
+    "Fp4Weights",
     "GroupedMetadata",
     "GroupedWeightedScatterAdd",
     "Int8MoEFeedForward",
@@ -59,6 +61,7 @@ __all__ = [
     "add_rms_norm_int8",
     "compress_rows",
     "compute_experts",
+    "fp4_linear",
     "gate_and_sort",
     "gelu_compress",
     "gelu_compressed_backward",
@@ -66,6 +69,7 @@ __all__ = [
     "permute_tokens",
     "quantize_rows",
     "quantize_weights",
+    "quantize_weights_fp4",
     "restore_rows",
     "route_tokens",
     "sandwich_norm",

@@ -163,6 +163,15 @@ SIGNATURES: dict[str, tuple] = {
         [_c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_i64, _c_vp, _c_vp, _c_vp, _c_int, _c_vp, _c_int, _c_i64,
          _c_vp, _c_i64, _c_i64, _c_int, _c_f32, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_vp, _c_i64, _c_vp],
     ),
+    "fmoe_quantize_fp4": (
+        _c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp],
+    ),
+    "fmoe_restore_fp4": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_vp]),
+    "fmoe_fp4_linear": (
+        _c_int,
+        [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64,
+         _c_i64, _c_i64, _c_i64, _c_vp, _c_i64, _c_int, _c_vp],
+    ),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -28,7 +28,8 @@ HOST_EXT_SOURCES = {"_host": "host_ext.cpp", "_rows": "rows_ext.cpp", "_block": 
 
 HIP_SOURCES = ["metadata.hip", "plan.hip", "plan_bucket.hip", "plan_radix.hip", "combine_fwd.hip",
                "combine_bwd.hip", "permute.hip", "noalloc.hip", "norm_quantize.hip", "hold.hip",
-               "int8_linear.hip", "route.hip", "sandwich.hip"]
+               "int8_linear.hip", "route.hip", "sandwich.hip",
+               "fp4_linear.hip"]
 HOST_SOURCES = ["abi.cpp"]
 
 ARCH = "gfx950"

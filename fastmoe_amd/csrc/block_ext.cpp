@@ -1,6 +1,6 @@
-// fastmoe_amd._block: the host side of the router and the norms around a block (not part of the C ABI): as in
-// fastmoe_amd._rows, a call allocates its results and calls the C entry point in one go, and a backward runs
-// in the engine's thread without the interpreter.
+// fastmoe_amd._block: the host side of the router, the norms around a block and the 4-bit weights (not part of the C
+// ABI): as in fastmoe_amd._rows, a call allocates its results and calls the C entry point in one go, and a backward
+// runs in the engine's thread without the interpreter.
 //
 // Each function but bind checks its arguments and returns NotImplemented where something is not as it
 // takes it, and under tracing; the caller then goes through the checks one by one and says what is wrong.
@@ -9,8 +9,14 @@
 //   route(logits, bias | None, top_k, score, groups, top_groups, group score, renormalize, scale, dtype code of
 //         the weights, recorded) -> (weights, ids): records its backward if `recorded`
 //   sandwich(x, post, residual, pre | None, gate | None, scale, eps, recorded) -> (y | None, stream)
+//   quantize_fp4(x) -> (data, scales)
+//   restore_fp4(data, scales, features, dtype code) -> values
+//   fp4_linear(x, weights' data, scales, features, offsets | None, rows | None, bias | None, activation,
+//              dtype code) -> out
 constexpr const char* kModuleName = "fastmoe_amd._block";
 #include "host_tensors.h"
+
+#include <vector>
 
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -24,7 +30,10 @@ namespace {
   X(fmoe_route_backward)                         \
   X(fmoe_sandwich_norm)                          \
   X(fmoe_sandwich_norm_backward)                 \
-  X(fmoe_sandwich_norm_backward_workspace_bytes)
+  X(fmoe_sandwich_norm_backward_workspace_bytes) \
+  X(fmoe_quantize_fp4)                           \
+  X(fmoe_restore_fp4)                            \
+  X(fmoe_fp4_linear)
 
 struct Api {
 #define FMOE_DECLARE(name) decltype(&::name) name = nullptr;
@@ -279,6 +288,91 @@ PyObject* sandwich(PyObject*, PyObject* const* a, Py_ssize_t n) {
   });
 }
 
+// ---- weights in 4 bits --------------------------------------------------------------------------------
+
+int64_t whole_pieces(int64_t n) { return (n + 127) / 128 * 128; }
+
+// [..., N, bytes of codes] and [..., N, bytes of scales] of `features` columns.
+bool good_fp4(const Tensor& q, const Tensor& s, int64_t features) {
+  return q.defined() && s.defined() && plain(q) && plain(s) && q.scalar_type() == at::kByte &&
+         s.scalar_type() == at::kByte && s.device() == q.device() && q.is_contiguous() && s.is_contiguous() &&
+         q.dim() >= 2 && q.dim() <= 3 && s.dim() == q.dim() && q.sizes().slice(0, q.dim() - 1) ==
+         s.sizes().slice(0, q.dim() - 1) && features >= 1 && features <= (int64_t(1) << 40) &&
+         q.size(-1) == whole_pieces(features) / 2 && s.size(-1) == whole_pieces(features) / 32 &&
+         (q.numel() == 0 || (reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0 &&
+                             reinterpret_cast<uintptr_t>(s.data_ptr()) % 4 == 0));
+}
+
+PyObject* quantize_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded<1>(n, [&] {
+    if (!tensors({a[0]})) return not_taken();
+    const Tensor x = tensor(a[0]);
+    if (!good_matrix(x) || recorded(x)) return not_taken();
+    const int64_t R = x.size(0), pad = whole_pieces(x.size(1));
+    Place place(x);
+    const Tensor q = empty({R, pad / 2}, x, at::kByte), s = empty({R, pad / 32}, x, at::kByte);
+    if (R)
+      check(api.fmoe_quantize_fp4(data(x), pitch(x), R, x.size(1), code(x.scalar_type()), data(q), data(s),
+                                  place.stream),
+            "fmoe_quantize_fp4");
+    return tuple(q, s);
+  });
+}
+
+PyObject* restore_fp4(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded<4>(n, [&] {
+    if (!tensors({a[0], a[1]})) return not_taken();
+    const Tensor q = tensor(a[0]), s = tensor(a[1]);
+    const int64_t K = integer(a[2]);
+    const int dtype = (int)integer(a[3]);
+    if (!good_fp4(q, s, K)) return not_taken();
+    Place place(q);
+    std::vector<int64_t> sizes(q.sizes().begin(), q.sizes().end());
+    sizes.back() = K;
+    const Tensor out = empty(sizes, q, type_of(dtype));
+    if (q.numel())
+      check(api.fmoe_restore_fp4(data(q), data(s), q.numel() / q.size(-1), K, data(out), dtype, place.stream),
+            "fmoe_restore_fp4");
+    return wrap(out);
+  });
+}
+
+PyObject* fp4_linear(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  return guarded<9>(n, [&] {
+    if (!tensors({a[0], a[1], a[2], a[4], a[5], a[6]})) return not_taken();
+    const Tensor x = tensor(a[0]), w = tensor(a[1]), s = tensor(a[2]), off = tensor(a[4]), rows = tensor(a[5]),
+                 bias = tensor(a[6]);
+    const int64_t K = integer(a[3]);
+    if (!good_matrix(x) || x.scalar_type() == at::kFloat || recorded(x) || x.size(1) != K || !good_fp4(w, s, K) ||
+        w.device() != x.device())
+      return not_taken();
+    const int64_t E = w.dim() == 3 ? w.size(0) : 1, N = w.size(-2);
+    auto here = [&](const Tensor& t) { return plain(t) && t.device() == x.device() && t.is_contiguous(); };
+    if (E < 1 || N < 1 ||
+        (off.defined() ? !here(off) || off.scalar_type() != at::kLong || off.dim() != 1 || off.size(0) != E + 1
+                       : E != 1) ||
+        (rows.defined() && (!here(rows) || rows.dim() != 1 ||
+                            (rows.scalar_type() != at::kLong && rows.scalar_type() != at::kInt) ||
+                            (rows.size(0) > 0 && x.size(0) == 0))) ||
+        (bias.defined() && (!here(bias) || !is_float(bias) || recorded(bias) ||
+                            !((bias.dim() == 2 && bias.size(0) == E && bias.size(1) == N) ||
+                              (E == 1 && bias.dim() == 1 && bias.size(0) == N)))))
+      return not_taken();
+    const int64_t R = rows.defined() ? rows.size(0) : x.size(0);
+    const int act = (int)integer(a[7]), dtype = (int)integer(a[8]);
+    Place place(x);
+    const Tensor out = empty({R, N}, x, type_of(dtype));
+    if (R)
+      check(api.fmoe_fp4_linear(data(x), pitch(x), x.size(0), code(x.scalar_type()), data(rows),
+                                rows.defined() ? code(rows.scalar_type()) : FMOE_I64, data(w), data(s), data(bias),
+                                bias.defined() ? code(bias.scalar_type()) : FMOE_F32, act,
+                                static_cast<const int64_t*>(data(off)), E, N, K, R, data(out), N, dtype,
+                                place.stream),
+            "fmoe_fp4_linear");
+    return wrap(out);
+  });
+}
+
 PyObject* bind(PyObject*, PyObject* dict) {
   Api found;
 #define FMOE_FIND(name)                                                                         \
@@ -303,10 +397,14 @@ PyMethodDef kMethods[] = {
     {"route", FMOE_FAST(route),
      "route(logits, bias, top_k, score, groups, top_groups, group_score, renormalize, scale, dtype, recorded)"},
     {"sandwich", FMOE_FAST(sandwich), "sandwich(x, post, residual, pre, gate, scale, eps, recorded)"},
+    {"quantize_fp4", FMOE_FAST(quantize_fp4), "quantize_fp4(x)"},
+    {"restore_fp4", FMOE_FAST(restore_fp4), "restore_fp4(data, scales, features, dtype)"},
+    {"fp4_linear", FMOE_FAST(fp4_linear),
+     "fp4_linear(x, data, scales, features, offsets, rows, bias, activation, dtype)"},
     {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_block",
-                       "Host side of fastmoe_amd's router and norms around a block", -1, kMethods};
+                       "Host side of fastmoe_amd's router, norms around a block and 4-bit weights", -1, kMethods};
 
 }  // namespace
 

@@ -585,6 +585,36 @@ FMOE_API int fmoe_sandwich_norm_backward(const void* d_grad_y, int64_t gy_row_st
                                          void* d_grad_pre, void* d_grad_gate, void* d_workspace,
                                          int64_t workspace_bytes, void* stream);
 
+/*
+ * Weights in 4 bits: v * 2^(s - 127) with v one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives (the code's bits: sign,
+ * two of exponent, one of mantissa) and s a byte for 32 neighbouring weights of a row (255: NaN).  d_q:
+ * [rows, Kp / 2] bytes, two codes each, the earlier column's in the low half; d_scales: [rows, Kp / 32] bytes, with Kp
+ * the columns rounded up to 128; codes beyond the columns are zero.  d_q starts at a multiple of 16 bytes.
+ * fmoe_quantize_fp4 takes for each 32 the smallest power of two (from 2^-127 on) with which none of them passes 6, and
+ * rounds to the nearest (ties to even); 32 zeros: s = 127; an infinity or a NaN among them: s = 255, codes 0.
+ * fmoe_restore_fp4 writes the values, packed.
+ */
+FMOE_API int fmoe_quantize_fp4(const void* d_x, int64_t x_row_stride, int64_t rows, int64_t cols, int dtype,
+                               void* d_q, void* d_scales, void* stream);
+FMOE_API int fmoe_restore_fp4(const void* d_q, const void* d_scales, int64_t rows, int64_t cols, void* d_out,
+                              int dtype, void* stream);
+
+/*
+ * Every expert's product of 16-bit rows with weights in 4 bits:
+ *     out[r, n] = act(sum_k x[i(r), k] * w[e, n, k] + bias[e, n])          (activation: fmoe_activation)
+ * for r in [offsets[e], offsets[e + 1]), offsets[0] read as 0.  i(r) is d_index[r] (int64 or int32), or r where
+ * d_index is null.  d_x: [x_rows, K], x_dtype FMOE_BF16 or FMOE_F16; the weights are [E, N, K] of that type, held
+ * as above (d_w_scales at a multiple of 4 bytes; a scale outside 2^-23..2^13 loses what fp16 cannot hold).  d_bias
+ * [E, N] or null.  d_offsets: int64[E + 1] on the device, or null for one expert.  Sums are fp32, in an order
+ * that hangs on the sizes alone.  Rows at or beyond offsets[E] are written as zero; a row whose index lies outside
+ * [0, x_rows) has a product of zero.  K <= 131072.
+ */
+FMOE_API int fmoe_fp4_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows, int x_dtype,
+                             const void* d_index, int index_dtype, const void* d_w, const void* d_w_scales,
+                             const void* d_bias, int bias_dtype, int activation, const int64_t* d_offsets,
+                             int64_t num_experts, int64_t N, int64_t K, int64_t rows, void* d_out,
+                             int64_t out_row_stride, int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
