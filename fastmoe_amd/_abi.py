@@ -167,6 +167,7 @@ SIGNATURES: dict[str, tuple] = {
         _c_int, [_c_vp, _c_i64, _c_i64, _c_i64, _c_int, _c_vp, _c_vp, _c_vp],
     ),
     "fmoe_restore_fp4": (_c_int, [_c_vp, _c_vp, _c_i64, _c_i64, _c_vp, _c_int, _c_vp]),
+    "fmoe_fp4_linear_tile": (_c_i64, [_c_i64, _c_i64, _c_i64, _c_i64]),
     "fmoe_fp4_linear": (
         _c_int,
         [_c_vp, _c_i64, _c_i64, _c_int, _c_vp, _c_int, _c_vp, _c_vp, _c_vp, _c_int, _c_int, _c_vp, _c_i64,
