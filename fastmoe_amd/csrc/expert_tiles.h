@@ -181,7 +181,9 @@ __device__ __forceinline__ void wave_order() {
   __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
   __builtin_amdgcn_wave_barrier();
 }
-template <int KB> __device__ __forceinline__ int swizzle(int row) { return row / (256 / KB) % (KB / 16); }
+template <int KB> __device__ __forceinline__ int swizzle(int row) {
+  return KB < 256 ? row / (256 / (KB < 256 ? KB : 256)) % (KB / 16) : row % 16;
+}
 
 }  // namespace fmoe
 

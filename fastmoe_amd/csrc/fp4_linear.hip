@@ -79,11 +79,6 @@ template <> struct Operand<f16_t> {
   }
 };
 
-// The scale of byte `at` of four.
-__device__ __forceinline__ float scale_of(uint32_t four, int at) {
-  return __uint_as_float((four >> (8 * at) & 0xff) << 23);
-}
-
 // Four neighbouring columns of one output row, of which those from `n` to N are there.
 template <typename TO>
 __device__ __forceinline__ void store4(const Fp4Args& a, const Tile& t, int64_t r, int64_t n, f32x4 acc) {
@@ -113,73 +108,157 @@ template <typename F> __device__ __forceinline__ void by_output(const Fp4Args& a
   else f(f16_t{});
 }
 
-// Few rows: 16 rows by 16 columns in a workgroup, whose eight waves take pieces of 128 of K in turn, straight from memory to
-// the matrix units' registers, and add their parts in LDS in one order.
-constexpr int kFp4Waves = 8;
-template <typename TX> __global__ __launch_bounds__(kFp4Waves * kWave) void k_fp4_few(Fp4Args a) {
-  __shared__ f32x4 part[kFp4Waves][kWave];
+// Few rows: up to 16, by 16 * TN columns for each of a workgroup's eight waves, or for each KS of them, which then take pieces
+// of 256 of K in turn and add their parts in LDS in one order.  A wave brings its own weights through a ring of three buffers in
+// LDS, eight lanes for the 128 bytes of a column's piece: whole lines.  (Straight to the matrix units' registers, where
+// neighbouring lanes have different columns, they came at 3.1 TB/s, whatever the waves and pieces in flight.)
+// The rows lie in LDS, as much of K at a time as fits.  No wave waits for another but where the next part of the rows comes.
+template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __launch_bounds__(W * kWave) void k_fp4_few(Fp4Args a) {
+  constexpr int BN = 16 * TN * (W / KS);
+  constexpr int kPiece = TN * (16 * 128 + 16 * 8), kLoads = 2 * TN + 1;  // codes, then scales, of a wave
+  // 16 bytes more for each row: the rows that a read's lanes touch together start in different banks
+  __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES + 16 * 16];
+  // separate objects: the compiler then sees that reads of one need not wait for the loads in flight to the others
+  __shared__ __attribute__((aligned(1024))) uint8_t ring0[W][kPiece];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring1[W][kPiece];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring2[W][kPiece];
+  static_assert(KS == 1 || W * TN * kWave * 16 <= BYTES, "the parts fit where the rows were");
   Tile t;
   int group;
   if (!place<16>(a, &t, &group)) return;
-  const int64_t n0 = (int64_t)group * 16;
+  const int64_t n0 = (int64_t)group * BN;
   if (t.expert == a.E) {
-    by_output(a, [&](auto to) { zero_rows<decltype(to)>(a, t, n0, 16); });
+    by_output(a, [&](auto to) { zero_rows<decltype(to)>(a, t, n0, BN); });
     return;
   }
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
-  const int l16 = lane & 15, quad = lane >> 4;
-  // lane l has row (of x) or column (of the weights) l % 16 and 32 of a piece's K from 32 * (l / 16) on; the
-  // order of K is the same for both, so eight of them at a time are as good as any
-  const int64_t row = source_row(a, t.row + min(l16, t.count - 1));
-  const bool live = l16 < t.count && row >= 0;
-  const TX* xp = static_cast<const TX*>(a.x) + max(row, (int64_t)0) * a.x_stride;
-  const int64_t col = t.expert * a.N + min(n0 + l16, a.N - 1);
-  const uint8_t* wp = a.w + col * (a.Kp / 2) + quad * 16;
-  const uint8_t* sp = a.s + col * (a.Kp / kFp4Block);
-  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
-  for (int64_t k = wave * 128; k < a.Kp; k += kFp4Waves * 128) {
-    const u32x4 w = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(wp + k / 2));
-    const float scale = scale_of(*reinterpret_cast<const uint32_t*>(sp + k / kFp4Block), quad);
+  const int l16 = lane & 15, quad = lane >> 4, part = wave % KS;
+  const int64_t col0 = n0 + wave / KS * (16 * TN);
+  const uint8_t *wp[2 * TN], *sp;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t at = k + quad * 32 + j * 8;
-      const u32x4 x = live ? Eight<TX>::template load<false>(xp, at, a.K) : Eight<TX>::zero();
-      acc = Operand<TX>::mfma16(Operand<TX>::weights(w[j], scale), x, acc);
+  for (int i = 0; i < 2 * TN; ++i)
+    wp[i] = a.w + (t.expert * a.N + min(col0 + i * 8 + lane / 8, a.N - 1)) * (a.Kp / 2);
+  sp = a.s + (t.expert * a.N + min(col0 + lane / 2 % (16 * TN), a.N - 1)) * (a.Kp / kFp4Block);
+  const int pieces = (int)((a.Kp + 255) / 256), mine = pieces > part ? (pieces - part + KS - 1) / KS : 0;
+  // Piece j of this wave's.  What lies beyond a column's end is read as its last chunk once more, and meets rows of zeros.
+  auto ask = [&](uint8_t (*ring)[kPiece], int j) __attribute__((always_inline)) {
+    const int64_t p = (int64_t)j * KS + part;
+#pragma unroll
+    for (int i = 0; i < 2 * TN; ++i) {
+      const int chunk = lane % 8 ^ swizzle<128>(i * 8 + lane / 8);
+      load_piece<CPOL>(wp[i] + min(p * 8 + chunk, a.Kp / 32 - 1) * 16, ring[wave] + i * 1024);
     }
-  }
-  part[wave][lane] = acc;
-  __syncthreads();
-  if (wave != 0 || l16 >= t.count) return;
+    if (TN > 1 || lane < 32)
+      __builtin_amdgcn_global_load_lds(
+          reinterpret_cast<const FMOE_GLOBAL uint32_t*>(
+              reinterpret_cast<uintptr_t>(sp + min(p * 2 + lane % 2, a.Kp / 128 - 1) * 4)),
+          (FMOE_LDS uint32_t*)(ring[wave] + TN * 16 * 128), 4, 0, kCPolCached);
+  };
+  if (mine > 0) ask(ring0, 0);
+  if (mine > 1) ask(ring1, 1);
+  // columns of the rows that LDS holds: whole rounds of the waves' pieces
+  const int round = 256 * KS;
+  const int held = max(BYTES / 2 / t.count / round, 1) * round, pitch = held * 2 + 16;
+  auto stage = [&](int64_t from) __attribute__((always_inline)) {
+    const int width = (int)min((int64_t)held, pieces * (int64_t)256 - from) / 8;  // 16-byte chunks of a row
+    for (int i = threadIdx.x; i < t.count * width; i += W * kWave) {
+      const int r = i / width, c = i % width;
+      const int64_t row = source_row(a, t.row + r);
+      const u32x4 v = row < 0 ? Eight<TX>::zero()
+                              : Eight<TX>::template load<false>(static_cast<const TX*>(a.x) + row * a.x_stride, from + c * 8, a.K);
+      *reinterpret_cast<u32x4*>(lds + r * pitch + c * 16) = v;
+    }
+  };
+  f32x4 acc[TN];
 #pragma unroll
-  for (int v = 1; v < kFp4Waves; ++v) acc += part[v][lane];
+  for (int n = 0; n < TN; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // lane l has row (of x) or column (of the weights) l % 16 and 64 of a piece's K from 64 * (l / 16) on; the
+  // order of K is the same for both, so eight of them at a time are as good as any
+  const uint8_t* xl = lds + min(l16, t.count - 1) * pitch + quad * 128;
+  const int rounds = held / round;  // pieces of this wave in LDS at a time
+  const int all = (pieces + KS - 1) / KS;  // the same for every wave: they meet at the barriers
+  stage(0);
+  __syncthreads();
+  int base = 0;  // this wave's first piece in LDS
+  auto step = [&](uint8_t (*old)[kPiece], const uint8_t (*cur)[kPiece], int i) __attribute__((always_inline)) {
+    if (i - base == rounds) {
+      __syncthreads();
+      stage((int64_t)i * round);
+      __syncthreads();
+      base = i;
+    }
+    if (i >= mine) return;
+    if (i + 1 < mine) wait_loads<kLoads>();
+    else wait_loads<0>();
+    u32x4 w[TN][2];
+    uint32_t e[TN];
+#pragma unroll
+    for (int n = 0; n < TN; ++n) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        w[n][h] = *reinterpret_cast<const u32x4*>(cur[wave] + (n * 16 + l16) * 128 + ((quad * 2 + h) ^ swizzle<128>(l16)) * 16);
+      e[n] = *reinterpret_cast<const uint16_t*>(cur[wave] + TN * 16 * 128 + (n * 16 + l16) * 8 + quad * 2);
+    }
+    if (i + 2 < mine) ask(old, i + 2);
+    const uint8_t* xs = xl + ((i - base) * KS + part) * 512;
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        const u32x4 x = *reinterpret_cast<const u32x4*>(xs + h * 64 + k * 16);
+#pragma unroll
+        for (int n = 0; n < TN; ++n) {
+          const float scale = __uint_as_float((h ? e[n] >> 8 : e[n] & 0xff) << 23);
+          acc[n] = Operand<TX>::mfma16(Operand<TX>::weights(w[n][h][k], scale), x, acc[n]);
+        }
+      }
+  };
+  for (int i = 0; i < all; i += 3) {
+    step(ring2, ring0, i);
+    if (i + 1 < all) step(ring0, ring1, i + 1);
+    if (i + 2 < all) step(ring1, ring2, i + 2);
+  }
+  if constexpr (KS > 1) {
+    __syncthreads();
+    f32x4(*parts)[kWave] = reinterpret_cast<f32x4(*)[kWave]>(lds);
+#pragma unroll
+    for (int n = 0; n < TN; ++n) parts[wave * TN + n][lane] = acc[n];
+    __syncthreads();
+    if (part != 0) return;
+#pragma unroll
+    for (int n = 0; n < TN; ++n)
+#pragma unroll
+      for (int v = 1; v < KS; ++v) acc[n] += parts[(wave + v) * TN + n][lane];
+  }
+  if (l16 >= t.count) return;
   // lane l of a 16 x 16 result has row l % 16 and columns 4 * (l / 16) + 0..3
-  by_output(a, [&](auto to) { store4<decltype(to)>(a, t, t.row + l16, n0 + quad * 4, acc); });
+  by_output(a, [&](auto to) {
+#pragma unroll
+    for (int n = 0; n < TN; ++n) store4<decltype(to)>(a, t, t.row + l16, col0 + n * 16 + quad * 4, acc[n]);
+  });
 }
 
-// BM rows by W * WN * 32 columns of one expert in a workgroup of W waves.  Each wave has every row and its own 32 WN
-// columns, so each weight is converted once and a converted one serves all rows.  Pieces of 64 of K go through a
-// ring of buffers in LDS, which the loads write directly where rows start at multiples of 16 bytes and K has whole pieces
-// (DIRECT); else the rows' part goes through registers, zeros beyond K.
+// TM * 32 rows by 4 * WN * 32 columns of one expert in a workgroup of four waves.  Each wave has every row and its own
+// 32 WN columns, so each weight is converted once and a converted one serves all rows.
 //
-// In LDS a row's piece is 128 bytes, its 16-byte chunk c at position c ^ swizzle(row); an output's is 32 bytes, its
-// halves exchanged in every other eight outputs: what a read's lanes touch together then lies in different banks.  Lane l of
-// a matrix unit's operand has row (output) l % 32, and of a piece's K the half l / 32: four steps of 8.
-// Scales lie in LDS for kWindow of K at a time; each wave brings its own outputs'.
-constexpr int kWindow = 512;
-template <typename TX, int BM, int W, int WN, int STAGES, bool DIRECT>
-__global__ __launch_bounds__(W * kWave, 2) void k_fp4_tile(Fp4Args a) {
-  constexpr int BN = W * WN * 32, TM = BM / 32;
-  constexpr int kX = BM * 128, kStage = kX + BN * 32;
-  constexpr int PX = BM / 8 / W, kLoads = (DIRECT ? PX : 0) + WN;  // loads of a wave a piece
-  static_assert(PX * 8 * W == BM, "whole loads");
-  static_assert(STAGES == 3 || STAGES == 4, "buffers");
-  // separate objects: the compiler then sees that reads of one stage need not wait for the loads in
-  // flight to the others
-  __shared__ __attribute__((aligned(1024))) uint8_t stage0[kStage];
-  __shared__ __attribute__((aligned(1024))) uint8_t stage1[kStage];
-  __shared__ __attribute__((aligned(1024))) uint8_t stage2[kStage];
-  __shared__ __attribute__((aligned(1024))) uint8_t stage3[STAGES > 3 ? kStage : 1];
-  __shared__ uint32_t scales[BN][kWindow / kFp4Block / 4];
+// The rows go in pieces of 64 of K through a ring of three buffers in LDS, which the loads write directly where rows start at
+// multiples of 16 bytes and K has whole pieces (DIRECT); else through registers, zeros beyond K.  A wave brings its own
+// weights 256 of K at a time, eight lanes for a column's 128 bytes (whole lines: with 32 bytes of a column at a time each line came
+// twice, and lines that pass the caches four times), into a buffer of its own, takes all of its codes from there
+// into registers, and asks for the next 256 at once: they are on their way while these are multiplied.
+//
+// In LDS a row's piece and a column's codes are 128 bytes each, their 16-byte chunk c at position c ^ swizzle: what a read's
+// lanes touch together then lies in different banks.  Lane l of a matrix unit's operand has row (column) l % 32, and of
+// a piece's K the half l / 32: four steps of 8, a chunk of codes for all four.
+template <typename TX, int TM, int WN, bool DIRECT>
+__global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
+  constexpr int W = 4, BM = TM * 32, BN = W * WN * 32;
+  constexpr int kX = BM * 128, kCodes = WN * 32 * 128, kW = WN * 5;  // loads of a wave for 256 of K of its columns
+  // separate objects: the compiler then sees that reads of one need not wait for the loads in flight to the others
+  __shared__ __attribute__((aligned(1024))) uint8_t rows0[kX];
+  __shared__ __attribute__((aligned(1024))) uint8_t rows1[kX];
+  __shared__ __attribute__((aligned(1024))) uint8_t rows2[kX];
+  __shared__ __attribute__((aligned(1024))) uint8_t weights[W][kCodes + WN * 32 * 8];  // codes, then scales
   __shared__ float col_bias[BN];
   __shared__ uint8_t row_live[BM];
   Tile t;
@@ -192,56 +271,53 @@ __global__ __launch_bounds__(W * kWave, 2) void k_fp4_tile(Fp4Args a) {
   }
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
   const int l32 = lane & 31, half = lane >> 5;
-  const int w0 = wave * WN * 32;  // this wave's outputs
-  const TX* xp[PX];
-  int xc[PX];  // the column that the lane reads of a piece
-#pragma unroll
-  for (int i = 0; i < PX; ++i) {
-    const int r = (wave * PX + i) * 8 + lane / 8;
-    xp[i] = static_cast<const TX*>(a.x) + max(source_row(a, t.row + min(r, t.count - 1)), (int64_t)0) * a.x_stride;
-    xc[i] = (lane % 8 ^ swizzle<128>(r)) * 8;
-    if constexpr (DIRECT) xp[i] += xc[i];
-  }
-  const uint8_t* wp[WN];
-#pragma unroll
-  for (int i = 0; i < WN; ++i) {
-    const int c = lane / 2;
-    const int64_t col = t.expert * a.N + min(n0 + w0 + i * 32 + c, a.N - 1);
-    wp[i] = a.w + col * (a.Kp / 2) + ((lane & 1) ^ (c >> 3 & 1)) * 16;
-  }
-  const int pieces = (int)((a.K + 63) / 64);
-  // loads beyond the last piece read it once more, into a buffer that nobody reads: the number of
-  // loads in flight is then the same in every step
-  auto at = [&](int piece) { return (int64_t)min(piece, pieces - 1); };
-  auto load_one = [&](uint8_t* s, int64_t piece, int i) {
-    if (DIRECT && i < PX)
-      load_piece<kCPolCached>(reinterpret_cast<const uint8_t*>(xp[i < PX ? i : 0] + piece * 64), s + (wave * PX + i) * 1024);
-    else {
-      const int j = i - (DIRECT ? PX : 0);
-      load_piece<kCPolCached>(wp[j] + piece * 32, s + kX + (wave * WN + j) * 1024);
+  const int w0 = wave * WN * 32;  // this wave's columns
+  // Its columns' codes and scales through descriptors that end with the last column: what lies beyond reads as zero.
+  const int here = (int)max(min((int64_t)WN * 32, a.N - n0 - w0), (int64_t)0);
+  const int64_t first = t.expert * a.N + min(n0 + w0, a.N - 1);
+  const int code_pitch = (int)(a.Kp / 2), scale_pitch = (int)(a.Kp / kFp4Block);
+  const rsrc_t codes_at = make_rsrc(a.w + first * code_pitch, (uint32_t)here * code_pitch);
+  const rsrc_t scales_at = make_rsrc(a.s + first * scale_pitch, (uint32_t)here * scale_pitch);
+  const int code_from = lane / 8 * code_pitch, scale_from = lane / 2 * scale_pitch + lane % 2 * 4;
+  auto load_w = [&](int s, int i) __attribute__((always_inline)) {  // load i of 256 of K
+    if (i < 4 * WN) {
+      const int chunk = (lane % 8) ^ swizzle<128>(i * 8 + lane / 8);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(codes_at, (FMOE_LDS void*)(weights[wave] + i * 1024), 16,
+                                               code_from + chunk * 16, i * 8 * code_pitch + s * 128, 0, kCPol);
+    } else {
+      const int n = i - 4 * WN;
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_at, (FMOE_LDS void*)(weights[wave] + kCodes + n * 256), 4, scale_from,
+                                               n * 32 * scale_pitch + s * 8, 0, kCPolCached);
     }
   };
-  u32x4 xr[DIRECT ? 1 : PX];  // the rows' part of a piece on its way
-  auto fetch = [&](int64_t piece) {
+#pragma unroll
+  for (int i = 0; i < kW; ++i) load_w(0, i);  // before the rows' places are known
+  const TX* xp[TM];
+  int xc[TM];  // the column that the lane reads of a piece
+#pragma unroll
+  for (int m = 0; m < TM; ++m) {
+    const int r = m * 32 + wave * 8 + lane / 8;
+    xp[m] = static_cast<const TX*>(a.x) + max(source_row(a, t.row + min(r, t.count - 1)), (int64_t)0) * a.x_stride;
+    xc[m] = (lane % 8 ^ swizzle<128>(r)) * 8;
+    if constexpr (DIRECT) xp[m] += xc[m];
+  }
+  for (int c = threadIdx.x; c < BN; c += W * kWave)
+    col_bias[c] = a.bias ? load_weight(a.bias, a.bias_dtype, t.expert * a.N + min(n0 + c, a.N - 1)) : 0.f;
+  for (int r = threadIdx.x; r < BM; r += W * kWave) row_live[r] = source_row(a, t.row + min(r, t.count - 1)) >= 0;
+  const int pieces = (int)((a.K + 63) / 64), supers = (pieces + 3) / 4;
+  auto load_x = [&](uint8_t* s, int piece, int m) __attribute__((always_inline)) {
+    load_piece<kCPolCached>(reinterpret_cast<const uint8_t*>(xp[m] + (int64_t)piece * 64), s + (m * 4 + wave) * 1024);
+  };
+  u32x4 xr[DIRECT ? 1 : TM];  // the rows' part of a piece on its way
+  auto fetch = [&](int piece) __attribute__((always_inline)) {
     if constexpr (!DIRECT)
 #pragma unroll
-      for (int i = 0; i < PX; ++i) xr[i] = Eight<TX>::template load<false>(xp[i], piece * 64 + xc[i], a.K);
+      for (int m = 0; m < TM; ++m) xr[m] = Eight<TX>::template load<false>(xp[m], (int64_t)piece * 64 + xc[m], a.K);
   };
-  auto put = [&](uint8_t* s) {
+  auto put = [&](uint8_t* s) __attribute__((always_inline)) {
     if constexpr (!DIRECT)
 #pragma unroll
-      for (int i = 0; i < PX; ++i) *reinterpret_cast<u32x4*>(s + (wave * PX + i) * 1024 + lane * 16) = xr[i];
-  };
-  // this wave's scales from column `k` on, an output's 16 bytes in four lanes
-  const uint8_t* sp = a.s + t.expert * a.N * (a.Kp / kFp4Block);
-  auto window = [&](int64_t k) {
-    const int64_t Ks = a.Kp / kFp4Block, from = k / kFp4Block + lane % 4 * 4;
-#pragma unroll
-    for (int i = 0; i < WN * 2; ++i) {
-      const int c = w0 + i * 16 + lane / 4;
-      scales[c][lane % 4] = *reinterpret_cast<const uint32_t*>(sp + min(n0 + c, a.N - 1) * Ks + min(from, Ks - 4));
-    }
-    wave_order();
+      for (int m = 0; m < TM; ++m) *reinterpret_cast<u32x4*>(s + (m * 4 + wave) * 1024 + lane * 16) = xr[m];
   };
   f32x16 acc[WN][TM];
 #pragma unroll
@@ -251,128 +327,115 @@ __global__ __launch_bounds__(W * kWave, 2) void k_fp4_tile(Fp4Args a) {
 #pragma unroll
       for (int i = 0; i < 16; ++i) acc[n][m][i] = 0.f;
   u32x4 xv[2][TM], wv[2][WN];  // operands of this and the next step
-  u32x4 codes[WN], next_codes[WN];
-  float scale[WN], next_scale[WN];
-  auto read_x = [&](const uint8_t* s, int k, int to, int m) {
+  u32x4 codes[WN][4];          // of 256 of K
+  uint32_t scales[WN][2];
+  auto read_x = [&](const uint8_t* s, int k, int to, int m) __attribute__((always_inline)) {
     xv[to][m] = *reinterpret_cast<const u32x4*>(s + (m * 32 + l32) * 128 + ((half * 4 + k) ^ swizzle<128>(l32)) * 16);
   };
-  auto read_codes = [&](const uint8_t* s, u32x4* to) {
-#pragma unroll
-    for (int n = 0; n < WN; ++n)
-      to[n] = *reinterpret_cast<const u32x4*>(s + kX + (w0 + n * 32 + l32) * 32 + (half ^ (l32 >> 3 & 1)) * 16);
-  };
-  auto read_scales = [&](int piece, float* to) {
+  auto read_w = [&] __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < WN; ++n) {
-      const uint8_t* four = reinterpret_cast<const uint8_t*>(scales[w0 + n * 32 + l32]);
-      to[n] = __uint_as_float((uint32_t)four[piece % (kWindow / 64) * 2 + half] << 23);
+      const u32x2 s = *reinterpret_cast<const u32x2*>(weights[wave] + kCodes + (n * 32 + l32) * 8);
+      scales[n][0] = s[0] >> (8 * half);
+      scales[n][1] = s[1] >> (8 * half);
     }
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+#pragma unroll
+      for (int n = 0; n < WN; ++n)
+        codes[n][c] = *reinterpret_cast<const u32x4*>(weights[wave] + (n * 32 + l32) * 128 + ((2 * c + half) ^ swizzle<128>(l32)) * 16);
   };
-  // Step i multiplies piece i in buffer `cur`, by `live` tiles of 32 rows.  Before its last part each wave has read all of
-  // the piece and waits until its loads of piece i + 1 have arrived; behind the barrier that holds for every
-  // wave, so `next` is read, and `cur` is free.  Piece i + STAGES - 1 is loaded into `old`.
-  auto step = [&](auto live, uint8_t* old, uint8_t* cur, const uint8_t* next, int i)
+  auto convert = [&](int c, int k, int to) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < WN; ++n)
+      wv[to][n] = Operand<TX>::weights(codes[n][c][k], __uint_as_float((scales[n][c / 2] >> (16 * (c % 2)) & 0xff) << 23));
+  };
+  // Step i multiplies piece i in buffer `cur`, the part c of 256 of K, by `live` tiles of 32 rows.  Before its last quarter each
+  // wave has read all of the piece and waits until its loads of piece i + 1 have arrived; behind the barrier that
+  // holds for every wave, so `next` is read, and `cur` is free.  Piece i + 2 is loaded into `old`.
+  auto step = [&](auto live, auto part, uint8_t* old, uint8_t* cur, const uint8_t* next, int i)
                   __attribute__((always_inline)) {
-    constexpr int kLive = decltype(live)::value;
-    const int64_t rest = at(i + STAGES - 1);
-    if ((i + 1) % (kWindow / 64) == 0 && i + 1 < pieces) window((int64_t)(i + 1) * 64);
+    constexpr int kLive = decltype(live)::value, c = decltype(part)::value, kParts = kLive * WN;
+    constexpr int kRows = DIRECT ? kLive : 0;  // loads of a wave a piece
+    const bool more_x = i + 2 < pieces, more_w = c < 2 && i / 4 + 1 < supers;
+    put(old);  // what was fetched in the last step
+    fetch(min(i + 3, pieces - 1));
+    if (c == 0 && more_w) __builtin_amdgcn_s_waitcnt(0xc07f);  // this wave's codes are in registers: their place is free
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       const int now = k & 1;
-      if (k == 0) {
-        put(old);  // what was fetched in the last step
-        fetch(at(i + STAGES));
-      }
-      if (k == 1) read_scales(i + 1, next_scale);
       if (k == 3) {
-        wait_loads<(STAGES - 2) * kLoads>();
+        // younger than the loads of piece i + 1 are those of piece i + 2 and, where they began in this step or the last, those
+        // of the weights
+        if (!more_x) wait_loads<0>();
+        else if (more_w) wait_loads<kRows + kW>();
+        else wait_loads<kRows>();
         barrier();
-        read_codes(next, next_codes);
+        if (c == 3) read_w();
       }
-      constexpr int kOps = kLive;
 #pragma unroll
-      for (int j = 0; j < kLive * WN; ++j) {
+      for (int j = 0; j < kParts; ++j) {
         const int m = j / WN, n = j % WN;
         acc[n][m] = Operand<TX>::mfma32(wv[now][n], xv[now][m], acc[n][m]);
+        if (n == WN - 1) read_x(k == 3 ? next : cur, k == 3 ? 0 : k + 1, now ^ 1, m);
+        if (k == 0 && more_x && n == 0)
+          if constexpr (DIRECT) load_x(old, i + 2, m);
+        if ((k == 1 || k == 2) && c == 0 && more_w) {
 #pragma unroll
-        for (int o = j * kOps / (kLive * WN); o < (j + 1) * kOps / (kLive * WN); ++o)
-          read_x(k == 3 ? next : cur, k == 3 ? 0 : k + 1, now ^ 1, o);
-        if (k < 3) {
-#pragma unroll
-          for (int l = kLoads * (k * kLive * WN + j) / (3 * kLive * WN); l < kLoads * (k * kLive * WN + j + 1) / (3 * kLive * WN); ++l)
-            load_one(old, rest, l);
+          for (int l = kW * ((k - 1) * kParts + j) / (2 * kParts); l < kW * ((k - 1) * kParts + j + 1) / (2 * kParts); ++l)
+            load_w(i / 4 + 1, l);
         }
-        // the next step's weights: of the next piece as late as can be, its codes were asked for in this step
-        constexpr int kLast = kLive * WN - 1;
-        if (j == (k == 3 ? kLast : kLast / 2)) {
-#pragma unroll
-          for (int q = 0; q < WN; ++q)
-            wv[now ^ 1][q] = k == 3 ? Operand<TX>::weights(next_codes[q][0], next_scale[q])
-                                    : Operand<TX>::weights(codes[q][(k + 1) % 4], scale[q]);
-        }
+        // the next step's weights; a new part's as late as can be, they are being read
+        if (j == (k == 3 && c == 3 ? kParts - 1 : (kParts - 1) / 2)) convert(k == 3 ? (c + 1) % 4 : c, (k + 1) % 4, now ^ 1);
         __builtin_amdgcn_sched_barrier(0);
       }
     }
-#pragma unroll
-    for (int n = 0; n < WN; ++n) {
-      codes[n] = next_codes[n];
-      scale[n] = next_scale[n];
-    }
   };
   auto run = [&](auto live) __attribute__((always_inline)) {
-    int i = 0;
-    if constexpr (STAGES == 3) {
-      for (; i + 3 <= pieces; i += 3) {
-        step(live, stage2, stage0, stage1, i);
-        step(live, stage0, stage1, stage2, i + 1);
-        step(live, stage1, stage2, stage0, i + 2);
-      }
-      if (i < pieces) step(live, stage2, stage0, stage1, i);
-      if (i + 1 < pieces) step(live, stage0, stage1, stage2, i + 1);
+    constexpr int kLive = decltype(live)::value;
+    if constexpr (DIRECT) {
+#pragma unroll
+      for (int m = 0; m < kLive; ++m) load_x(rows0, 0, m);
+#pragma unroll
+      for (int m = 0; m < kLive; ++m) load_x(rows1, min(1, pieces - 1), m);
     } else {
-      for (; i + 4 <= pieces; i += 4) {
-        step(live, stage3, stage0, stage1, i);
-        step(live, stage0, stage1, stage2, i + 1);
-        step(live, stage1, stage2, stage3, i + 2);
-        step(live, stage2, stage3, stage0, i + 3);
-      }
-      if (i < pieces) step(live, stage3, stage0, stage1, i);
-      if (i + 1 < pieces) step(live, stage0, stage1, stage2, i + 1);
-      if (i + 2 < pieces) step(live, stage1, stage2, stage3, i + 2);
+      fetch(0);
+      put(rows0);
+      fetch(min(1, pieces - 1));
+      put(rows1);
+      fetch(min(2, pieces - 1));
+    }
+    wait_loads<DIRECT ? kLive : 0>();
+    __syncthreads();
+    read_w();
+#pragma unroll
+    for (int m = 0; m < kLive; ++m) read_x(rows0, 0, 0, m);
+    convert(0, 0, 0);
+    using std::integral_constant;
+    constexpr integral_constant<int, 0> c0{};
+    constexpr integral_constant<int, 1> c1{};
+    constexpr integral_constant<int, 2> c2{};
+    constexpr integral_constant<int, 3> c3{};
+    for (int i = 0; i < pieces; i += 12) {
+      step(live, c0, rows2, rows0, rows1, i);
+      if (i + 1 < pieces) step(live, c1, rows0, rows1, rows2, i + 1);
+      if (i + 2 < pieces) step(live, c2, rows1, rows2, rows0, i + 2);
+      if (i + 3 < pieces) step(live, c3, rows2, rows0, rows1, i + 3);
+      if (i + 4 < pieces) step(live, c0, rows0, rows1, rows2, i + 4);
+      if (i + 5 < pieces) step(live, c1, rows1, rows2, rows0, i + 5);
+      if (i + 6 < pieces) step(live, c2, rows2, rows0, rows1, i + 6);
+      if (i + 7 < pieces) step(live, c3, rows0, rows1, rows2, i + 7);
+      if (i + 8 < pieces) step(live, c0, rows1, rows2, rows0, i + 8);
+      if (i + 9 < pieces) step(live, c1, rows2, rows0, rows1, i + 9);
+      if (i + 10 < pieces) step(live, c2, rows0, rows1, rows2, i + 10);
+      if (i + 11 < pieces) step(live, c3, rows1, rows2, rows0, i + 11);
     }
   };
-  auto ring = [&](int i) { return i == 0 ? stage0 : i == 1 ? stage1 : i == 2 ? stage2 : stage3; };
-  for (int c = threadIdx.x; c < BN; c += W * kWave)
-    col_bias[c] = a.bias ? load_weight(a.bias, a.bias_dtype, t.expert * a.N + min(n0 + c, a.N - 1)) : 0.f;
-  for (int r = threadIdx.x; r < BM; r += W * kWave) row_live[r] = source_row(a, t.row + min(r, t.count - 1)) >= 0;
-  window(0);
-#pragma unroll
-  for (int i = 0; i < STAGES - 1; ++i) {
-    fetch(at(i));
-    put(ring(i));
-#pragma unroll
-    for (int l = 0; l < kLoads; ++l) load_one(ring(i), at(i), l);
-  }
-  fetch(at(STAGES - 1));
-  wait_loads<(STAGES - 2) * kLoads>();
-  __syncthreads();
-  read_codes(stage0, codes);
-  read_scales(0, scale);
-#pragma unroll
-  for (int m = 0; m < TM; ++m) read_x(stage0, 0, 0, m);
-#pragma unroll
-  for (int n = 0; n < WN; ++n) wv[0][n] = Operand<TX>::weights(codes[n][0], scale[n]);
   const int tiles = (t.count + 31) / 32;
-  if constexpr (TM == 1) run(std::integral_constant<int, 1>{});
-  else if constexpr (TM == 2) {
-    if (tiles == 1) run(std::integral_constant<int, 1>{});
-    else run(std::integral_constant<int, 2>{});
-  } else {
-    if (tiles == 1) run(std::integral_constant<int, 1>{});
-    else if (tiles == 2) run(std::integral_constant<int, 2>{});
-    else if (tiles == 3) run(std::integral_constant<int, 3>{});
-    else run(std::integral_constant<int, 4>{});
-  }
+  if (TM >= 4 && tiles == 4) run(std::integral_constant<int, TM >= 4 ? 4 : 1>{});
+  else if (TM >= 3 && tiles == 3) run(std::integral_constant<int, TM >= 3 ? 3 : 1>{});
+  else if (TM >= 2 && tiles == 2) run(std::integral_constant<int, TM >= 2 ? 2 : 1>{});
+  else run(std::integral_constant<int, 1>{});
   wait_loads<0>();
   __syncthreads();
   // Each wave turns its results, 32 rows at a time, into rows of the output's type in LDS and stores
@@ -380,12 +443,12 @@ __global__ __launch_bounds__(W * kWave, 2) void k_fp4_tile(Fp4Args a) {
   by_output(a, [&](auto to_type) {
     using TO = decltype(to_type);
     constexpr int kSize = ElemInfo<TO>::kBytes;
-    constexpr auto fits = [](int tiles) { return kStage / (32 * (tiles * 32 * kSize + 16)) * STAGES >= W; };
+    constexpr auto fits = [](int tiles) { return kX / (32 * (tiles * 32 * kSize + 16)) * 3 >= W; };
     constexpr int CT = fits(WN) ? WN : 1;  // column tiles at a time
     constexpr int kPitch = CT * 32 * kSize + 16;  // 16 bytes more: the 32 rows start in different banks
-    constexpr int kPerStage = kStage / (32 * kPitch);
-    static_assert(kPerStage * STAGES >= W, "the stages hold the results");
-    uint8_t* mine = ring(wave / kPerStage) + wave % kPerStage * (32 * kPitch);
+    constexpr int kPerStage = kX / (32 * kPitch);
+    static_assert(kPerStage * 3 >= W, "the stages hold the results");
+    uint8_t* mine = (wave / kPerStage == 0 ? rows0 : wave / kPerStage == 1 ? rows1 : rows2) + wave % kPerStage * (32 * kPitch);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       const int first = m * 32;
@@ -506,44 +569,50 @@ using namespace fmoe;
 
 namespace {
 
-template <typename TX> int launch_few(const char* who, Fp4Args a, hipStream_t s) {
-  const int64_t groups = grid_of(who, &a, 16, 16, kFp4Waves * kWave);
+template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> int launch_few(const char* who, Fp4Args a, hipStream_t s) {
+  const int64_t groups = grid_of(who, &a, 16, 16 * TN * (W / KS), W * kWave);
   if (groups < 0) return FMOE_ERANGE;
-  hipLaunchKernelGGL((k_fp4_few<TX>), dim3((unsigned)groups), dim3(kFp4Waves * kWave), 0, s, a);
+  hipLaunchKernelGGL((k_fp4_few<TX, W, TN, KS, BYTES, CPOL>), dim3((unsigned)groups), dim3(W * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
-template <typename TX, int BM, int W, int WN, int STAGES>
-int launch_tile(const char* who, Fp4Args a, hipStream_t s) {
-  const int64_t groups = grid_of(who, &a, BM, W * WN * 32, W * kWave);
+template <typename TX, int TM, int WN> int launch_tile(const char* who, Fp4Args a, hipStream_t s) {
+  const int64_t groups = grid_of(who, &a, TM * 32, WN * 128, 4 * kWave);
   if (groups < 0) return FMOE_ERANGE;
   const bool direct = a.K % 64 == 0 && a.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
-  const dim3 grid((unsigned)groups), block(W * kWave);
-  if (direct) hipLaunchKernelGGL((k_fp4_tile<TX, BM, W, WN, STAGES, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((k_fp4_tile<TX, BM, W, WN, STAGES, false>), grid, block, 0, s, a);
+  const dim3 grid((unsigned)groups), block(4 * kWave);
+  if (direct) hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, true>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, false>), grid, block, 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
 // The variant for these sizes, as 1000 * rows + columns of its tile.
-enum Variant { kFew = 16016, k32x128 = 32128, k64x128 = 64128, k128x256 = 128256 };
+enum Variant { kFew = 16016, k96x128 = 96128, k96x256 = 96256 };
 #ifndef FMOE_FP4_TILE
 #define FMOE_FP4_TILE 0
+#endif
+#ifndef FMOE_FEW
+#define FMOE_FEW 8, 1, 1, 24576, kCPol
+#endif
+#ifndef FMOE_TW
+#define FMOE_TW 3, 2
+#endif
+#ifndef FMOE_TN
+#define FMOE_TN 3, 1
 #endif
 Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
   if (FMOE_FP4_TILE) return (Variant)FMOE_FP4_TILE;
   const int64_t per = rows / E;
   if (per <= 8) return kFew;
-  if (per <= 32) return k32x128;
-  if (per <= 64) return k64x128;
-  return k128x256;
+  if (per <= 32) return k96x128;
+  return k96x256;
 }
 
 template <typename TX> int launch_linear(const char* who, const Fp4Args& a, hipStream_t s) {
   switch (pick(a.rows, a.E, a.N, a.K)) {
-    case k32x128: return launch_tile<TX, 32, 4, 1, 4>(who, a, s);
-    case k64x128: return launch_tile<TX, 64, 4, 1, 4>(who, a, s);
-    case k128x256: return launch_tile<TX, 128, 4, 2, 3>(who, a, s);
-    default: return launch_few<TX>(who, a, s);
+    case k96x128: return launch_tile<TX, FMOE_TN>(who, a, s);
+    case k96x256: return launch_tile<TX, FMOE_TW>(who, a, s);
+    default: return launch_few<TX, FMOE_FEW>(who, a, s);
   }
 }
 
