@@ -108,21 +108,26 @@ template <typename F> __device__ __forceinline__ void by_output(const Fp4Args& a
   else f(f16_t{});
 }
 
-// Few rows: up to 16, by 16 * TN columns for each of a workgroup's eight waves, or for each KS of them, which then take pieces
+// Few rows: up to 16, by 16 columns for each of a workgroup's eight waves, or for each KS of them, which then take pieces
 // of 256 of K in turn and add their parts in LDS in one order.  A wave brings its own weights through a ring of three buffers in
 // LDS, eight lanes for the 128 bytes of a column's piece: whole lines.  (Straight to the matrix units' registers, where
-// neighbouring lanes have different columns, they came at 3.1 TB/s, whatever the waves and pieces in flight.)
+// neighbouring lanes have different columns, they came at 3.1 TB/s, whatever the waves and pieces in flight; so at 5.)
 // The rows lie in LDS, as much of K at a time as fits.  No wave waits for another but where the next part of the rows comes.
-template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __launch_bounds__(W * kWave) void k_fp4_few(Fp4Args a) {
-  constexpr int BN = 16 * TN * (W / KS);
-  constexpr int kPiece = TN * (16 * 128 + 16 * 8), kLoads = 2 * TN + 1;  // codes, then scales, of a wave
+constexpr int kFewWaves = 8;
+// Bytes of LDS for rows: at least a round of all waves' pieces of 16 rows; where K is split over one or two, two workgroups
+// share a CU's.
+template <int KS> constexpr int few_bytes() { return KS > 2 ? 16 * 256 * KS * 2 : 24576; }
+template <typename TX, int KS> __global__ __launch_bounds__(kFewWaves * kWave) void k_fp4_few(Fp4Args a) {
+  constexpr int BN = 16 * (kFewWaves / KS), kFewBytes = few_bytes<KS>();
+  constexpr int kCodes = 16 * 128, kPiece = kCodes + 16 * 8, kLoads = 3;  // codes, then scales, of a wave
   // 16 bytes more for each row: the rows that a read's lanes touch together start in different banks
-  __shared__ __attribute__((aligned(16))) uint8_t lds[BYTES + 16 * 16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[kFewBytes + 16 * 16];
   // separate objects: the compiler then sees that reads of one need not wait for the loads in flight to the others
-  __shared__ __attribute__((aligned(1024))) uint8_t ring0[W][kPiece];
-  __shared__ __attribute__((aligned(1024))) uint8_t ring1[W][kPiece];
-  __shared__ __attribute__((aligned(1024))) uint8_t ring2[W][kPiece];
-  static_assert(KS == 1 || W * TN * kWave * 16 <= BYTES, "the parts fit where the rows were");
+  __shared__ __attribute__((aligned(1024))) uint8_t ring0[kFewWaves][kPiece];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring1[kFewWaves][kPiece];
+  __shared__ __attribute__((aligned(1024))) uint8_t ring2[kFewWaves][kPiece];
+  static_assert(KS == 1 || kFewWaves * kWave * 16 <= kFewBytes, "the parts fit where the rows were");
+  static_assert(16 * 256 * KS * 2 <= kFewBytes, "a round of 16 rows fits");
   Tile t;
   int group;
   if (!place<16>(a, &t, &group)) return;
@@ -133,35 +138,32 @@ template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __
   }
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
   const int l16 = lane & 15, quad = lane >> 4, part = wave % KS;
-  const int64_t col0 = n0 + wave / KS * (16 * TN);
-  const uint8_t *wp[2 * TN], *sp;
-#pragma unroll
-  for (int i = 0; i < 2 * TN; ++i)
-    wp[i] = a.w + (t.expert * a.N + min(col0 + i * 8 + lane / 8, a.N - 1)) * (a.Kp / 2);
-  sp = a.s + (t.expert * a.N + min(col0 + lane / 2 % (16 * TN), a.N - 1)) * (a.Kp / kFp4Block);
+  const int64_t col0 = n0 + wave / KS * 16;
+  auto column = [&](int c) { return t.expert * a.N + min(col0 + c, a.N - 1); };
+  const uint8_t* const wp[2] = {a.w + column(lane / 8) * (a.Kp / 2), a.w + column(8 + lane / 8) * (a.Kp / 2)};
+  const uint8_t* const sp = a.s + column(lane / 2 % 16) * (a.Kp / kFp4Block);
   const int pieces = (int)((a.Kp + 255) / 256), mine = pieces > part ? (pieces - part + KS - 1) / KS : 0;
   // Piece j of this wave's.  What lies beyond a column's end is read as its last chunk once more, and meets rows of zeros.
   auto ask = [&](uint8_t (*ring)[kPiece], int j) __attribute__((always_inline)) {
     const int64_t p = (int64_t)j * KS + part;
 #pragma unroll
-    for (int i = 0; i < 2 * TN; ++i) {
+    for (int i = 0; i < 2; ++i) {
       const int chunk = lane % 8 ^ swizzle<128>(i * 8 + lane / 8);
-      load_piece<CPOL>(wp[i] + min(p * 8 + chunk, a.Kp / 32 - 1) * 16, ring[wave] + i * 1024);
+      load_piece<kCPol>(wp[i] + min(p * 8 + chunk, a.Kp / 32 - 1) * 16, ring[wave] + i * 1024);
     }
-    if (TN > 1 || lane < 32)
-      __builtin_amdgcn_global_load_lds(
-          reinterpret_cast<const FMOE_GLOBAL uint32_t*>(
-              reinterpret_cast<uintptr_t>(sp + min(p * 2 + lane % 2, a.Kp / 128 - 1) * 4)),
-          (FMOE_LDS uint32_t*)(ring[wave] + TN * 16 * 128), 4, 0, kCPolCached);
+    if (lane < 32)
+      __builtin_amdgcn_global_load_lds(reinterpret_cast<const FMOE_GLOBAL uint32_t*>(reinterpret_cast<uintptr_t>(
+                                           sp + min(p * 2 + lane % 2, a.Kp / 128 - 1) * 4)),
+                                       (FMOE_LDS uint32_t*)(ring[wave] + kCodes), 4, 0, kCPolCached);
   };
   if (mine > 0) ask(ring0, 0);
   if (mine > 1) ask(ring1, 1);
   // columns of the rows that LDS holds: whole rounds of the waves' pieces
   const int round = 256 * KS;
-  const int held = max(BYTES / 2 / t.count / round, 1) * round, pitch = held * 2 + 16;
+  const int held = kFewBytes / 2 / t.count / round * round, pitch = held * 2 + 16;
   auto stage = [&](int64_t from) __attribute__((always_inline)) {
     const int width = (int)min((int64_t)held, pieces * (int64_t)256 - from) / 8;  // 16-byte chunks of a row
-    for (int i = threadIdx.x; i < t.count * width; i += W * kWave) {
+    for (int i = threadIdx.x; i < t.count * width; i += kFewWaves * kWave) {
       const int r = i / width, c = i % width;
       const int64_t row = source_row(a, t.row + r);
       const u32x4 v = row < 0 ? Eight<TX>::zero()
@@ -169,13 +171,11 @@ template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __
       *reinterpret_cast<u32x4*>(lds + r * pitch + c * 16) = v;
     }
   };
-  f32x4 acc[TN];
-#pragma unroll
-  for (int n = 0; n < TN; ++n) acc[n] = f32x4{0.f, 0.f, 0.f, 0.f};
+  f32x4 acc = {0.f, 0.f, 0.f, 0.f};
   // lane l has row (of x) or column (of the weights) l % 16 and 64 of a piece's K from 64 * (l / 16) on; the
   // order of K is the same for both, so eight of them at a time are as good as any
   const uint8_t* xl = lds + min(l16, t.count - 1) * pitch + quad * 128;
-  const int rounds = held / round;  // pieces of this wave in LDS at a time
+  const int rounds = held / round;         // pieces of this wave in LDS at a time
   const int all = (pieces + KS - 1) / KS;  // the same for every wave: they meet at the barriers
   stage(0);
   __syncthreads();
@@ -190,28 +190,20 @@ template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __
     if (i >= mine) return;
     if (i + 1 < mine) wait_loads<kLoads>();
     else wait_loads<0>();
-    u32x4 w[TN][2];
-    uint32_t e[TN];
+    u32x4 w[2];
 #pragma unroll
-    for (int n = 0; n < TN; ++n) {
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-        w[n][h] = *reinterpret_cast<const u32x4*>(cur[wave] + (n * 16 + l16) * 128 + ((quad * 2 + h) ^ swizzle<128>(l16)) * 16);
-      e[n] = *reinterpret_cast<const uint16_t*>(cur[wave] + TN * 16 * 128 + (n * 16 + l16) * 8 + quad * 2);
-    }
+    for (int h = 0; h < 2; ++h)
+      w[h] = *reinterpret_cast<const u32x4*>(cur[wave] + l16 * 128 + ((quad * 2 + h) ^ swizzle<128>(l16)) * 16);
+    const uint32_t e = *reinterpret_cast<const uint16_t*>(cur[wave] + kCodes + l16 * 8 + quad * 2);
     if (i + 2 < mine) ask(old, i + 2);
     const uint8_t* xs = xl + ((i - base) * KS + part) * 512;
 #pragma unroll
-    for (int h = 0; h < 2; ++h)
+    for (int h = 0; h < 2; ++h) {
+      const float scale = __uint_as_float((h ? e >> 8 : e & 0xff) << 23);
 #pragma unroll
-      for (int k = 0; k < 4; ++k) {
-        const u32x4 x = *reinterpret_cast<const u32x4*>(xs + h * 64 + k * 16);
-#pragma unroll
-        for (int n = 0; n < TN; ++n) {
-          const float scale = __uint_as_float((h ? e[n] >> 8 : e[n] & 0xff) << 23);
-          acc[n] = Operand<TX>::mfma16(Operand<TX>::weights(w[n][h][k], scale), x, acc[n]);
-        }
-      }
+      for (int k = 0; k < 4; ++k)
+        acc = Operand<TX>::mfma16(Operand<TX>::weights(w[h][k], scale), *reinterpret_cast<const u32x4*>(xs + h * 64 + k * 16), acc);
+    }
   };
   for (int i = 0; i < all; i += 3) {
     step(ring2, ring0, i);
@@ -221,21 +213,15 @@ template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> __global__ __
   if constexpr (KS > 1) {
     __syncthreads();
     f32x4(*parts)[kWave] = reinterpret_cast<f32x4(*)[kWave]>(lds);
-#pragma unroll
-    for (int n = 0; n < TN; ++n) parts[wave * TN + n][lane] = acc[n];
+    parts[wave][lane] = acc;
     __syncthreads();
     if (part != 0) return;
 #pragma unroll
-    for (int n = 0; n < TN; ++n)
-#pragma unroll
-      for (int v = 1; v < KS; ++v) acc[n] += parts[(wave + v) * TN + n][lane];
+    for (int v = 1; v < KS; ++v) acc += parts[wave + v][lane];
   }
   if (l16 >= t.count) return;
   // lane l of a 16 x 16 result has row l % 16 and columns 4 * (l / 16) + 0..3
-  by_output(a, [&](auto to) {
-#pragma unroll
-    for (int n = 0; n < TN; ++n) store4<decltype(to)>(a, t, t.row + l16, col0 + n * 16 + quad * 4, acc[n]);
-  });
+  by_output(a, [&](auto to) { store4<decltype(to)>(a, t, t.row + l16, col0 + quad * 4, acc); });
 }
 
 // TM * 32 rows by 4 * WN * 32 columns of one expert in a workgroup of four waves.  Each wave has every row and its own
@@ -377,13 +363,21 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
       for (int j = 0; j < kParts; ++j) {
         const int m = j / WN, n = j % WN;
         acc[n][m] = Operand<TX>::mfma32(wv[now][n], xv[now][m], acc[n][m]);
-        if (n == WN - 1) read_x(k == 3 ? next : cur, k == 3 ? 0 : k + 1, now ^ 1, m);
-        if (k == 0 && more_x && n == 0)
-          if constexpr (DIRECT) load_x(old, i + 2, m);
-        if ((k == 1 || k == 2) && c == 0 && more_w) {
+        if (j == 0) {
+          // all of the next step's rows at once: with the reads between the products, a product's wait for its own, which
+          // counts from the oldest, took the newest with it
 #pragma unroll
-          for (int l = kW * ((k - 1) * kParts + j) / (2 * kParts); l < kW * ((k - 1) * kParts + j + 1) / (2 * kParts); ++l)
-            load_w(i / 4 + 1, l);
+          for (int q = 0; q < kLive; ++q) read_x(k == 3 ? next : cur, k == 3 ? 0 : k + 1, now ^ 1, q);
+          if constexpr (DIRECT)
+            if (k == 0 && more_x) {
+#pragma unroll
+              for (int q = 0; q < kLive; ++q) load_x(old, i + 2, q);
+            }
+          if ((k == 1 || k == 2) && c == 0 && more_w) {
+#pragma unroll
+            for (int l = 0; l < kW; ++l)
+              if (l * 2 / kW == k - 1) load_w(i / 4 + 1, l);
+          }
         }
         // the next step's weights; a new part's as late as can be, they are being read
         if (j == (k == 3 && c == 3 ? kParts - 1 : (kParts - 1) / 2)) convert(k == 3 ? (c + 1) % 4 : c, (k + 1) % 4, now ^ 1);
@@ -443,12 +437,14 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
   by_output(a, [&](auto to_type) {
     using TO = decltype(to_type);
     constexpr int kSize = ElemInfo<TO>::kBytes;
-    constexpr auto fits = [](int tiles) { return kX / (32 * (tiles * 32 * kSize + 16)) * 3 >= W; };
-    constexpr int CT = fits(WN) ? WN : 1;  // column tiles at a time
+    // column tiles at a time: where there are two, they fit where the wave's weights were
+    constexpr int CT = WN;
     constexpr int kPitch = CT * 32 * kSize + 16;  // 16 bytes more: the 32 rows start in different banks
     constexpr int kPerStage = kX / (32 * kPitch);
-    static_assert(kPerStage * 3 >= W, "the stages hold the results");
-    uint8_t* mine = (wave / kPerStage == 0 ? rows0 : wave / kPerStage == 1 ? rows1 : rows2) + wave % kPerStage * (32 * kPitch);
+    static_assert(WN == 2 ? 32 * kPitch <= (int)sizeof(weights[0]) : kPerStage * 3 >= W, "the buffers hold the results");
+    uint8_t* mine = WN == 2 ? weights[wave]
+                            : (wave / kPerStage == 0 ? rows0 : wave / kPerStage == 1 ? rows1 : rows2) +
+                                  wave % kPerStage * (32 * kPitch);
 #pragma unroll
     for (int m = 0; m < TM; ++m) {
       const int first = m * 32;
@@ -569,10 +565,10 @@ using namespace fmoe;
 
 namespace {
 
-template <typename TX, int W, int TN, int KS, int BYTES, int CPOL> int launch_few(const char* who, Fp4Args a, hipStream_t s) {
-  const int64_t groups = grid_of(who, &a, 16, 16 * TN * (W / KS), W * kWave);
+template <typename TX, int KS> int launch_few(const char* who, Fp4Args a, hipStream_t s) {
+  const int64_t groups = grid_of(who, &a, 16, 16 * (kFewWaves / KS), kFewWaves * kWave);
   if (groups < 0) return FMOE_ERANGE;
-  hipLaunchKernelGGL((k_fp4_few<TX, W, TN, KS, BYTES, CPOL>), dim3((unsigned)groups), dim3(W * kWave), 0, s, a);
+  hipLaunchKernelGGL((k_fp4_few<TX, KS>), dim3((unsigned)groups), dim3(kFewWaves * kWave), 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
@@ -586,33 +582,53 @@ template <typename TX, int TM, int WN> int launch_tile(const char* who, Fp4Args 
   return fmoe_host::check_launch(who);
 }
 
-// The variant for these sizes, as 1000 * rows + columns of its tile.
-enum Variant { kFew = 16016, k96x128 = 96128, k96x256 = 96256 };
-#ifndef FMOE_FP4_TILE
-#define FMOE_FP4_TILE 0
-#endif
-#ifndef FMOE_FEW
-#define FMOE_FEW 8, 1, 1, 24576, kCPol
-#endif
-#ifndef FMOE_TW
-#define FMOE_TW 3, 2
-#endif
-#ifndef FMOE_TN
-#define FMOE_TN 3, 1
-#endif
-Variant pick(int64_t rows, int64_t E, int64_t N, int64_t K) {
-  if (FMOE_FP4_TILE) return (Variant)FMOE_FP4_TILE;
-  const int64_t per = rows / E;
-  if (per <= 8) return kFew;
-  if (per <= 32) return k96x128;
-  return k96x256;
+// The variant for these sizes, as 1000 * rows + columns of its tile.  `per` is the rows of an expert were the routing even,
+// tiles(bm) the tiles of bm rows that the experts then have, on the average over random routing.  Times in us of
+// E experts' [N, K] at `per` rows each, by variant (16 x 128 / KS with K split over KS of the waves, 96 x 128, 96 x 256):
+//                         16x128  16x64  16x32  16x16  96x128  96x256
+//   1 [2048, 7168]    1    19.1    11.5    8.5    7.2    33.9    48.7
+//                    16    28.4    23.3   17.6   15.0    36.4    52.0
+//                   128    29.8    25.3   24.3   36.1    43.1    71.5
+//   1 [7168, 2048]    1     8.7     7.5    6.6    7.0    14.3    19.3
+//   8 [2048, 7168]    1    22.2    13.6   13.4   16.2    37.4    53.5
+//                     8    28.7    20.4   21.7   30.7    39.4    56.2
+//                    32    47.3    52.9   62.5   90.0    42.8    62.3
+//  64 [256, 2048]     1     8.6     7.6    7.5   10.1    14.6    19.4
+//                    16    11.5    13.2   15.9   23.3    15.4    20.7
+//                    64    25.4    30.1   41.1   65.3    19.1    28.0
+//  16 [4096, 4096]    8    32.3    39.8   54.1   80.2    37.3    40.6
+//                    16    56.3    62.3   82.7  127.7    37.4    40.8
+//                   128     225     308    440    713   102.2    89.7
+// 256 [2048, 2048]    4   111.7   138.2  218.3  380.8   148.7   119.7
+//                     8   124.4   162.5  254.7  439.5   150.4   123.0
+//                    64     471     743   1155   1960   211.4   183.0
+// A wave alone takes 0.55 us for 256 of K, so where there are few workgroups K is split until there are one or two on each
+// CU; each workgroup brings all of its expert's rows, which a split multiplies.  Tiles of 96 rows take over where
+// an expert's rows pass one tile of 16 (8 on the average, 5 where there are many workgroups), unless there are few workgroups
+// even so; 256 columns from where they make more than one workgroup on a CU.
+enum Variant { k16x128 = 16128, k16x64 = 16064, k16x32 = 16032, k16x16 = 16016, k96x128 = 96128, k96x256 = 96256 };
+Variant pick(int64_t rows, int64_t E, int64_t N) {
+  const double per = (double)rows / (double)E;
+  auto tiles = [&](double bm) {
+    const double spread = E > 1 ? 2 * std::sqrt(per) : 0, least = std::ceil(std::max(per - spread, 0.0) / bm);
+    const double more = E > 1 ? std::clamp((per + spread - least * bm) / (2 * spread), 0.0, 1.0) : 0.0;
+    return std::min((double)E * (least + more), (double)rows);
+  };
+  const double few = tiles(16) * (double)((N + 127) / 128), wide = tiles(96) * (double)((N + 255) / 256);
+  if (per <= (few >= 1024 ? 5 : 8) || few <= 280) {
+    return few * 8 <= 256 ? k16x16 : few * 4 <= 256 ? k16x32 : few * 2 <= (per < 3 ? 640 : 384) ? k16x64 : k16x128;
+  }
+  return wide >= 288 && N > 128 ? k96x256 : k96x128;
 }
 
 template <typename TX> int launch_linear(const char* who, const Fp4Args& a, hipStream_t s) {
-  switch (pick(a.rows, a.E, a.N, a.K)) {
-    case k96x128: return launch_tile<TX, FMOE_TN>(who, a, s);
-    case k96x256: return launch_tile<TX, FMOE_TW>(who, a, s);
-    default: return launch_few<TX, FMOE_FEW>(who, a, s);
+  switch (pick(a.rows, a.E, a.N)) {
+    case k16x128: return launch_few<TX, 1>(who, a, s);
+    case k16x64: return launch_few<TX, 2>(who, a, s);
+    case k16x32: return launch_few<TX, 4>(who, a, s);
+    case k16x16: return launch_few<TX, 8>(who, a, s);
+    case k96x128: return launch_tile<TX, 3, 1>(who, a, s);
+    default: return launch_tile<TX, 3, 2>(who, a, s);
   }
 }
 
@@ -676,7 +692,7 @@ extern "C" int fmoe_restore_fp4(const void* d_q, const void* d_scales, int64_t r
 
 extern "C" int64_t fmoe_fp4_linear_tile(int64_t rows, int64_t num_experts, int64_t N, int64_t K) {
   if (rows < 1 || num_experts < 1 || N < 1 || K < 1) return -1;
-  return pick(rows, num_experts, N, K);
+  return pick(rows, num_experts, N);
 }
 
 extern "C" int fmoe_fp4_linear(const void* d_x, int64_t x_row_stride, int64_t x_rows, int x_dtype,

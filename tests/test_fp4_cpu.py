@@ -53,3 +53,14 @@ def test_weight_entry_points_refuse():
     for bad in (dict(rows=1 << 31), dict(cols=1 << 25), dict(rows=1 << 30, cols=1 << 20)):
         assert to(**bad) == _abi.ERANGE and back(**bad) == _abi.ERANGE, bad
     assert to(rows=0, x=None) == _abi.OK and back(rows=0, out=None) == _abi.OK
+
+
+def test_tile_introspection():
+    tile = _abi.lib().fmoe_fp4_linear_tile
+    for bad in ((0, 1, 1, 1), (1, 0, 1, 1), (1, 1, 0, 1), (1, 1, 1, 0)):
+        assert tile(*bad) == -1
+    assert tile(1, 1, 2048, 7168) == 16016 and tile(49152, 64, 2048, 4096) == 96256
+    for rows in (1, 7, 64, 1000, (1 << 31) - 1):
+        for E in (1, 3, 256, 1 << 16):
+            for N in (1, 128, 129, 1 << 24):
+                assert tile(rows, E, N, 128) in (16016, 16032, 16064, 16128, 96128, 96256)

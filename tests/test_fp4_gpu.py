@@ -292,3 +292,24 @@ def test_refusals():
     with pytest.raises(RuntimeError, match="only on the GPU"):
         fm.quantize_weights_fp4(x.cpu())
     assert fm.fp4_linear(x[:0], w, torch.zeros(3, dtype=torch.int64, device=DEV)).shape == (0, 16)
+
+
+def _pick(rows, E, N, K):
+    from fastmoe_amd import _abi
+
+    return _abi.lib().fmoe_fp4_linear_tile(rows, E, N, K)
+
+
+@pytest.mark.parametrize("tile,counts,N,K", [
+    (16016, [1], 33, 700), (16016, [16], 250, 2304), (16016, [30], 130, 1100), (16016, [2], 17, 8192),
+    (16032, [3], 5000, 1500), (16032, [16], 4200, 2600), (16032, [13, 1, 0], 2000, 1024),
+    (16064, [4], 9000 + 5, 700), (16064, [40, 1, 2, 12], 2500, 520), (16064, [16, 16, 15, 1], 2300, 1792),
+    (16128, [1] * 60, 900, 520), (16128, [5, 0, 16, 11] * 6, 1300, 1040), (16128, [100], 5000, 513),
+    (96128, [30] * 40, 900, 512), (96128, [0, 97, 1, 64, 33, 200, 10, 70] * 3, 1050, 1001), (96128, [96, 95, 97, 31] * 8, 500, 832),
+    (96256, [30] * 40, 2900, 320), (96256, [192, 1, 0, 130, 65, 96] * 8, 2300, 768), (96256, [400] * 10, 2049, 65),
+], ids=str)
+def test_every_variant(tile, counts, N, K):
+    E, R = len(counts), sum(counts)
+    assert _pick(R, E, N, K) == tile
+    run(counts, N, K, bias=True, gelu=True)
+    run(counts, N, K, H, F, gather=77, behind=0)
