@@ -55,9 +55,8 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// e^x to 2^-36 for any x (NaN stays): x = n ln 2 + r, |r| <= ln 2 / 2, and the series of e^r up to r^9.
+// e^x to 2^-36 for |x| <= 700 (NaN stays): x = n ln 2 + r, |r| <= ln 2 / 2, and the series of e^r up to r^9.
 __device__ __forceinline__ double exp64(double x) {
-  x = x < -700.0 ? -700.0 : x > 700.0 ? 700.0 : x;
   const double n = __builtin_rint(x * 1.4426950408889634);
   const double r = __builtin_fma(n, -0.69314718055994531, x);  // |n| <= 1010: off by 6e-14 at most
   double p = 1.0 / 362880;
@@ -72,40 +71,75 @@ __device__ __forceinline__ double exp64(double x) {
   p = __builtin_fma(p, r, 1.0);
   return __builtin_ldexp(p, (int)n);
 }
-// 1 / x for a positive normal x: the hardware's estimate and two steps of Newton's.
+// Within +-700, where e^x is neither infinite nor zero; NaN stays.
+__device__ __forceinline__ float bounded700(float x) {
+  return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 700.f), -700.f);
+}
+// e^(l - from) for l <= from, not below e^-700; NaN stays.
+__device__ __forceinline__ double power64(float l, float from) {
+  const double d = (double)l - (double)from;
+  return exp64(d < -700. ? -700. : d);
+}
+// 1 / x for a positive normal x, to 2^-40: the hardware's estimate (2^-22 at least) and one step of Newton's.
 __device__ __forceinline__ double inverse64(double x) {
-  double y = __builtin_amdgcn_rcp(x);
-  y = __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
+  const double y = __builtin_amdgcn_rcp(x);
   return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
 }
+__device__ __forceinline__ double sigmoid64(float l) { return inverse64(1. + exp64(-(double)bounded700(l))); }
 
-// Over the L lanes of a token, L and the lanes' order as the hardware moves them: neighbours, pairs, halves
-// of eight (mirrored, where the quads agree already), halves of a row, rows.
-template <int STEP, typename F> __device__ __forceinline__ uint32_t across(uint32_t v, F&& f) {
-  if constexpr (STEP == 1) return f(v, dpp<0xb1>(v));
-  else if constexpr (STEP == 2) return f(v, dpp<0x4e>(v));
-  else if constexpr (STEP == 4) return f(v, dpp<0x141>(v));
-  else if constexpr (STEP == 8) return f(v, dpp<0x140>(v));
-  else return f(v, (uint32_t)__shfl_xor((int)v, STEP));
+// Over the L lanes of a token, as the hardware moves them: a lane's value and its neighbour's, pairs, halves of eight
+// (mirrored, where the quads agree already), halves of a row; rows and halves of the wave come as both lanes' values.
+struct Both {
+  uint32_t a, b;
+};
+template <int STEP> __device__ __forceinline__ Both across(uint32_t v) {
+  if constexpr (STEP == 1) return {v, dpp<0xb1>(v)};
+  else if constexpr (STEP == 2) return {v, dpp<0x4e>(v)};
+  else if constexpr (STEP == 4) return {v, dpp<0x141>(v)};
+  else if constexpr (STEP == 8) return {v, dpp<0x140>(v)};
+  else if constexpr (STEP == 16) {
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    return {r[0], r[1]};
+  } else {
+    const auto r = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return {r[0], r[1]};
+  }
 }
-template <int L> __device__ __forceinline__ uint32_t token_max(uint32_t v) {
-  auto most = [](uint32_t a, uint32_t b) { return max(a, b); };
-  v = across<1>(v, most);
-  v = across<2>(v, most);
-  if constexpr (L >= 16) v = across<8>(across<4>(v, most), most);
-  if constexpr (L >= 64) v = across<32>(across<16>(v, most), most);
+struct Both64 {
+  double a, b;
+};
+template <int STEP> __device__ __forceinline__ Both64 across(double v) {
+  const uint64_t u = __builtin_bit_cast(uint64_t, v);
+  const Both lo = across<STEP>((uint32_t)u), hi = across<STEP>((uint32_t)(u >> 32));
+  return {__builtin_bit_cast(double, (uint64_t)hi.a << 32 | lo.a), __builtin_bit_cast(double, (uint64_t)hi.b << 32 | lo.b)};
+}
+template <int STEP> __device__ __forceinline__ uint32_t step_max(uint32_t v) {
+  const Both w = across<STEP>(v);
+  return max(w.a, w.b);
+}
+template <int STEP> __device__ __forceinline__ double step_max(double v) {
+  const Both64 w = across<STEP>(v);
+  return __builtin_fmax(w.a, w.b);
+}
+template <int L, typename V> __device__ __forceinline__ V token_max(V v) {
+  v = step_max<2>(step_max<1>(v));
+  if constexpr (L >= 16) v = step_max<8>(step_max<4>(v));
+  if constexpr (L >= 64) v = step_max<32>(step_max<16>(v));
   return v;
+}
+template <int STEP> __device__ __forceinline__ float step_sum(float v) {
+  const Both w = across<STEP>(__float_as_uint(v));
+  return __uint_as_float(w.a) + __uint_as_float(w.b);
+}
+template <int STEP> __device__ __forceinline__ double step_sum(double v) {
+  const Both64 w = across<STEP>(v);
+  return w.a + w.b;
 }
 template <int L, typename V> __device__ __forceinline__ V token_sum(V v) {
-#pragma unroll
-  for (int d = 1; d < L; d *= 2) v += __shfl_xor(v, d);
+  v = step_sum<2>(step_sum<1>(v));
+  if constexpr (L >= 16) v = step_sum<8>(step_sum<4>(v));
+  if constexpr (L >= 64) v = step_sum<32>(step_sum<16>(v));
   return v;
-}
-// The lanes of this token for which `p` holds, lane 0 of them in bit 0.
-template <int L> __device__ __forceinline__ uint64_t token_ballot(bool p, int lane) {
-  const uint64_t b = __ballot(p);
-  if constexpr (L == kWave) return b;
-  else return b >> (lane & ~(L - 1)) & ((uint64_t(1) << L) - 1);
 }
 
 // VPL consecutive experts, of which `count` are there; the others read as zero.
@@ -121,10 +155,40 @@ __device__ __forceinline__ void load_logits(const T* row, int first, int count, 
   }
 }
 
+// A choice with its expert as one whole number below 2^44, in a double: the largest is the highest choice, of equal ones that of
+// the lowest index, and a comparison of two is one instruction.  -1 stands for none.
+constexpr int kIndexes = 4096;
+__device__ __forceinline__ double ranked(uint32_t key, int index) {
+  return __builtin_fma((double)key, (double)kIndexes, (double)(kIndexes - 1 - index));
+}
+__device__ __forceinline__ int rank_index(double r) {  // r + 2^52 has r in its low bits
+  return kIndexes - 1 - (int)(__builtin_bit_cast(uint64_t, r + 4503599627370496.0) & (kIndexes - 1));
+}
+__device__ __forceinline__ uint32_t rank_key(double r) { return (uint32_t)(r * (1.0 / kIndexes)); }
+
+// Falling order, by Batcher's merges of sorted halves (odd-even merge sort).
+template <int N> __device__ __forceinline__ void sort_falling(double* s) {
+#pragma unroll
+  for (int p = 1; p < N; p *= 2)
+#pragma unroll
+    for (int k = p; k >= 1; k /= 2)
+#pragma unroll
+      for (int j = k % p; j + k < N; j += 2 * k)
+#pragma unroll
+        for (int i = 0; i < k; ++i)
+          if (i + j + k < N && (i + j) / (2 * p) == (i + j + k) / (2 * p)) {
+            const double x = s[i + j], y = s[i + j + k];
+            s[i + j] = __builtin_fmax(x, y);
+            s[i + j + k] = __builtin_fmin(x, y);
+          }
+}
+
 // A token's experts lie in the registers of L lanes, VPL consecutive ones in each (a group starts in a lane of
-// its own), so that a wave takes 64 / L tokens and a maximum over them is a few register moves.
+// its own), so that a wave takes 64 / L tokens and a maximum over them is a few register moves.  Each lane sorts
+// its own once; then a round takes the highest of the lanes' first ones, and its lane moves the others up.  (Rounds that searched all
+// of a lane's for the highest again took 34 us for 32768 tokens, 256 experts in groups and 8 of them.)
 template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void k_route(RouteArgs a) {
-  __shared__ uint16_t chosen[kGroup / L][kMaxTopK];
+  __shared__ uint16_t chosen[kGroup / L][kMaxTopK];  // where a token's choices pass its lanes
   const int lane = threadIdx.x & (kWave - 1), sub = lane & (L - 1);
   const int slot = threadIdx.x / L;
   const int64_t token = (int64_t)blockIdx.x * (kGroup / L) + slot;
@@ -138,73 +202,52 @@ template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void
   else if (a.dtype == FMOE_BF16)
     load_logits<VPL>(static_cast<const bf16_t*>(a.logits) + at * a.stride, first, count, v);
   else load_logits<VPL>(static_cast<const f16_t*>(a.logits) + at * a.stride, first, count, v);
-  uint32_t key[VPL], best = 0;
-#pragma unroll
-  for (int i = 0; i < VPL; ++i) {
-    key[i] = i < count ? order_key(v[i]) : 0;
-    best = max(best, key[i]);
-  }
   const bool whole = !a.sigmoid && (SCORES || !a.renormalize);  // the softmax over all experts is wanted
   float top = 0.f;
   bool empty = false;  // every expert is masked
   double inv = 0.;     // 1 / the sum of e^(l - top)
   if (whole) {
-    top = key_value(token_max<L>(best));
+    uint32_t high = 0;
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) high = max(high, i < count ? order_key(v[i]) : 0u);
+    top = key_value(token_max<L>(high));
     empty = top == -HUGE_VALF;
     if (empty) top = 0.f;
   }
-  if constexpr (SCORES) {
-    double e[VPL <= 16 ? VPL : 1];
-    auto power = [&](int i) { return i < count && !empty ? exp64((double)v[i] - (double)top) : 0.; };
-    if (whole) {
+  auto power = [&](int i) { return i < count && !empty ? power64(v[i], top) : 0.; };
+  if (whole) {
+    if constexpr (SCORES) {
       double sum = 0.;
 #pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const double p = power(i);
-        if constexpr (VPL <= 16) e[i] = p;
-        sum += p;
-      }
-      sum = token_sum<L>(sum);
-      inv = empty ? 0. : 1. / sum;
-    }
-    best = 0;
+      for (int i = 0; i < VPL; ++i) sum += power(i);
+      inv = empty ? 0. : 1. / token_sum<L>(sum);
+    } else {
+      float sum = 0.f;
 #pragma unroll
-    for (int i = 0; i < VPL; ++i) {
-      if (i < count) {
-        float s;
-        if (a.sigmoid) s = (float)inverse64(1. + exp64(-(double)v[i]));
-        else if constexpr (VPL <= 16) s = (float)(e[i] * inv);
-        else s = (float)(power(i) * inv);
-        key[i] = order_key(a.bias ? s + a.bias[first + i] : s);
-      }
-      best = max(best, key[i]);
+      for (int i = 0; i < VPL; ++i) sum += i < count && !empty ? expf(v[i] - top) : 0.f;
+      inv = empty ? 0. : 1. / (double)token_sum<L>(sum);
     }
-  } else if (whole) {
-    float sum = 0.f;
-#pragma unroll
-    for (int i = 0; i < VPL; ++i) sum += i < count && !empty ? expf(v[i] - top) : 0.f;
-    sum = token_sum<L>(sum);
-    inv = empty ? 0. : 1. / (double)sum;
   }
+  double s[VPL];
+#pragma unroll
+  for (int i = 0; i < VPL; ++i) {
+    float c = v[i];
+    if constexpr (SCORES) {
+      c = a.sigmoid ? (float)sigmoid64(v[i]) : (float)(power(i) * inv);
+      if (a.bias && i < count) c += a.bias[first + i];
+    }
+    s[i] = i < count ? ranked(order_key(c), first + i) : -1.;
+  }
+  sort_falling<VPL>(s);
 
   if (a.top_groups < a.groups) {
-    uint32_t high = best, next = 0;
-    if (a.two) {
-      bool seen = false;  // the highest once, the others compete for the second place
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        const bool it = key[i] == high && !seen;
-        seen |= it;
-        next = max(next, it ? 0u : key[i]);
-      }
-    }
+    double high = s[0], next = VPL > 1 ? s[VPL > 1 ? 1 : 0] : -1.;
     auto join = [&](auto step) {
       constexpr int kStep = decltype(step)::value;
       if (kStep < L && a.group_lanes > kStep) {
-        auto other = [](uint32_t, uint32_t q) { return q; };
-        const uint32_t h = across<kStep>(high, other), n = across<kStep>(next, other);
-        next = max(min(high, h), max(next, n));
-        high = max(high, h);
+        const Both64 h = across<kStep>(high), n = across<kStep>(next);
+        next = __builtin_fmax(__builtin_fmin(h.a, h.b), __builtin_fmax(n.a, n.b));
+        high = __builtin_fmax(h.a, h.b);
       }
     };
     join(std::integral_constant<int, 1>{});
@@ -213,72 +256,77 @@ template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void
     join(std::integral_constant<int, 8>{});
     join(std::integral_constant<int, 16>{});
     join(std::integral_constant<int, 32>{});
-    uint32_t score = g < a.groups ? high : 0;
-    if (a.two && next) score = order_key(key_value(high) + key_value(next));
+    double score = -1.;
+    if (g < a.groups) {
+      uint32_t key = rank_key(high);
+      if (a.two && next >= 0.) key = order_key(key_value(key) + key_value(rank_key(next)));
+      score = ranked(key, g);
+    }
     bool stays = false;
-    for (int r = 0; r < a.top_groups; ++r) {
-      const uint32_t m = token_max<L>(score);
-      const int winner = __ffsll((unsigned long long)token_ballot<L>(score == m, lane)) - 1;
-      if (winner / a.group_lanes == g) {
+    for (int r = 0; r < a.top_groups; ++r)
+      if (score == token_max<L>(score)) {
         stays = true;
-        score = 0;
+        score = -1.;
       }
-    }
-    if (!stays) {
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) key[i] = 0;
-      best = 0;
-    }
+    if (!stays) s[0] = -1.;  // never the highest
   }
 
-  for (int r = 0; r < a.k; ++r) {
-    const uint32_t m = token_max<L>(best);
-    const int winner = __ffsll((unsigned long long)token_ballot<L>(best == m, lane)) - 1;
-    if (sub == winner) {
-      int it = 0;
+  int mine = 0;  // the choice that this lane has: number `sub`
+  auto rounds = [&](auto depth) __attribute__((always_inline)) {
+    constexpr int kDepth = decltype(depth)::value;
+    for (int r = 0; r < a.k; ++r) {
+      const double m = token_max<L>(s[0]);
+      const int id = rank_index(m);
+      if (a.k > L) {
+        if (sub == 0) chosen[slot][r] = (uint16_t)id;
+      } else if (sub == r) mine = id;
+      const bool won = s[0] == m;
 #pragma unroll
-      for (int i = VPL - 1; i >= 0; --i) it = key[i] == m ? i : it;
-      best = 0;
-#pragma unroll
-      for (int i = 0; i < VPL; ++i) {
-        key[i] = i == it ? 0u : key[i];
-        best = max(best, key[i]);
+      for (int i = 0; i < kDepth; ++i) {
+        const double up = i + 1 < VPL ? s[i + 1 < VPL ? i + 1 : 0] : -1.;
+        s[i] = won ? up : s[i];
       }
-      chosen[slot][r] = (uint16_t)(first + it);
     }
+  };
+  if (VPL > 8 && a.k <= 8) rounds(std::integral_constant<int, VPL < 8 ? VPL : 8>{});
+  else rounds(std::integral_constant<int, VPL>{});
+  if (a.k > L) {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's LDS accesses are served in order
+    __builtin_amdgcn_wave_barrier();
+    mine = sub < a.k ? chosen[slot][sub] : 0;
   }
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // a wave's LDS accesses are served in order
-  __builtin_amdgcn_wave_barrier();
 
   auto logit = [&](int id) {
     const int64_t i = at * a.stride + id;
     return load_weight(a.logits, a.dtype, i);
   };
-  // lane `sub` has the chosen sub, sub + L, ...; most tokens have no more than L
-  const int mine = sub < a.k ? chosen[slot][sub] : 0;
+  // lane `sub` has the choices sub, sub + L, ...; most tokens have no more than L
   const float mine_l = logit(mine);
   auto each = [&](auto&& f) {
     if (sub < a.k) f(sub, mine, mine_l);
     for (int j = sub + L; j < a.k; j += L) f(j, (int)chosen[slot][j], logit(chosen[slot][j]));
   };
-  double from = (double)top, over = inv;  // u = e^(l - from) * over, for a sigmoid divided by 1 + e^l too
+  float from = top;  // u = e^(l - from) * over, for a sigmoid divided by 1 + e^l too
+  double over = inv;
   bool none = empty;
   auto unit = [&](float l) {
-    if (!a.sigmoid) return exp64((double)l - from);
-    if (l > 0.f) return inverse64(1. + exp64(-(double)l));
-    return exp64((double)l - from) * inverse64(1. + exp64((double)l));
+    if (!a.sigmoid) return power64(l, from);
+    const double e = exp64(-(double)__builtin_fabsf(bounded700(l)));  // e^-|l|
+    double n = l > 0.f ? 1. : e;
+    if (from != 0.f) n = power64(l, from);
+    return n * inverse64(1. + e);
   };
   if (a.renormalize) {
     uint32_t high = 0;
     each([&](int, int, float l) { high = max(high, order_key(l)); });
     const float m = key_value(token_max<L>(high));
     none = m == -HUGE_VALF;
-    from = none ? 0. : a.sigmoid && m > 0.f ? 0. : (double)m;
+    from = none || (a.sigmoid && m > 0.f) ? 0.f : m;
     double sum = 0.;
     each([&](int, int, float l) { sum += l == -HUGE_VALF ? 0. : unit(l); });
     over = 1. / token_sum<L>(sum);
   } else if (a.sigmoid) {
-    from = 0.;
+    from = 0.f;
     over = 1.;
   }
   if (token >= a.T) return;
@@ -291,7 +339,7 @@ template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void
     else if (a.w_dtype == FMOE_BF16) st1(static_cast<bf16_t*>(a.weights) + i, w);
     else st1(static_cast<f16_t*>(a.weights) + i, w);
     if (a.share) a.share[i] = (float)u;
-    if (a.rest) a.rest[i] = (float)inverse64(1. + exp64((double)l));
+    if (a.rest) a.rest[i] = (float)sigmoid64(-l);
   });
   if (a.norm && sub == 0) {
     a.norm[2 * token] = top;

@@ -43,9 +43,26 @@ template <typename T> __device__ __forceinline__ void load_param(const void* p, 
 template <int THREADS> constexpr int rows_of() { return THREADS < kGroup ? kGroup / THREADS : 1; }
 template <int THREADS> constexpr int threads_of() { return THREADS < kGroup ? kGroup : THREADS; }
 
+// The compiler would keep the converted values over the sums, which takes twice the registers; now it
+// converts them again.
+template <typename R> __device__ __forceinline__ void opaque(R& raw, int words) {
+#pragma unroll
+  for (int i = 0; i < words; ++i) {
+    uint32_t w = raw[i];
+    asm volatile("" : "+v"(w));
+    raw[i] = w;
+  }
+}
+
+// 64 registers, so that two workgroups of 1024 threads share a CU (4096 x 16384: 102 us, one with 74 registers 120).  The
+// others are on a CU often enough as they are, and lose by the spills (4096 x 7168: 48 us, with 64 registers 56).
+template <typename T, int THREADS, int VPT> constexpr bool two_on_a_cu() {
+  return THREADS == 1024 && VPT == 2 && ElemInfo<T>::kBytes == 2;
+}
+
 // A row lies in the registers of THREADS threads, VPT vectors of eight columns each.
 template <typename T, int THREADS, int VPT>
-__global__ __launch_bounds__(threads_of<THREADS>()) void k_sandwich(SandwichArgs a) {
+__global__ __launch_bounds__(threads_of<THREADS>(), (two_on_a_cu<T, THREADS, VPT>() ? 8 : 1)) void k_sandwich(SandwichArgs a) {
   __shared__ float lds[2][16];
   using V = Eight<T>;
   const int64_t row = (int64_t)blockIdx.x * rows_of<THREADS>() + threadIdx.x / THREADS;
@@ -60,7 +77,7 @@ __global__ __launch_bounds__(threads_of<THREADS>()) void k_sandwich(SandwichArgs
     rr[v] = V::template load<true>(r, (v * THREADS + tid) * 8, a.cols);
   }
   const int64_t gate_at = a.gate ? row / a.run * a.cols : 0;
-  float f[VPT][8], w[VPT][8];
+  float w[VPT][8];
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
     load_param<T>(a.post, a.w_dtype, 0, (v * THREADS + tid) * 8, a.cols, w[v]);
@@ -72,37 +89,42 @@ __global__ __launch_bounds__(threads_of<THREADS>()) void k_sandwich(SandwichArgs
   float sum = 0.f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    V::V::cvt(xr[v], f[v]);
+    float f[8];
+    V::V::cvt(xr[v], f);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(f[v][i], f[v][i], sum);
+    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(f[i], f[i], sum);
   }
   const float cx = 1.0f / sqrtf(group_sum<THREADS>(sum, lds[0]) / (float)a.cols + a.eps);
   sum = 0.f;
 #pragma unroll
   for (int v = 0; v < VPT; ++v) {
-    float s[8];
+    float f[8], s[8];
+    opaque(xr[v], V::kWords);
+    V::V::cvt(xr[v], f);
     V::V::cvt(rr[v], s);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(f[v][i] * cx, w[v][i], s[i]);
-    const typename V::raw_t h = V::V::pack(s);
-    V::store(static_cast<T*>(a.h) + row * a.cols, (v * THREADS + tid) * 8, a.cols, h);
-    V::V::cvt(h, f[v]);  // the stream is normalised as it is stored
+    for (int i = 0; i < 8; ++i) s[i] = __builtin_fmaf(f[i] * cx, w[v][i], s[i]);
+    xr[v] = V::V::pack(s);
+    V::store(static_cast<T*>(a.h) + row * a.cols, (v * THREADS + tid) * 8, a.cols, xr[v]);
+    V::V::cvt(xr[v], f);  // the stream is normalised as it is stored
 #pragma unroll
-    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(f[v][i], f[v][i], sum);
+    for (int i = 0; i < 8; ++i) sum = __builtin_fmaf(f[i], f[i], sum);
   }
   if (!a.pre && !a.rstd) return;
   float ch = 0.f;
   if (a.pre) {
-    float p[VPT][8];
 #pragma unroll
-    for (int v = 0; v < VPT; ++v) load_param<T>(a.pre, a.w_dtype, 0, (v * THREADS + tid) * 8, a.cols, p[v]);
+    for (int v = 0; v < VPT; ++v) load_param<T>(a.pre, a.w_dtype, 0, (v * THREADS + tid) * 8, a.cols, w[v]);
     ch = 1.0f / sqrtf(group_sum<THREADS>(sum, lds[1]) / (float)a.cols + a.eps);
     T* y = static_cast<T*>(a.y) + row * a.cols;
 #pragma unroll
     for (int v = 0; v < VPT; ++v) {
+      float f[8];
+      opaque(xr[v], V::kWords);
+      V::V::cvt(xr[v], f);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) f[v][i] = f[v][i] * ch * p[v][i];
-      const typename V::raw_t q = V::V::pack(f[v]);
+      for (int i = 0; i < 8; ++i) f[i] = f[i] * ch * w[v][i];
+      const typename V::raw_t q = V::V::pack(f);
       if (a.stream_y) V::template store<true>(y, (v * THREADS + tid) * 8, a.cols, q);
       else V::store(y, (v * THREADS + tid) * 8, a.cols, q);
     }
@@ -198,17 +220,6 @@ template <int THREADS> __device__ __forceinline__ void group_sum3(float* s, floa
 #pragma unroll
       for (int w = 1; w < THREADS / kWave; ++w) s[i] += lds[i][w];
     }
-  }
-}
-
-// The compiler would keep the converted values over the sums, which takes twice the registers; now it
-// converts them again.
-template <typename R> __device__ __forceinline__ void opaque(R& raw, int words) {
-#pragma unroll
-  for (int i = 0; i < words; ++i) {
-    uint32_t w = raw[i];
-    asm volatile("" : "+v"(w));
-    raw[i] = w;
   }
 }
 
@@ -573,14 +584,18 @@ template <typename F> void by_type(int dtype, F&& f) {
 }
 template <int N> using Int = std::integral_constant<int, N>;
 
-template <typename F> void by_cols(int64_t cols, F&& f) {
+// Calls f(threads, vectors) with the variant that holds a row.  Few rows are given more threads: then a row's
+// latency counts (8 x 7168: 4.8 us with 1024 threads, 5.2 with 512, 6.3 with 256; 4096 x 7168: 52, 48 and 51).
+constexpr int64_t kFewRows = 512;
+template <typename F> void by_cols(int64_t rows, int64_t cols, F&& f) {
   const int64_t v = (cols + 7) / 8;
   if (v <= 64) f(Int<64>{}, Int<1>{});
   else if (v <= 128) f(Int<64>{}, Int<2>{});
   else if (v <= 256) f(Int<64>{}, Int<4>{});
   else if (v <= 512) f(Int<256>{}, Int<2>{});
-  else if (v <= 1024) f(Int<256>{}, Int<4>{});
-  else f(Int<512>{}, Int<4>{});
+  else if (v <= 1024 && rows <= kFewRows) f(Int<1024>{}, Int<1>{});
+  else if (v <= 1024) f(Int<512>{}, Int<2>{});
+  else f(Int<1024>{}, Int<2>{});
 }
 template <typename F> void by_cols_backward(int64_t cols, F&& f) {
   const int64_t v = (cols + 7) / 8;
@@ -661,7 +676,7 @@ extern "C" int fmoe_sandwich_norm(const void* d_x, int64_t x_row_stride, const v
       hipLaunchKernelGGL((k_sandwich_long<T>), dim3((unsigned)rows), dim3(1024), 0, s, a);
       return;
     }
-    by_cols(cols, [&](auto th, auto v) {
+    by_cols(rows, cols, [&](auto th, auto v) {
       constexpr int kT = decltype(th)::value;
       hipLaunchKernelGGL((k_sandwich<T, kT, decltype(v)::value>), grid_of<kT>(rows), dim3(threads_of<kT>()), 0, s, a);
     });
