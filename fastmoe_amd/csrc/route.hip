@@ -55,10 +55,12 @@ __device__ __forceinline__ float key_value(uint32_t key) {
   return __uint_as_float(key & 0x80000000u ? key ^ 0x80000000u : ~key);
 }
 
-// e^x to 2^-36 for |x| <= 700 (NaN stays): x = n ln 2 + r, |r| <= ln 2 / 2, and the series of e^r up to r^9.
-__device__ __forceinline__ double exp64(double x) {
-  const double n = __builtin_rint(x * 1.4426950408889634);
-  const double r = __builtin_fma(n, -0.69314718055994531, x);  // |n| <= 1010: off by 6e-14 at most
+// e^x to 2^-36 for |x| <= 700 (NaN stays), `about` x in fp32: x = n ln 2 + r with |r| below 0.347, the series of e^r up to r^9, and n
+// added to its exponent.  Only what needs 64 bits is in them: rounding, conversions and scaling take two to four times
+// as long there as an fp32 instruction.
+__device__ __forceinline__ double exp64(double x, float about) {
+  const float n = __builtin_rintf(about * 1.44269504f);
+  const double r = __builtin_fma((double)n, -0.69314718055994531, x);  // |n| <= 1010: off by 6e-14 at most
   double p = 1.0 / 362880;
   p = __builtin_fma(p, r, 1.0 / 40320);
   p = __builtin_fma(p, r, 1.0 / 5040);
@@ -69,23 +71,26 @@ __device__ __forceinline__ double exp64(double x) {
   p = __builtin_fma(p, r, 0.5);
   p = __builtin_fma(p, r, 1.0);
   p = __builtin_fma(p, r, 1.0);
-  return __builtin_ldexp(p, (int)n);
+  const uint64_t u = __builtin_bit_cast(uint64_t, p);
+  const uint32_t hi = (uint32_t)(u >> 32) + ((uint32_t)(int)n << 20);
+  return __builtin_bit_cast(double, (uint64_t)hi << 32 | (uint32_t)u);
 }
+__device__ __forceinline__ double exp64(float x) { return exp64((double)x, x); }
 // Within +-700, where e^x is neither infinite nor zero; NaN stays.
 __device__ __forceinline__ float bounded700(float x) {
   return __builtin_elementwise_maximum(__builtin_elementwise_minimum(x, 700.f), -700.f);
 }
 // e^(l - from) for l <= from, not below e^-700; NaN stays.
 __device__ __forceinline__ double power64(float l, float from) {
-  const double d = (double)l - (double)from;
-  return exp64(d < -700. ? -700. : d);
+  const double d = (double)l - (double)from, bounded = d < -700. ? -700. : d;
+  return exp64(bounded, (float)bounded);
 }
 // 1 / x for a positive normal x, to 2^-40: the hardware's estimate (2^-22 at least) and one step of Newton's.
 __device__ __forceinline__ double inverse64(double x) {
   const double y = __builtin_amdgcn_rcp(x);
   return __builtin_fma(__builtin_fma(-x, y, 1.0), y, y);
 }
-__device__ __forceinline__ double sigmoid64(float l) { return inverse64(1. + exp64(-(double)bounded700(l))); }
+__device__ __forceinline__ double sigmoid64(float l) { return inverse64(1. + exp64(-bounded700(l))); }
 
 // Over the L lanes of a token, as the hardware moves them: a lane's value and its neighbour's, pairs, halves of eight
 // (mirrored, where the quads agree already), halves of a row; rows and halves of the wave come as both lanes' values.
@@ -123,7 +128,8 @@ template <int STEP> __device__ __forceinline__ double step_max(double v) {
 }
 template <int L, typename V> __device__ __forceinline__ V token_max(V v) {
   v = step_max<2>(step_max<1>(v));
-  if constexpr (L >= 16) v = step_max<8>(step_max<4>(v));
+  if constexpr (L >= 8) v = step_max<4>(v);
+  if constexpr (L >= 16) v = step_max<8>(v);
   if constexpr (L >= 64) v = step_max<32>(step_max<16>(v));
   return v;
 }
@@ -137,7 +143,8 @@ template <int STEP> __device__ __forceinline__ double step_sum(double v) {
 }
 template <int L, typename V> __device__ __forceinline__ V token_sum(V v) {
   v = step_sum<2>(step_sum<1>(v));
-  if constexpr (L >= 16) v = step_sum<8>(step_sum<4>(v));
+  if constexpr (L >= 8) v = step_sum<4>(v);
+  if constexpr (L >= 16) v = step_sum<8>(v);
   if constexpr (L >= 64) v = step_sum<32>(step_sum<16>(v));
   return v;
 }
@@ -229,12 +236,18 @@ template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void
     }
   }
   double s[VPL];
+  float bias[SCORES ? VPL : 1];
+  if constexpr (SCORES) {
+#pragma unroll
+    for (int i = 0; i < VPL; ++i) bias[i] = 0.f;
+    if (a.bias) load_logits<VPL>(a.bias, first, count, bias);
+  }
 #pragma unroll
   for (int i = 0; i < VPL; ++i) {
     float c = v[i];
     if constexpr (SCORES) {
       c = a.sigmoid ? (float)sigmoid64(v[i]) : (float)(power(i) * inv);
-      if (a.bias && i < count) c += a.bias[first + i];
+      if (a.bias) c += bias[i];
     }
     s[i] = i < count ? ranked(order_key(c), first + i) : -1.;
   }
@@ -311,7 +324,7 @@ template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void
   bool none = empty;
   auto unit = [&](float l) {
     if (!a.sigmoid) return power64(l, from);
-    const double e = exp64(-(double)__builtin_fabsf(bounded700(l)));  // e^-|l|
+    const double e = exp64(-__builtin_fabsf(bounded700(l)));  // e^-|l|
     double n = l > 0.f ? 1. : e;
     if (from != 0.f) n = power64(l, from);
     return n * inverse64(1. + e);
