@@ -7,9 +7,11 @@ from .consts import MoEImplementation
 from .dispatch import PermutedTokens, permute_tokens
 from .fp4 import Fp4Weights, fp4_linear, quantize_weights_fp4
 from .moe import (
+    Fp4MoEFeedForward,
     Int8MoEFeedForward,
     MoEFeedForward,
     NormedMoEFeedForward,
+    SandwichMoEFeedForward,
     compute_experts,
     gate_and_sort,
     unpermute,
@@ -44,6 +46,7 @@ from .routing import RoutedTokens, Routing, route_tokens
 
 __all__ = [
     "CompressedRows",
+    "Fp4MoEFeedForward",
     "Fp4Weights",
     "GroupedMetadata",
     "GroupedWeightedScatterAdd",
@@ -57,6 +60,7 @@ __all__ = [
     "QuantizedRows",
     "RoutedTokens",
     "Routing",
+    "SandwichMoEFeedForward",
     "add_rms_norm",
     "add_rms_norm_int8",
     "compress_rows",

@@ -23,6 +23,13 @@ Beyond the reference, on the 8-bit operators of ``quantize``:
                               the backward (``MoEFeedForward(..., checkpoint="int8")``)
   NormedMoEFeedForward        the layer behind a root-mean-square norm with the residual's addition
   Int8MoEFeedForward          either layer for serving, with rows and experts' weights in 8 bits
+
+and on those of ``routing``, ``fp4`` and ``norms``:
+
+  gate_and_sort(..., routing=Routing(...)), MoEFeedForward(..., routing=...)  scores, groups, a bias for
+                              balance and weights by ``route_tokens`` instead of the reference's rule
+  Fp4MoEFeedForward           the layer for serving, with the experts' weights in 4 bits
+  SandwichMoEFeedForward      the layer between two norms, with a gate and a scale for what it adds
 """
 from __future__ import annotations
 
@@ -34,25 +41,33 @@ import torch.nn.functional as F
 
 from .consts import MoEImplementation
 from .dispatch import PermutedTokens, permute_tokens
+from .fp4 import Fp4Weights, fp4_linear, quantize_weights_fp4
+from .norms import sandwich_norm
 from .ops import (_apply, _combine_forward, _GroupedCombinePermuted, _refuse_autograd_capture,
                   _runs_plain, grouped_weighted_scatter_add)
 from .quantize import (CompressedRows, Int8Weights, _check_matrix, _compress, add_rms_norm,
                        add_rms_norm_int8, gelu_compressed_backward, int8_linear, quantize_rows,
                        quantize_weights, restore_rows)
+from .routing import Routing, route_tokens
 
-__all__ = ["Int8MoEFeedForward", "MoEFeedForward", "NormedMoEFeedForward", "compute_experts",
-           "gate_and_sort", "unpermute"]
+__all__ = ["Fp4MoEFeedForward", "Int8MoEFeedForward", "MoEFeedForward", "NormedMoEFeedForward",
+           "SandwichMoEFeedForward", "compute_experts", "gate_and_sort", "unpermute"]
 
 
-def _route(x_flat: torch.Tensor, router: nn.Module, top_k: int):
-    """(gates in x's type, expert ids), each [T, k] (tiny_model.py:92-100)."""
+def _route(x_flat: torch.Tensor, router: nn.Module, top_k: int, routing: Optional[Routing] = None,
+           bias: Optional[torch.Tensor] = None):
+    """(gates in x's type, expert ids), each [T, k] (tiny_model.py:92-100; ``routing``: by route_tokens)."""
     logits = router(x_flat)
+    if routing is not None:
+        return route_tokens(logits, top_k, routing, bias=bias, out_dtype=x_flat.dtype)
     topk_weights, topk_indices = torch.topk(logits, top_k, dim=-1)
     return F.softmax(topk_weights, dim=-1, dtype=torch.float32).type_as(x_flat), topk_indices
 
 
-def gate_and_sort(x: torch.Tensor, router: nn.Module, top_k: int, num_experts: int):
-    """Routing and permutation of tiny_model.py:79-164 at world size 1.
+def gate_and_sort(x: torch.Tensor, router: nn.Module, top_k: int, num_experts: int, *,
+                  routing: Optional[Routing] = None, bias: Optional[torch.Tensor] = None):
+    """Routing and permutation of tiny_model.py:79-164 at world size 1; with a ``routing``, experts and
+    weights are those of ``route_tokens`` (``bias`` float32 [E], for the choice alone).
 
     Returns ``(permuted_data, rank_counts, expert_counts_by_rank, reverse_map_indices,
     sorted_weights, (B, T))`` like the reference (:160-166): ``rank_counts`` = [T*k] (:158),
@@ -60,7 +75,9 @@ def gate_and_sort(x: torch.Tensor, router: nn.Module, top_k: int, num_experts: i
     """
     B, T, D = x.shape
     x_flat = x.reshape(-1, D)
-    topk_weights, topk_indices = _route(x_flat, router, top_k)
+    if routing is None and bias is not None:
+        raise ValueError("fastmoe_amd: a bias needs a routing")
+    topk_weights, topk_indices = _route(x_flat, router, top_k, routing, bias)
     p = permute_tokens(x_flat, topk_indices, topk_weights, num_experts)
     rank_counts = torch.tensor([p.permuted_data.shape[0]], device=x.device, dtype=torch.long)
     return _Routed((p.permuted_data, rank_counts, p.expert_counts.view(1, num_experts),
@@ -290,16 +307,40 @@ def unpermute(x_out: Union[torch.Tensor, Sequence[torch.Tensor]], reverse_map_in
     raise NotImplementedError(impl)
 
 
-class MoEFeedForward(nn.Module):
+class _Balanced(nn.Module):
+    """A layer whose ``balance_bias`` (float32 [E], or None) stays float32 when the layer is cast: steps of
+    1e-3 and less would be lost in 16 bits."""
+
+    def _apply(self, fn, recurse=True):
+        bias = self._buffers.get("balance_bias")
+        super()._apply(fn, recurse)
+        if bias is not None:
+            moved = self._buffers["balance_bias"]
+            if moved.dtype != torch.float32:
+                self._buffers["balance_bias"] = bias.to(moved.device)
+        return self
+
+
+class MoEFeedForward(_Balanced):
     """MoE feed-forward layer of tiny_model.py:42-77 on one GPU: router, E experts
     (Linear -> GELU -> Linear), HIP permutation, per-expert compute, grouped combine.
 
     ``checkpoint="int8"`` holds the experts' activations in 8 bits until the backward (see
-    ``compute_experts``); :meth:`int8` makes the layer that serves with 8-bit rows and weights."""
+    ``compute_experts``); :meth:`int8` makes the layer that serves with 8-bit rows and weights, :meth:`fp4`
+    the one with 4-bit weights.
+
+    ``routing``: how experts are chosen and weighed (``route_tokens``) instead of the reference's rule.
+    ``balance=True`` (with a routing) adds ``balance_bias`` to the scores that choose; in training mode the
+    layer counts the rows that each expert gets in ``expert_load``, and :meth:`update_balance`, called
+    after the optimiser's step, moves the bias against it."""
 
     def __init__(self, dim: int, ff_dim: int, num_experts: int, top_k: int,
-                 implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None) -> None:
+                 implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None,
+                 routing: Optional[Routing] = None, balance: bool = False) -> None:
         super().__init__()
+        if balance and routing is None:
+            raise ValueError("fastmoe_amd: balance needs a routing")
+        self.routing = routing
         if checkpoint not in (None, "int8"):
             raise ValueError(f"fastmoe_amd: unknown checkpoint {checkpoint!r} (expected None or "
                              "'int8')")
@@ -312,10 +353,26 @@ class MoEFeedForward(nn.Module):
         self.experts = nn.ModuleList(
             [nn.Sequential(nn.Linear(dim, ff_dim, bias=False), nn.GELU(),
                            nn.Linear(ff_dim, dim, bias=False)) for _ in range(num_experts)])
+        self.register_buffer("balance_bias", torch.zeros(num_experts) if balance else None)
+        self.register_buffer("expert_load", torch.zeros(num_experts, dtype=torch.int64) if balance else None,
+                             persistent=False)
+
+    @torch.no_grad()
+    def update_balance(self, rate: float = 1e-3) -> None:
+        """``balance_bias += rate * sign(mean load - load)`` of the rows counted since the last call, which
+        are forgotten."""
+        if self.balance_bias is None:
+            raise ValueError("fastmoe_amd: the layer was made without balance")
+        load = self.expert_load.double()
+        self.balance_bias.add_((rate * torch.sign(load.mean() - load)).float())
+        self.expert_load.zero_()
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
-        routed = gate_and_sort(x, self.router, self.top_k, self.num_experts)
+        routed = gate_and_sort(x, self.router, self.top_k, self.num_experts, routing=self.routing,
+                               bias=self.balance_bias)
         permuted, _, counts_by_rank, rev, weights, shape = routed
+        if self.training and self.balance_bias is not None:
+            self.expert_load.add_(counts_by_rank.view(-1))
         # the split sizes go to the host, as in the reference (recv_splits .tolist(), :197-207)
         tokens_per_expert = counts_by_rank.view(-1).tolist()
         outs = compute_experts(self.experts, permuted, tokens_per_expert,
@@ -330,6 +387,10 @@ class MoEFeedForward(nn.Module):
         do not reach it).  A layer with hooks, or a subclass with a forward of its own, is refused: what
         they add would be lost."""
         return Int8MoEFeedForward(self)
+
+    def fp4(self) -> "Fp4MoEFeedForward":
+        """As :meth:`int8`, with the experts' weights in 4 bits and the rows as they are."""
+        return Fp4MoEFeedForward(self)
 
 
 def _check_residual(x: torch.Tensor, residual: Optional[torch.Tensor]) -> None:
@@ -362,8 +423,116 @@ class NormedMoEFeedForward(nn.Module):
         _check_layer(self, NormedMoEFeedForward)
         return Int8MoEFeedForward(self.moe, self.norm_weight, self.eps)
 
+    def fp4(self) -> "NormedMoEFeedForward":
+        """As :meth:`MoEFeedForward.fp4`, behind a copy of the norm."""
+        _check_layer(self, NormedMoEFeedForward)
+        block = NormedMoEFeedForward(self.moe.fp4(), self.eps)
+        block.load_state_dict({"norm_weight": self.norm_weight}, strict=False)
+        return block.requires_grad_(False)
 
-class Int8MoEFeedForward(nn.Module):
+
+class SandwichMoEFeedForward(nn.Module):
+    """A layer between two norms: ``h = stream + scale * gate * rms(moe(rms(stream) * norm_weight)) *
+    post_weight``, where ``rms(v) = v / sqrt(mean(v^2) + eps)`` (``sandwich_norm``).
+
+    ``forward(stream, normed=None, gate=None, next_weight=None)`` returns ``(h, y)``: ``y = rms(h) *
+    next_weight`` is what the next block's layer reads, made in the same pass, and the next call's
+    ``normed`` (None without ``next_weight``).  ``gate``: [dim], or [batch, dim] with one for each sequence;
+    ``gated=True`` adds a parameter ``gate`` [dim], ones at first, for calls that give none.  ``moe``: a
+    :class:`MoEFeedForward`, or one of its serving forms without a norm."""
+
+    def __init__(self, moe: nn.Module, eps: float = 1e-6, scale: float = 1.0, gated: bool = False) -> None:
+        super().__init__()
+        self.moe, self.eps, self.scale = moe, eps, scale
+        like = dict(dtype=moe.router.weight.dtype, device=moe.router.weight.device)
+        self.norm_weight = nn.Parameter(torch.ones(moe.dim, **like))
+        self.post_weight = nn.Parameter(torch.ones(moe.dim, **like))
+        self.gate = nn.Parameter(torch.ones(moe.dim, **like)) if gated else None
+
+    def forward(self, stream: torch.Tensor, normed: Optional[torch.Tensor] = None,
+                gate: Optional[torch.Tensor] = None, next_weight: Optional[torch.Tensor] = None):
+        D = stream.shape[-1]
+        flat = stream.reshape(-1, D)
+        if normed is None:
+            normed = add_rms_norm(flat, self.norm_weight, eps=self.eps)[0]
+        else:
+            _check_residual(stream, normed)
+        gate = self.gate if gate is None else gate
+        if gate is not None and gate.dim() > 1 and gate.shape[0] != stream.shape[0]:
+            raise ValueError(f"fastmoe_amd: gate must be [{D}] or [{stream.shape[0]}, {D}], got "
+                             f"{tuple(gate.shape)}")
+        out = self.moe(normed.reshape(stream.shape)).reshape(-1, D)
+        y, h = sandwich_norm(out, self.post_weight, flat, next_weight, gate=gate, scale=self.scale, eps=self.eps)
+        return h.view(stream.shape), None if y is None else y.view(stream.shape)
+
+    def fp4(self) -> "SandwichMoEFeedForward":
+        """This block for serving: a copy with the experts' weights in 4 bits."""
+        _check_layer(self, SandwichMoEFeedForward)
+        block = SandwichMoEFeedForward(self.moe.fp4(), self.eps, self.scale, self.gate is not None)
+        own = {n: p for n, p in self.named_parameters(recurse=False)}
+        block.load_state_dict(own, strict=False)
+        return block.requires_grad_(False)
+
+
+class Fp4MoEFeedForward(_Balanced):
+    """An MoE layer for serving with the experts' weights in 4 bits, a scale for 32 of them (Linear -> GELU ->
+    Linear, biases in their own type), and 16-bit rows.  Made by :meth:`MoEFeedForward.fp4` (or those of
+    the layers around it).
+
+    ``forward(x)`` returns the layer's output.  The experts' first product reads each token's row
+    through the reverse map and applies GELU: no [T*k, D] copy of the rows is made.  The host reads
+    nothing back, so a call can be captured in a HIP graph.  No gradients.
+    """
+
+    def __init__(self, moe: MoEFeedForward) -> None:
+        super().__init__()
+        _check_layer(moe, MoEFeedForward)
+        params = _mlp_parameters(moe.experts)
+        if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
+            raise TypeError("fastmoe_amd: the router is not a Linear without hooks")
+        if moe.router.weight.dtype not in (torch.bfloat16, torch.float16):
+            raise TypeError(f"fastmoe_amd: the 4-bit layer's rows are bfloat16 or float16; this one is "
+                            f"{moe.router.weight.dtype}")
+        self.dim, self.num_experts, self.top_k = moe.dim, moe.num_experts, moe.top_k
+        self.routing = moe.routing
+        self.hidden = params[0][0].shape[0]
+        self.router = nn.Linear(moe.dim, moe.num_experts, bias=moe.router.bias is not None,
+                                dtype=moe.router.weight.dtype, device=moe.router.weight.device)
+        self.router.load_state_dict(moe.router.state_dict())
+        self.router.requires_grad_(False)
+
+        def keep(name, t):
+            self.register_buffer(name, None if t is None else t.detach().clone())
+
+        keep("balance_bias", moe.balance_bias)
+        for i, name in ((0, "1"), (2, "2")):
+            w = quantize_weights_fp4([p[i] for p in params])
+            self.register_buffer("w" + name, w.data)
+            self.register_buffer("s" + name, w.scales)
+            biases = [p[i + 1] for p in params]
+            if any((b is None) != (biases[0] is None) for b in biases):
+                raise ValueError("fastmoe_amd: some experts have biases and some have none")
+            keep("b" + name, None if biases[0] is None else torch.stack([b.detach() for b in biases]))
+
+    @torch.no_grad()
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        if x.dim() != 3 or x.shape[2] != self.dim:
+            raise ValueError(f"fastmoe_amd: x must be [batch, tokens, {self.dim}], got "
+                             f"{tuple(x.shape)}")
+        B, T, D = x.shape
+        flat = x.reshape(-1, D)
+        if flat.shape[0] == 0:
+            return x.new_empty(x.shape)
+        gates, ids = _route(flat, self.router, self.top_k, self.routing, self.balance_bias)
+        # the sort alone: what it gathers is one column
+        p = permute_tokens(flat[:, :1], ids, gates, self.num_experts)
+        h = fp4_linear(flat, Fp4Weights(self.w1, self.s1, D), p.expert_offsets, rows=p.reverse_map_indices,
+                       bias=self.b1, activation="gelu")
+        h = fp4_linear(h, Fp4Weights(self.w2, self.s2, self.hidden), p.expert_offsets, bias=self.b2)
+        return unpermute(h, p.reverse_map_indices, p.sorted_weights, (B, T), permutation=p)
+
+
+class Int8MoEFeedForward(_Balanced):
     """An MoE layer for serving in 8 bits: rows with one scale each, experts' weights with one scale for
     each output (Linear -> GELU -> Linear, biases in their own type).  Made by
     :meth:`MoEFeedForward.int8` or :meth:`NormedMoEFeedForward.int8`.
@@ -384,6 +553,7 @@ class Int8MoEFeedForward(nn.Module):
         if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
             raise TypeError("fastmoe_amd: the router is not a Linear without hooks")
         self.dim, self.num_experts, self.top_k, self.eps = moe.dim, moe.num_experts, moe.top_k, eps
+        self.routing = moe.routing
         self.hidden = params[0][0].shape[0]
         self.router = nn.Linear(moe.dim, moe.num_experts, bias=moe.router.bias is not None,
                                 dtype=moe.router.weight.dtype, device=moe.router.weight.device)
@@ -394,6 +564,7 @@ class Int8MoEFeedForward(nn.Module):
             self.register_buffer(name, None if t is None else t.detach().clone())
 
         keep("norm_weight", norm_weight)
+        keep("balance_bias", moe.balance_bias)
         for i, name in ((0, "1"), (2, "2")):
             w = quantize_weights([p[i] for p in params])
             self.register_buffer("w" + name, w.data)
@@ -422,7 +593,7 @@ class Int8MoEFeedForward(nn.Module):
         if flat.shape[0] == 0:
             out = x.new_empty(x.shape)
         else:
-            gates, ids = _route(y, self.router, self.top_k)
+            gates, ids = _route(y, self.router, self.top_k, self.routing, self.balance_bias)
             # the sort alone: what it gathers are the rows' scales, four bytes each
             p = permute_tokens(rows.scales.view(-1, 1), ids, gates, self.num_experts)
             h = int8_linear(rows, Int8Weights(self.w1, self.s1, D), p.expert_offsets,
