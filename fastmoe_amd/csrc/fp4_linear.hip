@@ -111,7 +111,8 @@ template <typename F> __device__ __forceinline__ void by_output(const Fp4Args& a
 // Few rows: up to 16, by 16 columns for each of a workgroup's eight waves, or for each KS of them, which then take pieces
 // of 256 of K in turn and add their parts in LDS in one order.  A wave brings its own weights through a ring of three buffers in
 // LDS, eight lanes for the 128 bytes of a column's piece: whole lines.  (Straight to the matrix units' registers, where
-// neighbouring lanes have different columns, they came at 3.1 TB/s, whatever the waves and pieces in flight; so at 5.)
+// neighbouring lanes have different columns, they came at 3.1 TB/s, whatever the waves and pieces in flight.)  256 experts'
+// [2048, 2048] (570 MB) at 4 rows each take 122 us: 4.7 TB/s.
 // The rows lie in LDS, as much of K at a time as fits.  No wave waits for another but where the next part of the rows comes.
 constexpr int kFewWaves = 8;
 // Bytes of LDS for rows: at least a round of all waves' pieces of 16 rows; where K is split over one or two, two workgroups
@@ -236,7 +237,13 @@ template <typename TX, int KS> __global__ __launch_bounds__(kFewWaves * kWave) v
 // In LDS a row's piece and a column's codes are 128 bytes each, their 16-byte chunk c at position c ^ swizzle: what a read's
 // lanes touch together then lies in different banks.  Lane l of a matrix unit's operand has row (column) l % 32, and of
 // a piece's K the half l / 32: four steps of 8, a chunk of codes for all four.
-template <typename TX, int TM, int WN, bool DIRECT>
+//
+// Many rows are bound by the matrix units at the clock that they leave: 49152 rows of 64 experts' [2048, 4096] in 715 us are 1.15
+// PFLOP/s, about two thirds of their cycles at 1.7 GHz (a large product of the library's: 1.38).
+//
+// Weights that one tile of rows reads pass the caches; where more of an expert's tiles read them (AGAIN), they stay: at 128 experts'
+// [2048, 7168] 128 rows each take 574 us instead of 607, 768 rows 2460 instead of 2690, but 64 rows 323 instead of 308.
+template <typename TX, int TM, int WN, bool DIRECT, bool AGAIN>
 __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
   constexpr int W = 4, BM = TM * 32, BN = W * WN * 32;
   constexpr int kX = BM * 128, kCodes = WN * 32 * 128, kW = WN * 5;  // loads of a wave for 256 of K of its columns
@@ -269,7 +276,7 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
     if (i < 4 * WN) {
       const int chunk = (lane % 8) ^ swizzle<128>(i * 8 + lane / 8);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(codes_at, (FMOE_LDS void*)(weights[wave] + i * 1024), 16,
-                                               code_from + chunk * 16, i * 8 * code_pitch + s * 128, 0, kCPol);
+                                               code_from + chunk * 16, i * 8 * code_pitch + s * 128, 0, AGAIN ? kCPolCached : kCPol);
     } else {
       const int n = i - 4 * WN;
       __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_at, (FMOE_LDS void*)(weights[wave] + kCodes + n * 256), 4, scale_from,
@@ -572,13 +579,13 @@ template <typename TX, int KS> int launch_few(const char* who, Fp4Args a, hipStr
   return fmoe_host::check_launch(who);
 }
 
-template <typename TX, int TM, int WN> int launch_tile(const char* who, Fp4Args a, hipStream_t s) {
+template <typename TX, int TM, int WN, bool AGAIN> int launch_tile(const char* who, Fp4Args a, hipStream_t s) {
   const int64_t groups = grid_of(who, &a, TM * 32, WN * 128, 4 * kWave);
   if (groups < 0) return FMOE_ERANGE;
   const bool direct = a.K % 64 == 0 && a.x_stride % 8 == 0 && reinterpret_cast<uintptr_t>(a.x) % 16 == 0;
   const dim3 grid((unsigned)groups), block(4 * kWave);
-  if (direct) hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, true>), grid, block, 0, s, a);
-  else hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, false>), grid, block, 0, s, a);
+  if (direct) hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, true, AGAIN>), grid, block, 0, s, a);
+  else hipLaunchKernelGGL((k_fp4_tile<TX, TM, WN, false, AGAIN>), grid, block, 0, s, a);
   return fmoe_host::check_launch(who);
 }
 
@@ -586,26 +593,29 @@ template <typename TX, int TM, int WN> int launch_tile(const char* who, Fp4Args 
 // tiles(bm) the tiles of bm rows that the experts then have, on the average over random routing.  Times in us of
 // E experts' [N, K] at `per` rows each, by variant (16 x 128 / KS with K split over KS of the waves, 96 x 128, 96 x 256):
 //                         16x128  16x64  16x32  16x16  96x128  96x256
-//   1 [2048, 7168]    1    19.1    11.5    8.5    7.2    33.9    48.7
-//                    16    28.4    23.3   17.6   15.0    36.4    52.0
-//                   128    29.8    25.3   24.3   36.1    43.1    71.5
-//   1 [7168, 2048]    1     8.7     7.5    6.6    7.0    14.3    19.3
-//   8 [2048, 7168]    1    22.2    13.6   13.4   16.2    37.4    53.5
-//                     8    28.7    20.4   21.7   30.7    39.4    56.2
-//                    32    47.3    52.9   62.5   90.0    42.8    62.3
-//  64 [256, 2048]     1     8.6     7.6    7.5   10.1    14.6    19.4
-//                    16    11.5    13.2   15.9   23.3    15.4    20.7
-//                    64    25.4    30.1   41.1   65.3    19.1    28.0
-//  16 [4096, 4096]    8    32.3    39.8   54.1   80.2    37.3    40.6
-//                    16    56.3    62.3   82.7  127.7    37.4    40.8
-//                   128     225     308    440    713   102.2    89.7
-// 256 [2048, 2048]    4   111.7   138.2  218.3  380.8   148.7   119.7
-//                     8   124.4   162.5  254.7  439.5   150.4   123.0
-//                    64     471     743   1155   1960   211.4   183.0
+//   1 [2048, 7168]    1    18.5    11.5     8.4    7.0    34.1    47.8
+//                    16    27.9    23.6    17.8   14.9    36.0    51.4
+//                    64    27.8    23.8    19.2   29.1    41.2    60.6
+//   1 [7168, 2048]    1     8.3     7.5     6.6    9.4    14.8    19.2
+//   8 [2048, 7168]    1    21.7    13.7    17.0   21.2    37.6    53.8
+//                     8    28.6    20.5    32.5   48.9    39.2    56.4
+//                    16    30.9    33.5    50.8   79.7    39.5    56.7
+//                    32    46.8    52.8    90.8    142    43.1    62.7
+//  64 [256, 2048]     1     8.5     7.2    10.5   14.6    15.2    19.2
+//                    16    11.3    12.9    21.7   36.4    15.3    20.5
+//                    64    25.3    30.1    66.5    110    19.2    28.3
+//  16 [4096, 4096]    8    31.6    38.9    81.4    129    35.2    40.5
+//                    16    55.1    62.2     133    220    36.1    40.7
+//                   128     223     309     733   1208    97.2    82.4
+//  32 [7168, 2048]    8    55.4    72.2     179    319    70.8    59.0
+//                    16    83.6     118     302    524    71.3    61.3
+// 256 [2048, 2048]    4     122     146     340    610     153     128
+//                     8     126     163     420    731     153     123
+//                    64     469     746    1964   3402     203     182
 // A wave alone takes 0.55 us for 256 of K, so where there are few workgroups K is split until there are one or two on each
 // CU; each workgroup brings all of its expert's rows, which a split multiplies.  Tiles of 96 rows take over where
-// an expert's rows pass one tile of 16 (8 on the average, 5 where there are many workgroups), unless there are few workgroups
-// even so; 256 columns from where they make more than one workgroup on a CU.
+// an expert's rows pass one tile of 16 (8 on the average), unless there are few workgroups even so; 256 columns from where
+// they make more than one workgroup on a CU.
 enum Variant { k16x128 = 16128, k16x64 = 16064, k16x32 = 16032, k16x16 = 16016, k96x128 = 96128, k96x256 = 96256 };
 Variant pick(int64_t rows, int64_t E, int64_t N) {
   const double per = (double)rows / (double)E;
@@ -615,8 +625,8 @@ Variant pick(int64_t rows, int64_t E, int64_t N) {
     return std::min((double)E * (least + more), (double)rows);
   };
   const double few = tiles(16) * (double)((N + 127) / 128), wide = tiles(96) * (double)((N + 255) / 256);
-  if (per <= (few >= 1024 ? 5 : 8) || few <= 280) {
-    return few * 8 <= 256 ? k16x16 : few * 4 <= 256 ? k16x32 : few * 2 <= (per < 3 ? 640 : 384) ? k16x64 : k16x128;
+  if (per <= 8 || few <= 280) {
+    return few * 8 <= 256 ? k16x16 : few * 4 <= 256 ? k16x32 : few * 2 <= (per < 3 ? 640 : 300) ? k16x64 : k16x128;
   }
   return wide >= 288 && N > 128 ? k96x256 : k96x128;
 }
@@ -627,8 +637,10 @@ template <typename TX> int launch_linear(const char* who, const Fp4Args& a, hipS
     case k16x64: return launch_few<TX, 2>(who, a, s);
     case k16x32: return launch_few<TX, 4>(who, a, s);
     case k16x16: return launch_few<TX, 8>(who, a, s);
-    case k96x128: return launch_tile<TX, 3, 1>(who, a, s);
-    default: return launch_tile<TX, 3, 2>(who, a, s);
+    case k96x128: return launch_tile<TX, 3, 1, false>(who, a, s);
+    default:
+      // more than a tile's rows for many of the experts
+      return a.rows > 80 * a.E ? launch_tile<TX, 3, 2, true>(who, a, s) : launch_tile<TX, 3, 2, false>(who, a, s);
   }
 }
 

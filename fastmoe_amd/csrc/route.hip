@@ -193,7 +193,8 @@ template <int N> __device__ __forceinline__ void sort_falling(double* s) {
 // A token's experts lie in the registers of L lanes, VPL consecutive ones in each (a group starts in a lane of
 // its own), so that a wave takes 64 / L tokens and a maximum over them is a few register moves.  Each lane sorts
 // its own once; then a round takes the highest of the lanes' first ones, and its lane moves the others up.  (Rounds that searched all
-// of a lane's for the highest again took 34 us for 32768 tokens, 256 experts in groups and 8 of them.)
+// of a lane's for the highest again took 34 us for 32768 tokens, 256 experts in groups and 8 of them; so 26.6, with the vector
+// units two thirds busy: sums, sorts and 64-bit scores bound it, not the 37 MB.)
 template <int VPL, int L, bool SCORES> __global__ __launch_bounds__(kGroup) void k_route(RouteArgs a) {
   __shared__ uint16_t chosen[kGroup / L][kMaxTopK];  // where a token's choices pass its lanes
   const int lane = threadIdx.x & (kWave - 1), sub = lane & (L - 1);
@@ -374,7 +375,8 @@ struct RouteBwdArgs {
 };
 
 // Eight columns of a token's row in a lane at a time, each row written once.  Every lane reads the token's k
-// gradients itself: they come from the cache, and no lane waits for another.
+// gradients itself: they come from the cache, and no lane waits for another.  32768 tokens,
+// 6 of 64 experts, bf16, take 8 us, half of it a launch's.
 template <typename T> __global__ __launch_bounds__(kGroup) void k_route_bwd(RouteBwdArgs a) {
   const int64_t token = ((int64_t)blockIdx.x * kGroup + threadIdx.x) / a.lanes;
   const int sub = threadIdx.x & (a.lanes - 1);
@@ -479,8 +481,13 @@ extern "C" int fmoe_route(const void* d_logits, int64_t row_stride, int64_t num_
     return a.group_lanes * a.groups;
   };
   hipStream_t s = static_cast<hipStream_t>(stream);
-  if (T <= 4096 && lanes(4) <= 64) {
-    if (lanes(4) <= 16) launch_route<4, 16>(a, scores, s);
+  // Four experts in a lane make short waves, sixteen fewer of them: 256 experts in 8 groups take 5.6 us instead of 6.8 with 8
+  // tokens, 7.4 instead of 7.6 with 2048, 10.4 instead of 7.7 with 4096; 64 experts 3.5 instead of 5.4 with 8 tokens, 4.4
+  // instead of 5.9 with 8192, 5.6 instead of 6.1 with 16384.  128 experts would leave half of the lanes idle: 4.3 instead of
+  // 4.3 with 8 tokens, 5.4 instead of 4.8 with 2048.
+  const int few = lanes(4), few_l = few <= 16 ? 16 : 64;
+  if ((few <= 16 || few == 64) && T * few_l <= (1 << 17)) {
+    if (few <= 16) launch_route<4, 16>(a, scores, s);
     else launch_route<4, 64>(a, scores, s);
   } else if (lanes(16) <= 4) launch_route<16, 4>(a, scores, s);
   else if (lanes(16) <= 16) launch_route<16, 16>(a, scores, s);

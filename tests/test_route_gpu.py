@@ -52,7 +52,8 @@ SIZES = [  # T, E, k, groups, top_groups
     (1, 1, 1, 1, 1), (1, 8, 2, 1, 1), (3, 7, 7, 1, 1), (130, 64, 6, 1, 1), (5000, 64, 6, 1, 1),
     (5001, 60, 5, 6, 3), (65, 60, 5, 6, 3), (4100, 256, 8, 8, 4), (9, 256, 8, 8, 4), (17, 333, 9, 1, 1),
     (5, 1024, 64, 1, 1), (4099, 1023, 3, 3, 2), (6, 4096, 8, 1, 1), (3, 4001, 33, 1, 1), (7, 64, 4, 64, 5),
-    (21, 1024, 16, 64, 4), (4097, 1024, 4, 5 - 1, 2), (11, 48, 3, 2, 2), (2, 130, 64, 2, 1), (4098, 3, 2, 3, 2)]
+    (21, 1024, 16, 64, 4), (4097, 1024, 4, 5 - 1, 2), (11, 48, 3, 2, 2), (2, 130, 64, 2, 1), (4098, 3, 2, 3, 2),
+    (8193, 64, 6, 1, 1), (8192, 61, 3, 1, 1), (2049, 256, 8, 8, 4), (2048, 256, 5, 1, 1), (2050, 192, 6, 3, 2)]
 
 
 @pytest.mark.parametrize("dtype", TYPES, ids=str)
