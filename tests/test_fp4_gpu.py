@@ -313,3 +313,17 @@ def test_every_variant(tile, counts, N, K):
     assert _pick(R, E, N, K) == tile
     run(counts, N, K, bias=True, gelu=True)
     run(counts, N, K, H, F, gather=77, behind=0)
+
+
+@pytest.mark.parametrize("K", [1, 5, 8, 9, 63, 66, 68, 71, 130, 189, 255])
+@pytest.mark.parametrize("tile,counts,N", [
+    (96128, [0, 97, 1, 64, 33, 200, 10, 70] * 3, 700), (96256, [30] * 40, 2900), (96256, [400, 90, 101, 0] * 10, 2049)], ids=str)
+def test_rows_whose_last_piece_is_not_whole(tile, counts, N, K):
+    assert _pick(sum(counts), len(counts), N, K) == tile
+    run(counts, N, K, H if K % 2 else B, gather=50 if K % 3 else None)
+
+
+@pytest.mark.parametrize("per", [79, 80, 81])
+def test_rows_about_where_weights_stay_in_the_caches(per):
+    assert _pick(per * 24, 24, 4096, 192) == 96256
+    run([per] * 24, 4096, 192, bias=True)
