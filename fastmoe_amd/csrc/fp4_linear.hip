@@ -251,7 +251,7 @@ __device__ __forceinline__ u32x4 without(u32x4 v, int n) {
 // a piece's K the half l / 32: four steps of 8, a chunk of codes for all four.
 //
 // Many rows are bound by the matrix units at the clock that they leave: 49152 rows of 64 experts' [2048, 4096] in 715 us are 1.15
-// PFLOP/s, about two thirds of their cycles at 1.7 GHz (a large product of the library's: 1.38).
+// PFLOP/s, 63 % of their cycles at 1.95 GHz (a large product of the library's: 1.38).
 //
 // Weights that one tile of rows reads pass the caches; where more of an expert's tiles read them (AGAIN), they stay: at 128 experts'
 // [2048, 7168] 128 rows each take 574 us instead of 607, 768 rows 2460 instead of 2690, but 64 rows 323 instead of 308.

@@ -21,6 +21,7 @@
 #include "rows8.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace fmoe {
 
@@ -468,6 +469,7 @@ extern "C" int fmoe_route(const void* d_logits, int64_t row_stride, int64_t num_
     return FMOE_ERANGE;
   }
   FMOE_REQUIRE(row_stride >= 0, "%s: negative row stride", who);
+  FMOE_REQUIRE(std::isfinite(scale), "%s: the scale is not a finite fp32 number", who);
   if (T == 0) return FMOE_OK;
   FMOE_REQUIRE(d_logits && d_weights && d_ids, "%s: null device pointer", who);
   const bool scores = d_bias || (groups > 1 && group_score == FMOE_GROUP_TOP2);

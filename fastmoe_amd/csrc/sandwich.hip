@@ -16,6 +16,7 @@
 #include "rows8.h"
 
 #include <algorithm>
+#include <cmath>
 
 namespace fmoe {
 
@@ -659,8 +660,8 @@ Shares shares_of(int64_t rows, int64_t cols, int64_t runs) {
   Shares s{0, 0, 1, cols > kMaxRegCols};
   if (rows == 0) return s;
   // Each workgroup's part is 8 bytes a column to write and to read again; two workgroups are on a CU together where rows are
-  // short (with the join, bf16, 16384 x 2048: 97 us with 512 workgroups, 127 with 256, 120 with 1024; 16384 x 4096: 162, 201
-  // and 186; 8192 x 7168: 170, 157 and 196; 4096 x 16384: 188, 170 and 216).
+  // short (with the join, bf16, 16384 x 2048: 83 us with 512 workgroups, 118 with 256, 91 with 1024; 16384 x 4096: 147, 194
+  // and 156; 8192 x 7168: 155, 150 and 169; 4096 x 16384: 177, 164 and 198).
   const int64_t most = cols <= 4096 ? 512 : 256;
   const bool whole = runs >= most;
   s.long_rows |= whole && cols > kMaxSumCols;
@@ -685,6 +686,8 @@ extern "C" int fmoe_sandwich_norm(const void* d_x, int64_t x_row_stride, const v
   const char* who = "fmoe_sandwich_norm";
   if (int rc = check_sandwich(who, rows, cols, dtype, weight_dtype, d_gate, gate_dtype, gate_rows, d_post)) return rc;
   FMOE_REQUIRE(x_row_stride >= 0 && residual_row_stride >= 0, "%s: negative row stride", who);
+  FMOE_REQUIRE(std::isfinite(scale) && eps >= 0.f && std::isfinite(eps),
+               "%s: the scale must be finite, eps finite and not negative", who);
   if (rows == 0) return FMOE_OK;
   FMOE_REQUIRE(d_x && d_residual && d_h && !d_pre == !d_y, "%s: null device pointer", who);
   const SandwichArgs a{d_x, d_residual, x_row_stride, residual_row_stride, d_post, d_pre, d_gate, weight_dtype,

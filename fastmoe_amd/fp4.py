@@ -34,7 +34,7 @@ class Fp4Weights(NamedTuple):
     expert."""
 
     data: torch.Tensor    # uint8 [E, N, features rounded up to 128, / 2], codes of zero from ``features`` on
-    scales: torch.Tensor  # uint8 [E, N, features rounded up to 128, / 32]
+    scales: torch.Tensor  # uint8 [E, N, features rounded up to 128, / 32], not 255 from ``features`` on
     features: int
 
     def dequantize(self, dtype: torch.dtype = torch.float32) -> torch.Tensor:

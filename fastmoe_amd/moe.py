@@ -45,7 +45,7 @@ from .fp4 import Fp4Weights, fp4_linear, quantize_weights_fp4
 from .norms import sandwich_norm
 from .ops import (_apply, _combine_forward, _GroupedCombinePermuted, _refuse_autograd_capture,
                   _runs_plain, grouped_weighted_scatter_add)
-from .quantize import (CompressedRows, Int8Weights, _check_matrix, _compress, add_rms_norm,
+from .quantize import (CompressedRows, Int8Weights, _check_matrix, _compress, _no_gradient, add_rms_norm,
                        add_rms_norm_int8, gelu_compressed_backward, int8_linear, quantize_rows,
                        quantize_weights, restore_rows)
 from .routing import Routing, route_tokens
@@ -320,6 +320,12 @@ class _Balanced(nn.Module):
                 self._buffers["balance_bias"] = bias.to(moved.device)
         return self
 
+    def __setstate__(self, state):
+        super().__setstate__(state)
+        if "routing" not in self.__dict__:  # pickled before layers had one
+            self.routing = None
+            self._buffers.update(balance_bias=None, expert_load=None)
+
 
 class MoEFeedForward(_Balanced):
     """MoE feed-forward layer of tiny_model.py:42-77 on one GPU: router, E experts
@@ -332,7 +338,8 @@ class MoEFeedForward(_Balanced):
     ``routing``: how experts are chosen and weighed (``route_tokens``) instead of the reference's rule.
     ``balance=True`` (with a routing) adds ``balance_bias`` to the scores that choose; in training mode the
     layer counts the rows that each expert gets in ``expert_load``, and :meth:`update_balance`, called
-    after the optimiser's step, moves the bias against it."""
+    after the optimiser's step, moves the bias against it.  Where several processes train copies of the layer, sum
+    ``expert_load`` over them first, so that their biases stay alike."""
 
     def __init__(self, dim: int, ff_dim: int, num_experts: int, top_k: int,
                  implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None,
@@ -462,6 +469,9 @@ class SandwichMoEFeedForward(nn.Module):
             raise ValueError(f"fastmoe_amd: gate must be [{D}] or [{stream.shape[0]}, {D}], got "
                              f"{tuple(gate.shape)}")
         out = self.moe(normed.reshape(stream.shape)).reshape(-1, D)
+        if len(flat) and torch.is_grad_enabled() and normed.requires_grad and not out.requires_grad:
+            raise RuntimeError("fastmoe_amd: the layer between the norms has no gradients; call the block under "
+                               "torch.no_grad()")
         y, h = sandwich_norm(out, self.post_weight, flat, next_weight, gate=gate, scale=self.scale, eps=self.eps)
         return h.view(stream.shape), None if y is None else y.view(stream.shape)
 
@@ -481,7 +491,7 @@ class Fp4MoEFeedForward(_Balanced):
 
     ``forward(x)`` returns the layer's output.  The experts' first product reads each token's row
     through the reverse map and applies GELU: no [T*k, D] copy of the rows is made.  The host reads
-    nothing back, so a call can be captured in a HIP graph.  No gradients.
+    nothing back, so a call can be captured in a HIP graph.  It has no gradients, and refuses an x that requires one.
     """
 
     def __init__(self, moe: MoEFeedForward) -> None:
@@ -514,11 +524,15 @@ class Fp4MoEFeedForward(_Balanced):
                 raise ValueError("fastmoe_amd: some experts have biases and some have none")
             keep("b" + name, None if biases[0] is None else torch.stack([b.detach() for b in biases]))
 
-    @torch.no_grad()
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         if x.dim() != 3 or x.shape[2] != self.dim:
             raise ValueError(f"fastmoe_amd: x must be [batch, tokens, {self.dim}], got "
                              f"{tuple(x.shape)}")
+        _no_gradient("the layer in 4 bits", x)
+        with torch.no_grad():
+            return self._serve(x)
+
+    def _serve(self, x: torch.Tensor) -> torch.Tensor:
         B, T, D = x.shape
         flat = x.reshape(-1, D)
         if flat.shape[0] == 0:

@@ -28,7 +28,8 @@ def sandwich_norm(x: torch.Tensor, post_weight: torch.Tensor, residual: torch.Te
 
     Returns ``(y, h)``, y None without ``pre_weight``.  ``x`` and ``residual`` [T, D] (unit column
     stride); the weights [D], both in x's type or both float32; ``gate`` [D], or [G, D] with a row for each
-    of G equal runs of neighbouring rows (a sequence's, where T = G * its tokens), in x's type or float32.
+    of G equal runs of neighbouring rows (a sequence's, where T = G * its tokens), in x's type or float32; one that is
+    not contiguous, as a slice or a broadcast one, is copied first.
     h is rounded to x's type and y computed from it in float32 and rounded once.  Differentiable in all five;
     sums over rows run in a fixed order.  A row of x whose sum of squares passes float32's range adds nothing.
     """
@@ -40,6 +41,8 @@ def sandwich_norm(x: torch.Tensor, post_weight: torch.Tensor, residual: torch.Te
     out = call("sandwich", *given, scale, eps, records)
     if out is NotImplemented:
         _check_sandwich(*given, scale, eps)
+        if gate is not None and not gate.is_contiguous():
+            return sandwich_norm(x, post_weight, residual, pre_weight, gate=gate.contiguous(), scale=scale, eps=eps)
         _not_taken("sandwich_norm")
     return out
 
@@ -55,8 +58,10 @@ def _check_sandwich(x, post_weight, residual, pre_weight, gate, scale, eps) -> N
         if t is None and name != "post_weight":
             continue
         need_gpu(t, name)
-        if t.dim() not in ((1, 2) if name == "gate" else (1,)) or t.shape[-1] != D or not t.is_contiguous():
-            raise ValueError(f"fastmoe_amd: {name} must be contiguous [{D}], got {tuple(t.shape)}")
+        if t.dim() not in ((1, 2) if name == "gate" else (1,)) or t.shape[-1] != D or \
+                (name != "gate" and not t.is_contiguous()):
+            raise ValueError(f"fastmoe_amd: {name} must be {'' if name == 'gate' else 'contiguous '}[{D}], got "
+                             f"{tuple(t.shape)}")
         if t.dtype not in (x.dtype, torch.float32):
             raise TypeError(f"fastmoe_amd: {name} must be {x.dtype} or float32, got {t.dtype}")
         if t.device != x.device:

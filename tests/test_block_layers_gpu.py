@@ -279,3 +279,37 @@ def test_layers_that_would_lose_something_are_refused():
         layer(64, 32, 4, 2).fp4()(torch.zeros(2, 64, device=DEV, dtype=torch.bfloat16))
     with pytest.raises(ValueError, match="balance needs"):
         fm.MoEFeedForward(8, 8, 2, 1, balance=True)
+
+
+def test_layers_without_gradients_say_so():
+    x = rand(2, 5, 64, dtype=torch.bfloat16).requires_grad_(True)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        layer(64, 32, 4, 2).fp4()(x)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        fm.NormedMoEFeedForward(layer(64, 32, 4, 2)).cuda().fp4()(x)
+    for serving in (layer(64, 32, 4, 2).fp4(), layer(64, 32, 4, 2).int8()):
+        block = fm.SandwichMoEFeedForward(serving).cuda()
+        with pytest.raises(RuntimeError, match="no gradient"):
+            block(x)
+        with torch.no_grad():
+            h, _ = block(x)
+        assert not h.requires_grad
+        assert torch.equal(h, block.requires_grad_(False)(x.detach())[0])
+
+
+def test_layers_pickled_without_a_routing():
+    moe = layer(64, 32, 4, 2)
+    state = {k: v for k, v in moe.__dict__.items() if k != "routing"}
+    state["_buffers"] = {}
+    old = fm.MoEFeedForward.__new__(fm.MoEFeedForward)
+    old.__setstate__(copy.deepcopy(state))
+    x = rand(1, 9, 64, dtype=torch.bfloat16)
+    assert torch.equal(old(x), moe(x)) and old.state_dict().keys() == moe.state_dict().keys()
+    for form in ("int8", "fp4"):
+        assert torch.equal(getattr(old, form)()(x), getattr(moe, form)()(x))
+
+
+def test_an_empty_batch_between_norms():
+    block = fm.SandwichMoEFeedForward(layer(64, 32, 4, 2)).cuda()
+    h, y = block(rand(0, 5, 64, dtype=torch.bfloat16).requires_grad_(True), next_weight=block.norm_weight)
+    assert h.shape == y.shape == (0, 5, 64)

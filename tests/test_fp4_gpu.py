@@ -327,3 +327,36 @@ def test_rows_whose_last_piece_is_not_whole(tile, counts, N, K):
 def test_rows_about_where_weights_stay_in_the_caches(per):
     assert _pick(per * 24, 24, 4096, 192) == 96256
     run([per] * 24, 4096, 192, bias=True)
+
+
+def test_weights_and_rows_beyond_32_bits():
+    """Codes of the last expert begin past 4 GiB, rows of x end past it: as a call on that expert, on those rows."""
+    E, N, K = 5, 1 << 18, 8192
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    data = torch.randint(0, 256, (E, N, K // 2), dtype=torch.uint8, generator=gen, device=DEV)
+    scales = torch.randint(117, 122, (E, N, K // 32), dtype=torch.uint8, generator=gen, device=DEV)
+    x = torch.zeros((1 << 18) + 200, K, dtype=B, device=DEV)
+    x[-120:] = torch.randn(120, K, generator=gen, device=DEV).to(B)
+    for per in (3, 120):
+        off = torch.tensor([0, 0, 2, 2, 2, 2 + per], device=DEV)
+        rows = torch.cat([torch.zeros(2, dtype=torch.int64), torch.arange(len(x) - per, len(x))]).to(DEV)
+        out = fm.fp4_linear(x, fm.Fp4Weights(data, scales, K), off, rows=rows)
+        assert not out[:2].any()
+        pick = torch.arange(0, N, 1021)
+        w = fm.Fp4Weights(data[4][pick], scales[4][pick], K)
+        y = x[-per:]
+        want, size = y.double() @ w.dequantize().double().T, y.double().abs() @ w.dequantize().double().abs().T
+        check(out[2:][:, pick], want.cpu(), size.cpu(), K)
+    del data, scales
+
+
+@pytest.mark.parametrize("count", [4, 300])
+def test_rows_outside_are_zero_whatever_x_holds(count):
+    w = fm.Fp4Weights(*(t.to(DEV) for t in ref.weights(1, 300, 256)), 256)
+    x = torch.full((3, 256), float("nan"), device=DEV, dtype=B)
+    x[1] = 1
+    rows = torch.full((count,), 1, device=DEV)
+    rows[::3], rows[1::7] = -1, 99
+    out = fm.fp4_linear(x, w, rows=rows)
+    live = rows == 1
+    assert not out[~live].any() and torch.equal(out[live], fm.fp4_linear(x[1:2], w).expand(int(live.sum()), -1))

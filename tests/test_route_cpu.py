@@ -68,3 +68,10 @@ def test_backward_entry_point_refuses():
     assert call(norm=DEV, x=DEV, rest=DEV, renorm=0) == _abi.EINVAL
     assert call(T=1 << 40) == _abi.ERANGE
     assert call(T=0, g=None) == _abi.OK
+
+
+@pytest.mark.parametrize("scale", [float("inf"), float("nan")])
+def test_entry_point_refuses_a_scale_beyond_fp32(scale):
+    call = _abi.lib().fmoe_route
+    assert call(DEV, 8, 4, 8, _abi.F32, None, 2, 0, 1, 1, 0, 1, scale, DEV, _abi.F32, DEV, None, None, None,
+                None) == _abi.EINVAL

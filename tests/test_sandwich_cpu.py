@@ -54,3 +54,9 @@ def test_backward_entry_point_refuses():
                 dict(cols=20000, gpost=None, gpre=None, ggate=None, ws=None)):
         assert call(**bad) == _abi.EINVAL, bad
     assert call(rows=1 << 40) == _abi.ERANGE
+
+
+@pytest.mark.parametrize("scale,eps", [(float("inf"), 1e-6), (float("nan"), 1e-6), (1.0, float("inf")), (1.0, -1.0)])
+def test_forward_entry_point_refuses_numbers(scale, eps):
+    call = _abi.lib().fmoe_sandwich_norm
+    assert call(DEV, 8, DEV, 8, DEV, DEV, B, None, F, 0, 4, 8, B, scale, eps, DEV, DEV, None, None) == _abi.EINVAL

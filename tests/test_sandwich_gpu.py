@@ -289,3 +289,50 @@ def test_refusals():
         _call({**on, "gate": d["gate"]}, 1.0)
     with pytest.raises(TypeError, match="tensor"):
         fm.sandwich_norm(on["x"], on["post"], None)
+
+
+def test_gates_that_are_slices_or_broadcast():
+    """As a copy of them; the gradient comes back through the copy, a broadcast one's as the sum over its rows."""
+    d, gy, gh = _inputs(12, 40, torch.bfloat16, gates=3)
+    on = {k: v.to(DEV) for k, v in d.items()}
+    many = torch.randn(3, 120, device=DEV).bfloat16().requires_grad_(True)
+    one = torch.randn(1, 40, device=DEV).requires_grad_(True)
+    for leaf, view in ((many, lambda t: t[:, 40:80]), (many, lambda t: t.chunk(3, -1)[2]), (one, lambda t: t.expand(3, 40)),
+                       (many, lambda t: t.t()[:3, 0].expand(40, 3).t())):
+        copy = view(leaf).detach().contiguous().requires_grad_(True)
+        got = _call({**on, "gate": view(leaf)}, 0.5)
+        want = _call({**on, "gate": copy}, 0.5)
+        for g, w in zip(got, want):
+            assert torch.equal(g, w)
+        up = [gy.to(DEV), gh.to(DEV)]
+        g, = torch.autograd.grad(got, leaf, up)
+        w, = torch.autograd.grad(want, copy, up)
+        assert torch.equal(g, torch.autograd.grad(view(leaf), leaf, w)[0])
+
+
+def test_numbers_beyond_fp32_are_refused():
+    d, *_ = _inputs(4, 16, torch.float32)
+    on = {k: v.to(DEV) for k, v in d.items()}
+    with pytest.raises(ValueError, match="finite"):
+        _call(on, 1e39)
+    with pytest.raises(ValueError, match="finite"):
+        fm.sandwich_norm(on["x"], on["post"], on["residual"], eps=1e39)
+    with pytest.raises(ValueError, match="finite"):
+        fm.route_tokens(on["x"], 2, fm.Routing(scale=1e39))
+
+
+def test_rows_beyond_32_bits_of_elements():
+    """2^31 elements are passed: the last rows hold to the definition, forward and backward.  (A call on them alone may
+    differ by roundings: few rows are given more threads.)"""
+    T, D = (1 << 18) + 3, 8192
+    gen = torch.Generator(device=DEV).manual_seed(0)
+    r = lambda *s: torch.randn(*s, generator=gen, device=DEV, dtype=torch.bfloat16)
+    on = {"x": r(T, D), "residual": r(T, D), "post": r(D), "pre": r(D), "gate": r(D)}
+    for t in on.values():
+        t.requires_grad_(True)
+    y, h = _call(on, 0.5)
+    gx, gr = torch.autograd.grad([y, h], [on["x"], on["residual"]], [y.detach(), h.detach()])
+    last = lambda t: t.detach()[-5:].cpu()
+    d = {k: last(v) if v.dim() == 2 else v.detach().cpu() for k, v in on.items()}
+    _forward(d, 0.5, y.detach()[-5:], h.detach()[-5:])
+    _backward(d, 0.5, last(h), last(y), last(h), {"x": gx[-5:], "residual": gr[-5:]})
