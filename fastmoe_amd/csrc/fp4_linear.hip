@@ -456,9 +456,9 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
     }
   };
   const int tiles = (t.count + 31) / 32;
-  if (TM >= 4 && tiles == 4) run(std::integral_constant<int, TM >= 4 ? 4 : 1>{});
-  else if (TM >= 3 && tiles == 3) run(std::integral_constant<int, TM >= 3 ? 3 : 1>{});
-  else if (TM >= 2 && tiles == 2) run(std::integral_constant<int, TM >= 2 ? 2 : 1>{});
+  static_assert(TM == 3, "a case for each number of tiles");
+  if (tiles == 3) run(std::integral_constant<int, 3>{});
+  else if (tiles == 2) run(std::integral_constant<int, 2>{});
   else run(std::integral_constant<int, 1>{});
   wait_loads<0>();
   __syncthreads();
@@ -467,10 +467,9 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
   by_output(a, [&](auto to_type) {
     using TO = decltype(to_type);
     constexpr int kSize = ElemInfo<TO>::kBytes;
-    // column tiles at a time: where there are two, they fit where the wave's weights were
-    constexpr int CT = WN;
-    constexpr int kPitch = CT * 32 * kSize + 16;  // 16 bytes more: the 32 rows start in different banks
+    constexpr int kPitch = WN * 32 * kSize + 16;  // 16 bytes more: the 32 rows start in different banks
     constexpr int kPerStage = kX / (32 * kPitch);
+    // where a wave has two tiles of columns, they fit where its weights were; else where the rows were
     static_assert(WN == 2 ? 32 * kPitch <= (int)sizeof(weights[0]) : kPerStage * 3 >= W, "the buffers hold the results");
     uint8_t* mine = WN == 2 ? weights[wave]
                             : (wave / kPerStage == 0 ? rows0 : wave / kPerStage == 1 ? rows1 : rows2) +
@@ -482,44 +481,41 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
       const bool dead = !row_live[first + l32];
       // lane l of a 32 x 32 result has row l % 32 and columns 8 * q + 4 * (l / 32) + 0..3, q = 0..3
 #pragma unroll
-      for (int base = 0; base < WN; base += CT) {
+      for (int n = 0; n < WN; ++n)
 #pragma unroll
-        for (int n = 0; n < CT; ++n)
+        for (int q = 0; q < 4; ++q) {
+          const int c = n * 32 + q * 8 + half * 4;
+          float f[4];
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            const int c = n * 32 + q * 8 + half * 4;
-            float f[4];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-              f[j] = (dead ? 0.f : acc[base + n][m][4 * q + j]) + col_bias[w0 + base * 32 + c + j];
-              if (a.gelu) f[j] = gelu<TO>(f[j]);
-            }
-            apart<TO>(f);
-            *reinterpret_cast<typename Vec<TO, 4>::raw_t*>(mine + l32 * kPitch + c * kSize) = Vec<TO, 4>::pack(f);
+          for (int j = 0; j < 4; ++j) {
+            f[j] = (dead ? 0.f : acc[n][m][4 * q + j]) + col_bias[w0 + c + j];
+            if (a.gelu) f[j] = gelu<TO>(f[j]);
           }
-        constexpr int kLanes = CT * 32 * kSize / 16;  // lanes of a row
-        wave_order();
-#pragma unroll
-        for (int p = 0; p < 32 * kLanes / kWave; ++p) {
-          const int r = p * (kWave / kLanes) + lane / kLanes, c = lane % kLanes * (16 / kSize);
-          const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * kPitch + c * kSize);
-          const int64_t n = n0 + w0 + base * 32 + c;
-          if (first + r >= t.count || n >= a.N) continue;
-          TO* to = static_cast<TO*>(a.out) + (t.row + first + r) * a.out_stride + n;
-          if (n + 16 / kSize <= a.N) {
-            *reinterpret_cast<u32x4_any*>(to) = v;
-          } else {
-            const int left = (int)(a.N - n);
-#pragma unroll
-            for (int j = 0; j < 16 / kSize; ++j)
-              if (j < left) {
-                if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(to)[j] = v[j];
-                else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(v[j / 2] >> (16 * (j % 2)));
-              }
-          }
+          apart<TO>(f);
+          *reinterpret_cast<typename Vec<TO, 4>::raw_t*>(mine + l32 * kPitch + c * kSize) = Vec<TO, 4>::pack(f);
         }
-        wave_order();  // the next tiles' results go where these lay
+      constexpr int kLanes = WN * 32 * kSize / 16;  // lanes of a row
+      wave_order();
+#pragma unroll
+      for (int p = 0; p < 32 * kLanes / kWave; ++p) {
+        const int r = p * (kWave / kLanes) + lane / kLanes, c = lane % kLanes * (16 / kSize);
+        const u32x4 v = *reinterpret_cast<const u32x4*>(mine + r * kPitch + c * kSize);
+        const int64_t n = n0 + w0 + c;
+        if (first + r >= t.count || n >= a.N) continue;
+        TO* to = static_cast<TO*>(a.out) + (t.row + first + r) * a.out_stride + n;
+        if (n + 16 / kSize <= a.N) {
+          *reinterpret_cast<u32x4_any*>(to) = v;
+        } else {
+          const int left = (int)(a.N - n);
+#pragma unroll
+          for (int j = 0; j < 16 / kSize; ++j)
+            if (j < left) {
+              if constexpr (kSize == 4) reinterpret_cast<uint32_t*>(to)[j] = v[j];
+              else reinterpret_cast<uint16_t*>(to)[j] = (uint16_t)(v[j / 2] >> (16 * (j % 2)));
+            }
+        }
       }
+      wave_order();  // the next tile's results go where these lay
     }
   });
 }
