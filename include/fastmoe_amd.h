@@ -589,7 +589,7 @@ FMOE_API int fmoe_sandwich_norm_backward(const void* d_grad_y, int64_t gy_row_st
  * Weights in 4 bits: v * 2^(s - 127) with v one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives (the code's bits: sign,
  * two of exponent, one of mantissa) and s a byte for 32 neighbouring weights of a row (255: NaN).  d_q:
  * [rows, Kp / 2] bytes, two codes each, the earlier column's in the low half; d_scales: [rows, Kp / 32] bytes, with Kp
- * the columns rounded up to 128; codes beyond the columns are zero.  d_q starts at a multiple of 16 bytes.
+ * the columns rounded up to 128; beyond the columns codes are zero and scales not 255.  d_q starts at a multiple of 16 bytes.
  * fmoe_quantize_fp4 takes for each 32 the smallest power of two (from 2^-127 on) with which none of them passes 6, and
  * rounds to the nearest (ties to even); 32 zeros: s = 127; an infinity or a NaN among them: s = 255, codes 0.
  * fmoe_restore_fp4 writes the values, packed.

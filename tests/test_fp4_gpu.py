@@ -360,3 +360,19 @@ def test_rows_outside_are_zero_whatever_x_holds(count):
     out = fm.fp4_linear(x, w, rows=rows)
     live = rows == 1
     assert not out[~live].any() and torch.equal(out[live], fm.fp4_linear(x[1:2], w).expand(int(live.sum()), -1))
+
+
+@pytest.mark.parametrize("K", [3, 64, 100, 128, 192, 257, 400, 1000])
+@pytest.mark.parametrize("counts", [[1], [3, 0, 12], [200, 97]], ids=str)
+def test_what_lies_beside_the_rows_is_not_read(counts, K):
+    """x is a slice of rows whose other columns hold NaN; padded codes are zero, their scales the largest."""
+    data, scales = ref.weights(len(counts), 70, K)
+    scales[..., (K + 31) // 32:] = 254
+    w = fm.Fp4Weights(data.to(DEV), scales.to(DEV), K)
+    x = torch.randn(sum(counts), K, generator=torch.Generator().manual_seed(K)).to(B)
+    wide = torch.full((sum(counts), 16 + K + 24), float("nan"), dtype=B, device=DEV)
+    off = offsets_of(counts)
+    for at in (16, 11):
+        wide.fill_(float("nan"))
+        wide[:, at:at + K] = x.to(DEV)
+        check(fm.fp4_linear(wide[:, at:at + K], w, off.to(DEV)), *ref.linear(x, ref.values(data, scales, K), off), K)
