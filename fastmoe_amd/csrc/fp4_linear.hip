@@ -8,7 +8,7 @@
 // A weight is v * 2^(s - 127): v one of 0, 0.5, 1, 1.5, 2, 3, 4, 6 and their negatives (sign, two bits of exponent, one of
 // mantissa), s a byte for 32 neighbouring weights of an output (255: NaN).  That is the form that gfx950 converts two
 // of in one instruction, the scale with them, to bf16 or fp16, so the products run on the 16-bit matrix units
-// with the rows as they are: bf16 holds such a weight exactly; fp16 does where 2^-23 <= scale <= 2^13, smaller ones are
+// with the rows as they are: bf16 holds such a weight exactly where fp32 does; fp16 does where 2^-23 <= scale <= 2^13, smaller ones are
 // rounded to its smallest numbers and larger ones pass its range.  Products are exact and summed in fp32; the result is
 // rounded once, to the output's type.
 //

@@ -83,8 +83,8 @@ def fp4_linear(x: torch.Tensor, weights: Fp4Weights, expert_offsets: Optional[to
 
     for r in [expert_offsets[e], expert_offsets[e + 1]), i = ``rows[r]`` (the reverse map of
     ``permute_tokens``), or i = r without ``rows``.  ``x`` [T, K], bfloat16 or float16 (unit column stride);
-    W the weights in x's type (bfloat16 holds every one, float16 those whose scale lies between 2^-23 and
-    2^13).  ``expert_offsets`` int64 [E + 1] on the device (``PermutedTokens.expert_offsets``), starting at 0
+    W the weights in x's type (bfloat16 holds every one that float32 does, float16 those whose scale lies
+    between 2^-23 and 2^13).  ``expert_offsets`` int64 [E + 1] on the device (``PermutedTokens.expert_offsets``), starting at 0
     and not falling; None for one expert's weights.  ``bias`` [E, N] (or [N]).  ``activation``: None or "gelu" (the
     exact form, as ``torch.nn.GELU()``).  Sums are float32; the result is rounded once.
 
