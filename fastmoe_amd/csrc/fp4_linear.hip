@@ -277,7 +277,8 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
   const int lane = threadIdx.x & (kWave - 1), wave = uniform(threadIdx.x / kWave);
   const int l32 = lane & 31, half = lane >> 5;
   const int w0 = wave * WN * 32;  // this wave's columns
-  // Its columns' codes and scales through descriptors that end with the last column: what lies beyond reads as zero.
+  // Its columns' codes and scales through descriptors that end with the last column: what lies beyond reads as zero.  A load's
+  // whole place is in its vector offset: a scalar one has no part in the range check.
   const int here = (int)max(min((int64_t)WN * 32, a.N - n0 - w0), (int64_t)0);
   const int64_t first = t.expert * a.N + min(n0 + w0, a.N - 1);
   const int code_pitch = (int)(a.Kp / 2), scale_pitch = (int)(a.Kp / kFp4Block);
@@ -288,11 +289,12 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
     if (i < 4 * WN) {
       const int chunk = (lane % 8) ^ swizzle<128>(i * 8 + lane / 8);
       __builtin_amdgcn_raw_ptr_buffer_load_lds(codes_at, (FMOE_LDS void*)(weights[wave] + i * 1024), 16,
-                                               code_from + chunk * 16, i * 8 * code_pitch + s * 128, 0, AGAIN ? kCPolCached : kCPol);
+                                               code_from + chunk * 16 + (i * 8 * code_pitch + s * 128), 0, 0,
+                                               AGAIN ? kCPolCached : kCPol);
     } else {
       const int n = i - 4 * WN;
-      __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_at, (FMOE_LDS void*)(weights[wave] + kCodes + n * 256), 4, scale_from,
-                                               n * 32 * scale_pitch + s * 8, 0, kCPolCached);
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(scales_at, (FMOE_LDS void*)(weights[wave] + kCodes + n * 256), 4,
+                                               scale_from + (n * 32 * scale_pitch + s * 8), 0, 0, kCPolCached);
     }
   };
 #pragma unroll
