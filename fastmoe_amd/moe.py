@@ -407,6 +407,14 @@ def _check_residual(x: torch.Tensor, residual: Optional[torch.Tensor]) -> None:
                          f"{tuple(residual.shape)}")
 
 
+def _copy_parameters(of: nn.Module, to: nn.Module, *names: str) -> None:
+    """``to`` gets copies of these parameters of ``of`` in their own type: a norm may be float32 around a layer in
+    16 bits."""
+    for name in names:
+        p = getattr(of, name)
+        to.register_parameter(name, None if p is None else nn.Parameter(p.detach().clone()))
+
+
 class NormedMoEFeedForward(nn.Module):
     """A :class:`MoEFeedForward` behind the root-mean-square norm of a pre-norm block: the residual's
     addition and the norm are one kernel (``add_rms_norm``).  ``forward(x, residual=None)`` returns
@@ -434,7 +442,7 @@ class NormedMoEFeedForward(nn.Module):
         """As :meth:`MoEFeedForward.fp4`, behind a copy of the norm."""
         _check_layer(self, NormedMoEFeedForward)
         block = NormedMoEFeedForward(self.moe.fp4(), self.eps)
-        block.load_state_dict({"norm_weight": self.norm_weight}, strict=False)
+        _copy_parameters(self, block, "norm_weight")
         return block.requires_grad_(False)
 
 
@@ -479,8 +487,7 @@ class SandwichMoEFeedForward(nn.Module):
         """This block for serving: a copy with the experts' weights in 4 bits."""
         _check_layer(self, SandwichMoEFeedForward)
         block = SandwichMoEFeedForward(self.moe.fp4(), self.eps, self.scale, self.gate is not None)
-        own = {n: p for n, p in self.named_parameters(recurse=False)}
-        block.load_state_dict(own, strict=False)
+        _copy_parameters(self, block, "norm_weight", "post_weight", "gate")
         return block.requires_grad_(False)
 
 
