@@ -412,7 +412,7 @@ def _copy_parameters(of: nn.Module, to: nn.Module, *names: str) -> None:
     16 bits."""
     for name in names:
         p = getattr(of, name)
-        to.register_parameter(name, None if p is None else nn.Parameter(p.detach().clone()))
+        setattr(to, name, None if p is None else nn.Parameter(p.detach().clone()))
 
 
 class NormedMoEFeedForward(nn.Module):
