@@ -309,7 +309,10 @@ def unpermute(x_out: Union[torch.Tensor, Sequence[torch.Tensor]], reverse_map_in
 
 class _Balanced(nn.Module):
     """A layer whose ``balance_bias`` (float32 [E], or None) stays float32 when the layer is cast: steps of
-    1e-3 and less would be lost in 16 bits."""
+    1e-3 and less would be lost in 16 bits.  ``expert_load`` (int64 [E], or None) moves with the layer, but is no
+    buffer: data-parallel wrappers copy the first process's buffers over the others' before a forward."""
+
+    expert_load: Optional[torch.Tensor] = None
 
     def _apply(self, fn, recurse=True):
         bias = self._buffers.get("balance_bias")
@@ -318,13 +321,22 @@ class _Balanced(nn.Module):
             moved = self._buffers["balance_bias"]
             if moved.dtype != torch.float32:
                 self._buffers["balance_bias"] = bias.to(moved.device)
+        load = self.expert_load
+        if load is not None:
+            moved = fn(load)
+            if load.is_meta and not moved.is_meta:  # memory without values
+                moved = torch.zeros_like(moved)
+            self.expert_load = moved if moved.dtype == load.dtype else load.to(moved.device)
         return self
 
     def __setstate__(self, state):
         super().__setstate__(state)
         if "routing" not in self.__dict__:  # pickled before layers had one
             self.routing = None
-            self._buffers.update(balance_bias=None, expert_load=None)
+            self._buffers.update(balance_bias=None)
+        if "expert_load" in self._buffers:  # pickled when it was one
+            self._non_persistent_buffers_set.discard("expert_load")
+            self.expert_load = self._buffers.pop("expert_load")
 
 
 class MoEFeedForward(_Balanced):
@@ -338,8 +350,9 @@ class MoEFeedForward(_Balanced):
     ``routing``: how experts are chosen and weighed (``route_tokens``) instead of the reference's rule.
     ``balance=True`` (with a routing) adds ``balance_bias`` to the scores that choose; in training mode the
     layer counts the rows that each expert gets in ``expert_load``, and :meth:`update_balance`, called
-    after the optimiser's step, moves the bias against it.  Where several processes train copies of the layer, sum
-    ``expert_load`` over them first, so that their biases stay alike."""
+    after the optimiser's step, moves the bias against it.  ``expert_load`` is what this process counted, neither a
+    buffer nor part of the layer's state.  Where several processes train copies of the layer, sum it over them first,
+    so that their biases stay alike."""
 
     def __init__(self, dim: int, ff_dim: int, num_experts: int, top_k: int,
                  implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None,
@@ -361,8 +374,7 @@ class MoEFeedForward(_Balanced):
             [nn.Sequential(nn.Linear(dim, ff_dim, bias=False), nn.GELU(),
                            nn.Linear(ff_dim, dim, bias=False)) for _ in range(num_experts)])
         self.register_buffer("balance_bias", torch.zeros(num_experts) if balance else None)
-        self.register_buffer("expert_load", torch.zeros(num_experts, dtype=torch.int64) if balance else None,
-                             persistent=False)
+        self.expert_load = torch.zeros(num_experts, dtype=torch.int64) if balance else None
 
     @torch.no_grad()
     def update_balance(self, rate: float = 1e-3) -> None:
