@@ -9,8 +9,8 @@
 // A choice is a comparison of numbers that may lie next to each other, so s is computed in 64 bits (to
 // 2^-36) and rounded to fp32 once; the bias and the sum of two are added in fp32.  Whoever rounds the same
 // scores to fp32 makes the same choices.  The weights are computed from the chosen logits in 64 bits: k of
-// them cost little.  Masked experts (-inf) have no share; where all that count are masked, no weight either.
-// A NaN ranks above every number and makes the weights that depend on it NaN.
+// them cost little.  Masked experts (-inf) have no share, and their choice is their bias alone; where all
+// that count are masked, no weight either.  A NaN ranks above every number and makes the weights that depend on it NaN.
 //
 // Backward, with g the weights' gradient and S = sum_j u_j g_j over the chosen:
 //   softmax, renormalised   dl_i = scale u_i (g_i - S), the chosen alone

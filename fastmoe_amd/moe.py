@@ -379,7 +379,8 @@ class MoEFeedForward(_Balanced):
     @torch.no_grad()
     def update_balance(self, rate: float = 1e-3) -> None:
         """``balance_bias += rate * sign(mean load - load)`` of the rows counted since the last call, which
-        are forgotten."""
+        are forgotten.  A bias of -inf stays: an expert that the router masks in every row is to have it, else its bias
+        rises until it takes places with weight 0."""
         if self.balance_bias is None:
             raise ValueError("fastmoe_amd: the layer was made without balance")
         load = self.expert_load.double()

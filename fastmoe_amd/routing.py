@@ -74,9 +74,11 @@ def route_tokens(logits: torch.Tensor, top_k: int, routing: Routing = _DEFAULT, 
     computed in 64 bits and rounded once.  Differentiable in the logits; the bias only chooses, and one that
     requires a gradient is refused.
 
-    A logit of -inf masks its expert: weight 0, chosen only if nothing else is left.  Where nothing is left
-    the ids are still different experts, with weights of 0.  A NaN ranks highest and makes the weights that
-    depend on it NaN.  At most 64 of 4096 experts; with groups at most 1024 experts in 64 groups.
+    A logit of -inf masks its expert: score and weight 0.  Where the logits choose, it is chosen only if nothing else is
+    left; where ``s + bias`` does, its choice is its bias alone, and one above others' choices takes a place with weight
+    0.  A bias of -inf leaves an expert out of every row.  Where nothing is left the ids are still different experts,
+    with weights of 0.  A NaN ranks highest and makes the weights that depend on it NaN.  At most 64 of 4096
+    experts; with groups at most 1024 experts in 64 groups.
     """
     _refuse_transforms("route_tokens")
     w_code = _FLOAT_CODES.get(out_dtype if out_dtype is not None else getattr(logits, "dtype", None), -1)

@@ -530,7 +530,8 @@ FMOE_API int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_
  *     ids = the top_k highest c of those groups, highest first, the lowest index first among equals
  *     weights = scale * s[ids], divided by sum(s[ids]) with renormalize
  * d_bias: fp32[E] or null.  d_weights [T, top_k] in weight_dtype, d_ids int64[T, top_k].  A masked expert
- * (-inf) has no weight; where every expert that counts is masked, the ids are still different experts and the
+ * (-inf) has s = 0 and no weight: where s + bias chooses, a high bias may still choose it, and a bias of -inf
+ * leaves it out.  Where every expert that counts is masked, the ids are still different experts and the
  * weights zero.  A NaN ranks highest.  For the backward, null where none follows: d_share fp32[T, top_k], the
  * weights before the scale; d_rest fp32[T, top_k], 1 - s (a sigmoid); d_norm fp32[T, 2], maximum and 1 / sum
  * of e^(l - maximum) (a softmax without renormalize; written for that alone).
