@@ -7,10 +7,14 @@
 //   weights w = scale * u with u = s[ids], or s[ids] / sum(s[ids])
 //
 // A choice is a comparison of numbers that may lie next to each other, so s is computed in 64 bits (to
-// 2^-36) and rounded to fp32 once; the bias and the sum of two are added in fp32.  Whoever rounds the same
-// scores to fp32 makes the same choices.  The weights are computed from the chosen logits in 64 bits: k of
-// them cost little.  Masked experts (-inf) have no share, and their choice is their bias alone; where all
-// that count are masked, no weight either.  A NaN ranks above every number and makes the weights that depend on it NaN.
+// 2^-36) and rounded to fp32 once; the bias and the sum of two are added in fp32.  Whoever rounds the exact scores to
+// fp32 has the same ones but for about four in a million, which lie so near the middle of two fp32 numbers that they
+// round to the other one, and makes the same choices unless such a score decides one.  The weights are computed from
+// the chosen logits in 64 bits: k of them cost little.  Only the sum under a softmax over all experts is fp32 where no
+// scores are compared, to 2^-17 and measured to 2^-20 (in 64 bits 32768 tokens with 64 experts take 8.8 us
+// instead of 7.7, with 256 experts 22.5 instead of 18.7).  Masked experts (-inf) have no share, and their choice is their
+// bias alone; where all that count are masked, no weight either.  A NaN ranks above every number and makes the weights that
+// depend on it NaN.
 //
 // Backward, with g the weights' gradient and S = sum_j u_j g_j over the chosen:
 //   softmax, renormalised   dl_i = scale u_i (g_i - S), the chosen alone

@@ -68,10 +68,11 @@ def route_tokens(logits: torch.Tensor, top_k: int, routing: Routing = _DEFAULT, 
     """The ``top_k`` experts of each row of ``logits`` [T, E] (unit column stride), and their weights in
     ``out_dtype`` (None: the logits' type).
 
-    With s the scores, experts are chosen by ``s + bias`` (``bias`` float32 [E]; s is rounded to float32
-    from 64 bits, then the bias is added), or, without a bias and without groups ranked by a sum, by the
-    logits, which rank alike.  Equal choices go to the lowest index.  The weights are of s alone,
-    computed in 64 bits and rounded once.  Differentiable in the logits; the bias only chooses, and one that
+    With s the scores, experts are chosen by ``s + bias`` (``bias`` float32 [E]; s is computed to 2^-36 and rounded to
+    float32, then the bias is added), or, without a bias and without groups ranked by a sum, by the logits, which
+    rank alike.  Equal choices go to the lowest index.  The weights are of s alone, computed in 64 bits and
+    rounded once; where the logits choose, the sum under a softmax over all experts is float32 (the weights then hold
+    to 2^-17, and measured to 2^-20).  Differentiable in the logits; the bias only chooses, and one that
     requires a gradient is refused.
 
     A logit of -inf masks its expert: score and weight 0.  Where the logits choose, it is chosen only if nothing else is

@@ -524,11 +524,12 @@ FMOE_API int64_t fmoe_int8_linear_tile(int64_t rows, int64_t num_experts, int64_
 /*
  * Routing of tokens to experts: for each row of logits[T, E] (row_stride elements apart, of `dtype`),
  *     s = softmax(l) over all experts, or sigmoid(l)             (score: fmoe_score)
- *     c = s + bias, both in fp32 (s rounded from 64 bits), with a bias or groups ranked by a sum; else l
+ *     c = s + bias, both in fp32 (s to 2^-36, then rounded), with a bias or groups ranked by a sum; else l
  *     the top_groups of `groups` equal groups of neighbouring experts, by their highest c or the sum of
  *     their two highest in fp32                                  (group_score: fmoe_group_score)
  *     ids = the top_k highest c of those groups, highest first, the lowest index first among equals
  *     weights = scale * s[ids], divided by sum(s[ids]) with renormalize
+ * in 64 bits, rounded once (but the sum under a softmax over all experts where c = l: fp32).
  * d_bias: fp32[E] or null.  d_weights [T, top_k] in weight_dtype, d_ids int64[T, top_k].  A masked expert
  * (-inf) has s = 0 and no weight: where s + bias chooses, a high bias may still choose it, and a bias of -inf
  * leaves it out.  Where every expert that counts is masked, the ids are still different experts and the
