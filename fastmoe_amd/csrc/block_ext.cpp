@@ -59,17 +59,17 @@ void refuse_second(const variable_list& grads, const char* message) {
   for (const Tensor& g : grads)
     if (g.defined() && g.requires_grad()) throw std::runtime_error(message);
 }
+void refuse_history(Tensor& t, torch::autograd::edge_list to, const char* message) {
+  torch::autograd::set_history(t, std::shared_ptr<torch::autograd::Node>(
+                                      new torch::autograd::Error(message, std::move(to)), torch::autograd::deleteNode));
+}
 void mark_second(std::initializer_list<Tensor*> results, const variable_list& inputs, const char* message) {
   if (!at::GradMode::is_enabled()) return;
   bool any = false;
   for (const Tensor& t : inputs) any |= t.defined() && t.requires_grad();
   if (!any) return;
   for (Tensor* g : results)
-    if (g->defined())
-      torch::autograd::set_history(
-          *g, std::shared_ptr<torch::autograd::Node>(
-                  new torch::autograd::Error(message, torch::autograd::collect_next_edges(inputs)),
-                  torch::autograd::deleteNode));
+    if (g->defined()) refuse_history(*g, torch::autograd::collect_next_edges(inputs), message);
 }
 
 // ---- the router -----------------------------------------------------------------------------------
@@ -111,8 +111,10 @@ class Route : public torch::autograd::Function<Route> {
  public:
   static variable_list forward(AutogradContext* ctx, Tensor logits, Routing o) {
     Routed r = run_route(logits, o, true);
-    // the logits are kept where a gradient reads them, and for what depends on them under create_graph
-    ctx->save_for_backward({logits, r.ids, r.share, r.rest, r.norm});
+    // the logits are kept where the gradient reads them
+    ctx->save_for_backward({r.norm.defined() ? logits : Tensor(), r.ids, r.share, r.rest, r.norm});
+    ctx->saved_data["experts"] = logits.size(1);
+    ctx->saved_data["dtype"] = (int64_t)logits.scalar_type();
     ctx->saved_data["renormalize"] = (int64_t)o.renormalize;
     ctx->saved_data["scale"] = (double)o.scale;
     ctx->mark_non_differentiable({r.ids});
@@ -128,16 +130,22 @@ class Route : public torch::autograd::Function<Route> {
     Place place(share);
     refuse_capture("the router's backward");
     const Tensor g = by_rows(grads[0]).contiguous();
-    const int64_t T = logits.size(0), E = logits.size(1);
-    Tensor out = empty({T, E}, logits);
+    const int64_t T = ids.size(0), E = ctx->saved_data["experts"].toInt();
+    const auto dtype = (at::ScalarType)ctx->saved_data["dtype"].toInt();
+    Tensor out = empty({T, E}, share, dtype);
     check(api.fmoe_route_backward(data(g), code(g.scalar_type()), static_cast<const int64_t*>(data(ids)),
                                   static_cast<const float*>(data(share)), static_cast<const float*>(data(rest)),
-                                  static_cast<const float*>(data(norm)), data(logits), pitch(logits), T, E,
-                                  ids.size(1), code(logits.scalar_type()),
+                                  static_cast<const float*>(data(norm)), data(logits),
+                                  logits.defined() ? pitch(logits) : E, T, E, ids.size(1), code(dtype),
                                   (int)ctx->saved_data["renormalize"].toInt(),
                                   (float)ctx->saved_data["scale"].toDouble(), data(out), place.stream),
           "fmoe_route_backward");
-    mark_second({&out}, {logits}, kNoSecondRoute);
+    // the result depends on the logits, whether they are kept or not: what this node's gradient goes to
+    if (at::GradMode::is_enabled()) {
+      const auto node = torch::autograd::get_current_node();
+      if (!node) throw std::runtime_error(kNoSecondRoute);
+      refuse_history(out, node->next_edges(), kNoSecondRoute);
+    }
     return {out, Tensor()};
   }
 };

@@ -52,3 +52,48 @@ def test_balance_leaves_a_bias_of_minus_infinity():
         assert int(moe.expert_load[2]) == 0 and int(moe.expert_load.sum()) == 80
         moe.update_balance(0.25)
     assert moe.balance_bias[2] == -INF and torch.isfinite(moe.balance_bias).sum() == 5
+
+
+RULES = [fm.Routing(), fm.Routing("sigmoid"), fm.Routing("sigmoid", renormalize=False), fm.Routing(renormalize=False)]
+
+
+@pytest.mark.parametrize("r", RULES, ids=str)
+@pytest.mark.parametrize("leaf", [True, False])
+def test_logits_changed_before_the_backward(r, leaf):
+    """Only the gradient of a softmax over all experts reads the logits again; it says so."""
+    x = _logits(40, 24, torch.float32).to(DEV).requires_grad_(True)
+    g = torch.randn(40, 3, device=DEV, generator=torch.Generator(DEV).manual_seed(1))
+    logits = x if leaf else x * 1
+    w, _ = fm.route_tokens(logits, 3, r)
+    (want,) = torch.autograd.grad(w, x, g, retain_graph=True)
+    with torch.no_grad():
+        logits.zero_()
+    if r.score == "softmax" and not r.renormalize:
+        with pytest.raises(RuntimeError, match="modified"):
+            torch.autograd.grad(w, x, g)
+    else:
+        assert torch.equal(torch.autograd.grad(w, x, g)[0], want)
+
+
+def test_logits_are_not_held_for_a_gradient_that_does_not_read_them():
+    x = torch.zeros(1 << 14, 1 << 10, device=DEV, requires_grad=True)  # 64 MiB
+    for r, held in ((RULES[0], False), (RULES[1], False), (RULES[3], True)):
+        before = torch.cuda.memory_allocated()
+        w, _ = fm.route_tokens(x * 1, 2, r)
+        assert (torch.cuda.memory_allocated() - before > 1 << 25) == held
+        assert torch.autograd.grad(w.sum(), x)[0].shape == x.shape
+        del w, _
+
+
+@pytest.mark.parametrize("r", RULES, ids=str)
+@pytest.mark.parametrize("leaf", [True, False])
+def test_a_second_derivative_is_refused_by_every_rule(r, leaf):
+    x = _logits(6, 10, torch.float32).to(DEV).requires_grad_(True)
+    w, _ = fm.route_tokens(x if leaf else x * 1, 3, r)
+    (d,) = torch.autograd.grad(w, x, torch.randn(6, 3, device=DEV), create_graph=True)
+    assert d.requires_grad
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        d.square().sum().backward()
+    g = torch.randn(6, 3, device=DEV, requires_grad=True)
+    with pytest.raises(RuntimeError, match="no gradient of its own"):
+        torch.autograd.grad(w, x, g, create_graph=True)
