@@ -199,7 +199,8 @@ bool good_sandwich(const Sandwich& s) {
          s.post.defined() && good_param(s.post, s.x, false) &&
          (!s.pre.defined() || (good_param(s.pre, s.x, false) && s.pre.scalar_type() == s.post.scalar_type())) &&
          (!s.gate.defined() ||
-          (good_param(s.gate, s.x, true) && s.gate_rows() >= 1 && s.x.size(0) % s.gate_rows() == 0)) &&
+          (good_param(s.gate, s.x, true) &&
+           (s.gate_rows() ? s.x.size(0) % s.gate_rows() == 0 : s.x.size(0) == 0))) &&
          std::isfinite(s.scale) && s.eps >= 0 && s.eps < HUGE_VAL;
 }
 
@@ -267,8 +268,8 @@ class SandwichNorm : public torch::autograd::Function<SandwichNorm> {
     const Tensor ws = empty({bytes}, h, at::kByte);
     check(api.fmoe_sandwich_norm_backward(
               data(gy), gy.defined() ? pitch(gy) : 0, data(gh), gh.defined() ? pitch(gh) : 0, data(x), pitch(x),
-              data(h), data(post), data(pre), code(post.scalar_type()), data(gate),
-              has_gate ? code(gate.scalar_type()) : FMOE_F32, runs, static_cast<const float*>(data(rstd)), T, D,
+              data(h), data(post), data(pre), code(post.scalar_type()),
+              runs ? data(gate) : nullptr, has_gate ? code(gate.scalar_type()) : FMOE_F32, runs, static_cast<const float*>(data(rstd)), T, D,
               code(h.scalar_type()), (float)ctx->saved_data["scale"].toDouble(), data(out[0]), data(out[2]),
               data(out[1]), gy.defined() ? data(out[3]) : nullptr, T ? data(out[4]) : nullptr, data(ws), bytes,
               place.stream),

@@ -71,7 +71,7 @@ def _check_sandwich(x, post_weight, residual, pre_weight, gate, scale, eps) -> N
     if pre_weight is not None and pre_weight.dtype != post_weight.dtype:
         raise TypeError(f"fastmoe_amd: the weights must share a dtype, got {post_weight.dtype} and "
                         f"{pre_weight.dtype}")
-    if gate is not None and gate.dim() == 2 and (gate.shape[0] < 1 or T % gate.shape[0]):
+    if gate is not None and gate.dim() == 2 and (T % gate.shape[0] if gate.shape[0] else T):
         raise ValueError(f"fastmoe_amd: {gate.shape[0]} rows of the gate do not share out {T} rows")
     if not math.isfinite(scale):
         raise ValueError(f"fastmoe_amd: the scale must be finite, got {scale}")

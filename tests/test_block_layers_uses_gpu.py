@@ -56,3 +56,22 @@ def test_a_parameter_used_twice_is_copied_twice():
         block.norm_weight.copy_(rand(64))
     served = block.fp4()
     assert torch.equal(served.post_weight, block.norm_weight) and torch.equal(served.norm_weight, block.norm_weight)
+
+
+@pytest.mark.parametrize("B,T", [(0, 5), (3, 0)])
+def test_an_empty_batch_with_a_gate_for_each_sequence(B, T):
+    D = 64
+    block = fm.SandwichMoEFeedForward(layer(D, 32, 4, 2)).cuda()
+    gate = rand(B, D, dtype=torch.bfloat16).requires_grad_(True)
+    x = rand(B, T, D, dtype=torch.bfloat16).requires_grad_(True)
+    h, y = block(x, gate=gate, next_weight=block.norm_weight)
+    assert h.shape == y.shape == (B, T, D)
+    leaves = [x, gate, block.post_weight, block.norm_weight]
+    for t, g in zip(leaves, torch.autograd.grad([h, y], leaves, [torch.zeros_like(h), torch.zeros_like(y)])):
+        assert g.shape == t.shape and g.dtype == t.dtype and not g.any()
+    many = rand(4, D, dtype=torch.bfloat16)
+    with torch.no_grad():
+        h, y = block.fp4()(x, gate=many[:B], next_weight=block.norm_weight)
+    assert h.shape == y.shape == (B, T, D)
+    with pytest.raises(ValueError, match="gate"):  # no gate for the rows that there are
+        fm.sandwich_norm(rand(6, D), rand(D), rand(6, D), gate=rand(0, D))
