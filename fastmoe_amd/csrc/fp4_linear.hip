@@ -144,7 +144,9 @@ template <typename TX, int KS> __global__ __launch_bounds__(kFewWaves * kWave) v
   const uint8_t* const wp[2] = {a.w + column(lane / 8) * (a.Kp / 2), a.w + column(8 + lane / 8) * (a.Kp / 2)};
   const uint8_t* const sp = a.s + column(lane / 2 % 16) * (a.Kp / kFp4Block);
   const int pieces = (int)((a.Kp + 255) / 256), mine = pieces > part ? (pieces - part + KS - 1) / KS : 0;
-  // Piece j of this wave's.  What lies beyond a column's end is read as its last chunk once more, and meets rows of zeros.
+  const int beyond = (int)(a.Kp / 64) - quad;  // in 64s of K, where a column ends for this lane
+  // Piece j of this wave's.  What lies beyond a column's end is read as its last chunk once more, and meets rows of zeros; its
+  // scale is taken as the smallest: another's might make an infinity of these codes.
   auto ask = [&](uint8_t (*ring)[kPiece], int j) __attribute__((always_inline)) {
     const int64_t p = (int64_t)j * KS + part;
 #pragma unroll
@@ -195,7 +197,8 @@ template <typename TX, int KS> __global__ __launch_bounds__(kFewWaves * kWave) v
 #pragma unroll
     for (int h = 0; h < 2; ++h)
       w[h] = *reinterpret_cast<const u32x4*>(cur[wave] + l16 * 128 + ((quad * 2 + h) ^ swizzle<128>(l16)) * 16);
-    const uint32_t e = *reinterpret_cast<const uint16_t*>(cur[wave] + kCodes + l16 * 8 + quad * 2);
+    uint32_t e = *reinterpret_cast<const uint16_t*>(cur[wave] + kCodes + l16 * 8 + quad * 2);
+    if ((i * KS + part) * 4 >= beyond) e = 0;
     if (i + 2 < mine) ask(old, i + 2);
     const uint8_t* xs = xl + ((i - base) * KS + part) * 512;
 #pragma unroll
