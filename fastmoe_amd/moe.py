@@ -135,17 +135,19 @@ def _hooked(*modules: nn.Module) -> bool:
     return any(getattr(m, hooks, None) for m in modules for hooks in _HOOKS)
 
 
-def _check_layer(layer: nn.Module, kind: type) -> None:
-    """What ``int8`` reads of a layer is all that its call computes."""
+def _check_layer(layer: nn.Module, kind: type, form: str) -> None:
+    """What ``form`` ("int8" or "fp4") reads of a layer is all that its call computes."""
     if not _computes_as(layer, kind):
         raise TypeError(f"fastmoe_amd: {type(layer).__name__} is not a {kind.__name__} with that class's "
-                        "forward; int8() would lose what it adds")
+                        f"forward; {form}() would lose what it adds")
     if _hooked(layer):
-        raise ValueError(f"fastmoe_amd: the {kind.__name__} has hooks, which its 8-bit form would not call")
+        raise ValueError(f"fastmoe_amd: the {kind.__name__} has hooks, which the layer that {form}() makes would "
+                         "not call")
 
 
-def _mlp_parameters(experts: Sequence[nn.Module]):
-    """[(w1, b1, w2, b2), ...] of experts Sequential(Linear, GELU(), Linear); biases may be None."""
+def _mlp_parameters(experts: Sequence[nn.Module], bits: int = 8):
+    """[(w1, b1, w2, b2), ...] of experts Sequential(Linear, GELU(), Linear); biases may be None.  ``bits``: of the
+    operators that are to compute them."""
     out = []
     for e, expert in enumerate(experts):
         parts = list(expert) if _computes_as(expert, nn.Sequential) else []
@@ -154,11 +156,11 @@ def _mlp_parameters(experts: Sequence[nn.Module]):
             raise TypeError(f"fastmoe_amd: expert {e} is not Sequential(Linear, GELU, Linear)")
         if parts[1].approximate != "none":
             raise ValueError(f"fastmoe_amd: expert {e} has a GELU approximation "
-                             f"({parts[1].approximate!r}); the 8-bit operators compute the exact form")
+                             f"({parts[1].approximate!r}); the {bits}-bit operators compute the exact form")
         out.append((parts[0].weight, parts[0].bias, parts[2].weight, parts[2].bias))
         if _hooked(expert, *parts):
-            raise ValueError(f"fastmoe_amd: expert {e} has hooks, which the 8-bit operators would not "
-                             "call")
+            raise ValueError(f"fastmoe_amd: expert {e} has hooks, which the {bits}-bit operators would "
+                             "not call")
     if not out:
         raise ValueError("fastmoe_amd: no experts")
     return out
@@ -448,12 +450,12 @@ class NormedMoEFeedForward(nn.Module):
 
     def int8(self) -> "Int8MoEFeedForward":
         """As :meth:`MoEFeedForward.int8`, the norm included."""
-        _check_layer(self, NormedMoEFeedForward)
+        _check_layer(self, NormedMoEFeedForward, "int8")
         return Int8MoEFeedForward(self.moe, self.norm_weight, self.eps)
 
     def fp4(self) -> "NormedMoEFeedForward":
         """As :meth:`MoEFeedForward.fp4`, behind a copy of the norm."""
-        _check_layer(self, NormedMoEFeedForward)
+        _check_layer(self, NormedMoEFeedForward, "fp4")
         block = NormedMoEFeedForward(self.moe.fp4(), self.eps)
         _copy_parameters(self, block, "norm_weight")
         return block.requires_grad_(False)
@@ -498,7 +500,7 @@ class SandwichMoEFeedForward(nn.Module):
 
     def fp4(self) -> "SandwichMoEFeedForward":
         """This block for serving: a copy with the experts' weights in 4 bits."""
-        _check_layer(self, SandwichMoEFeedForward)
+        _check_layer(self, SandwichMoEFeedForward, "fp4")
         block = SandwichMoEFeedForward(self.moe.fp4(), self.eps, self.scale, self.gate is not None)
         _copy_parameters(self, block, "norm_weight", "post_weight", "gate")
         return block.requires_grad_(False)
@@ -516,8 +518,8 @@ class Fp4MoEFeedForward(_Balanced):
 
     def __init__(self, moe: MoEFeedForward) -> None:
         super().__init__()
-        _check_layer(moe, MoEFeedForward)
-        params = _mlp_parameters(moe.experts)
+        _check_layer(moe, MoEFeedForward, "fp4")
+        params = _mlp_parameters(moe.experts, 4)
         if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
             raise TypeError("fastmoe_amd: the router is not a Linear without hooks")
         if moe.router.weight.dtype not in (torch.bfloat16, torch.float16):
@@ -582,7 +584,7 @@ class Int8MoEFeedForward(_Balanced):
     def __init__(self, moe: MoEFeedForward, norm_weight: Optional[torch.Tensor] = None,
                  eps: float = 1e-6) -> None:
         super().__init__()
-        _check_layer(moe, MoEFeedForward)
+        _check_layer(moe, MoEFeedForward, "int8")
         params = _mlp_parameters(moe.experts)
         if not _computes_as(moe.router, nn.Linear) or _hooked(moe.router):
             raise TypeError("fastmoe_amd: the router is not a Linear without hooks")
