@@ -617,7 +617,8 @@ FMOE_API int fmoe_fp4_linear(const void* d_x, int64_t x_row_stride, int64_t x_ro
                              int64_t num_experts, int64_t N, int64_t K, int64_t rows, void* d_out,
                              int64_t out_row_stride, int out_dtype, void* stream);
 
-/* The tile that fmoe_fp4_linear chooses by size, as 1000 * rows + columns (introspection). */
+/* The tile that fmoe_fp4_linear chooses by rows, experts and N, as 1000 * rows + columns (introspection).  K has no
+ * part in the choice. */
 FMOE_API int64_t fmoe_fp4_linear_tile(int64_t rows, int64_t num_experts, int64_t N, int64_t K);
 
 #ifdef __cplusplus
