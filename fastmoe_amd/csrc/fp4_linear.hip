@@ -526,7 +526,9 @@ __global__ __launch_bounds__(4 * kWave, 2) void k_fp4_tile(Fp4Args a) {
 }
 
 // ---- weights to 4 bits and back ---------------------------------------------------------------------
-// A thread takes the 32 weights of a scale: the smallest power of two with which none of them passes 6.
+// A thread takes the 32 weights of a scale: the smallest power of two with which none of them passes 6.  This is done once, when
+// a layer is made: 64 experts' [2048, 4096] (1.36 GB with their bf16) take 0.96 ms, a launch and two copies for each, and back
+// to bf16 in one launch 0.39 ms.
 template <typename T> __global__ __launch_bounds__(kGroup) void k_to_fp4(const T* x, int64_t stride, int64_t rows,
                                                                          int64_t cols, int64_t blocks, uint8_t* q,
                                                                          uint8_t* s) {
@@ -640,6 +642,9 @@ template <typename TX, int TM, int WN, bool AGAIN> int launch_tile(const char* w
 // CU; each workgroup brings all of its expert's rows, which a split multiplies.  Tiles of 96 rows take over where
 // an expert's rows pass one tile of 16 (8 on the average), unless there are few workgroups even so; 256 columns from where
 // they make more than one workgroup on a CU.
+// The host knows how many rows there are, not whose.  Where one expert has most of them, its tiles of 16 read its weights
+// again: 1024 rows of 256 experts' [2048, 2048] take 119 us evenly, 123 where one has 514 of them and 132 with 769; 512 of
+// 64 experts' [2048, 4096] 64, 71 (260) and 78 (386); 256 of 32 experts' [7168, 2048] 58, 66 (132) and 70 (194).
 enum Variant { k16x128 = 16128, k16x64 = 16064, k16x32 = 16032, k16x16 = 16016, k96x128 = 96128, k96x256 = 96256 };
 Variant pick(int64_t rows, int64_t E, int64_t N) {
   const double per = (double)rows / (double)E;

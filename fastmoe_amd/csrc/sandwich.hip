@@ -237,7 +237,8 @@ struct UnitRows {
 
 // A unit (the threads that hold a row) keeps its parts of the column sums, in registers or, for the longest rows
 // (LDS_SUMS), in LDS, each thread its own: one pass over the four inputs, whatever the number of rows.  HBM bounds it: 12 bytes
-// an element in 16 bits, 4096 x 16384 in 146 us: 5.5 TB/s.
+// an element in 16 bits, 4096 x 16384 in 146 us: 5.5 TB/s.  In fp32, 2048 x 8192 takes 83 us: 4.9 TB/s; rows of 16384 do not fit
+// the registers by 42 a thread, which pass through scratch memory: 2048 of them take 190 us, 4.3 TB/s.
 // WHOLE: units take whole runs, write each one's gate's gradient and keep the sum of scale gate A in LDS.  Where a unit is a
 // wave, the workgroup's four join their parts.
 template <typename T, int THREADS, int VPT, bool WHOLE, bool LDS_SUMS>
