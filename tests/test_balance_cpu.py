@@ -2,6 +2,8 @@
 from __future__ import annotations
 
 import copy
+import datetime
+import os
 import pickle
 
 import pytest
@@ -34,7 +36,9 @@ def plain_gate_and_sort(x, router, top_k, num_experts, *, routing=None, bias=Non
 
 
 def count(rank, store, out):
-    torch.distributed.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2)
+    os.environ["GLOO_SOCKET_IFNAME"] = "lo"  # the host's name need not resolve
+    torch.distributed.init_process_group("gloo", init_method=f"file://{store}", rank=rank, world_size=2,
+                                         timeout=datetime.timedelta(seconds=120))
     layers.gate_and_sort = plain_gate_and_sort  # in this process alone
     moe = make()
     ddp = torch.nn.parallel.DistributedDataParallel(moe, find_unused_parameters=True)  # an expert may have no rows
