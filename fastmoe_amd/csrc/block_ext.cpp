@@ -269,7 +269,8 @@ class SandwichNorm : public torch::autograd::Function<SandwichNorm> {
     check(api.fmoe_sandwich_norm_backward(
               data(gy), gy.defined() ? pitch(gy) : 0, data(gh), gh.defined() ? pitch(gh) : 0, data(x), pitch(x),
               data(h), data(post), data(pre), code(post.scalar_type()),
-              runs ? data(gate) : nullptr, has_gate ? code(gate.scalar_type()) : FMOE_F32, runs, static_cast<const float*>(data(rstd)), T, D,
+              runs ? data(gate) : nullptr, has_gate ? code(gate.scalar_type()) : FMOE_F32, runs,
+              static_cast<const float*>(data(rstd)), T, D,
               code(h.scalar_type()), (float)ctx->saved_data["scale"].toDouble(), data(out[0]), data(out[2]),
               data(out[1]), gy.defined() ? data(out[3]) : nullptr, T ? data(out[4]) : nullptr, data(ws), bytes,
               place.stream),

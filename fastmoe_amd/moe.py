@@ -353,8 +353,8 @@ class MoEFeedForward(_Balanced):
     ``balance=True`` (with a routing) adds ``balance_bias`` to the scores that choose; in training mode the
     layer counts the rows that each expert gets in ``expert_load``, and :meth:`update_balance`, called
     after the optimiser's step, moves the bias against it.  ``expert_load`` is what this process counted (a forward that
-    activation checkpointing runs again counts again), neither a buffer nor part of the layer's state.  Where several processes train copies of the layer, sum it over them first,
-    so that their biases stay alike."""
+    activation checkpointing runs again counts again), neither a buffer nor part of the layer's state.  Where several
+    processes train copies of the layer, sum it over them first, so that their biases stay alike."""
 
     def __init__(self, dim: int, ff_dim: int, num_experts: int, top_k: int,
                  implementation=MoEImplementation.FAST, checkpoint: Optional[str] = None,
